@@ -285,6 +285,98 @@ int qh_lora_silu(void* stream, const float* xa, int split, int m_cols, const uin
                  const int32_t* tab, const int32_t* tok_slot, const float* slot_scale, size_t n, const float* y,
                  size_t ldy, void* mid_bf16);
 
+/* ---- attention of a decode step -------------------------------------------------------------------------------- */
+
+/* Between the in-projection's product and the out-projection's: attn_prep makes queries, keys and values of the product's
+ * partials, the cache keeps keys and values quantised in pages, tree_attn attends over them. All buffers are the
+ * caller's, on the device. */
+
+enum qh_kv_fmt {
+    QH_KV_I8 = 1,  /* code q + 128, q = v / scale rounded to nearest even, scale = max|v| / 127 */
+    QH_KV_E4M3 = 2 /* code: e4m3 (no infinities) of v / scale rounded to nearest even, scale = max|v| / 448 */
+};
+
+/* The KV cache of one layer: `pages` pages of `page` tokens (a power of two from 64 to 1024) of `heads` kv heads of
+ * head_dim (64, 128 or 256) dimensions; slot s is token s % page of page s / page (pages * page < 2^31).
+ * codes u8 [pages][heads][2][page * head_dim] and scales f32 [pages][heads][2][page] (qh_kv_sizes), keys then values, a
+ * scale per vector. In a block of page * head_dim codes, token t's dimension d lies, of keys, at
+ *   (t / 16) * 16 head_dim + (d / 64) * 1024 + (t % 16) * 64 + d % 64,
+ * and of values at (t / 64) * 64 head_dim + d * 64 + (t % 16 / 4) * 16 + (t % 64 / 16) * 4 + t % 4.
+ * Buffers 16-byte aligned; they need no clearing: what was not written is never used. A vector with a value that is not
+ * finite is stored with scale NaN: what attends to it is NaN, as the plain sum would be. */
+typedef struct qh_kv {
+    int32_t fmt; /* enum qh_kv_fmt */
+    int32_t heads;
+    int32_t head_dim;
+    int32_t page;
+    size_t pages;
+    void* codes;
+    float* scales;
+} qh_kv;
+
+int qh_kv_sizes(const qh_kv* kv, size_t* code_bytes, size_t* scale_bytes);
+
+/* k, v bf16 [n][heads][head_dim] quantised into slots[0..n) (int32, distinct; one outside the cache is skipped), and the
+ * slots' keys and values back as bf16 (zeros for a slot outside the cache). Buffers 16-byte aligned. Launch only. */
+int qh_kv_write(void* stream, const qh_kv* kv, const void* k_bf16, const void* v_bf16, const int32_t* slots, size_t n);
+int qh_kv_read(void* stream, const qh_kv* kv, const int32_t* slots, size_t n, void* k_bf16, void* v_bf16);
+
+/* Codes and scales of slot src[i] to slot dst[i], unchanged, for the moves start[b] .. start[b + 1] of each of n_seq
+ * sequences (int32 start [n_seq + 1], n moves in all): after a step that verified a tree, the accepted path's slots
+ * together. A sequence's moves are read before they are written, 64 at a time in order (an ascending path may overlap its
+ * destination); different sequences' moves must not overlap. A move from or to a slot outside the cache is skipped.
+ * Launch only. */
+int qh_kv_move(void* stream, const qh_kv* kv, const int32_t* src, const int32_t* dst, size_t n, const int32_t* start,
+               int n_seq);
+
+/* Rows of the attention in-projection: q_heads heads of head_dim (with `gated`: each followed by its gate's head_dim), then
+ * kv_heads of keys and as many of values. The first `rot` (even, <= head_dim, 0: none) dimensions of queries and keys are
+ * rotated, dimension i with i + rot / 2. */
+typedef struct qh_attn_rows {
+    int32_t q_heads;
+    int32_t kv_heads;
+    int32_t head_dim; /* 64, 128 or 256 */
+    int32_t rot;
+    int32_t gated;
+} qh_attn_rows;
+
+/* The consumer of the in-projection (attn_prep, kernels/qwen.cu:156-202): x f32 [splits][n][rows], the product's
+ * partials. Sums them; norms each head of queries and keys, q_w * q / sqrt(mean(q^2) + eps) (k_w likewise, f32
+ * [head_dim]; NULL: no norm); rotates pair i by pos[t] * inv_freq[i] (int32 positions, f32 [rot / 2]; the angle is
+ * exact: far positions lose nothing). q, gate (NULL unless gated) bf16 [n][q_heads][head_dim]. Keys and values go, with kv,
+ * quantised into slots[0..n) as qh_kv_write's, else as bf16 to k, v [n][kv_heads][head_dim]. Buffers 16-byte aligned.
+ * Launch only. */
+int qh_attn_prep(void* stream, const float* x, int splits, size_t n, const qh_attn_rows* rows, const float* q_w,
+                 const float* k_w, float eps, const float* inv_freq, const int32_t* pos, void* q, void* gate,
+                 const qh_kv* kv, const int32_t* slots, void* k, void* v);
+
+/* The sequences of a step: sequence b has tokens start[b] .. start[b + 1] of the step's n (int32 [n_seq + 1]; up to
+ * max_new <= 64 of one sequence, none is fine), len[b] cached positions before them, and its positions' pages in table[b]
+ * (int32 [n_seq][table_ld]): position p is token p % page of page table[b][p / page]. The step's tokens are in the cache
+ * at len[b], len[b] + 1, .. (attn_prep or kv_write put them there). mask (u64 [n], or NULL): bit j of token i's: it sees
+ * the sequence's j-th token of this step (a tree: itself and its ancestors); NULL: itself and those before it. All
+ * tokens see the cached positions. A token that sees nothing gets zeros. n_seq <= 1024. A sequence whose numbers do not
+ * fit (start not ascending or past n, len past the table) or that reads a page outside the cache gets NaN. */
+typedef struct qh_tree {
+    size_t n;
+    int32_t n_seq;
+    int32_t max_new;
+    const int32_t* start;
+    const int32_t* len;
+    const int32_t* table;
+    size_t table_ld;
+    const uint64_t* mask;
+} qh_tree;
+
+/* out bf16 [n][q_heads * head_dim] = softmax(scale * q . k) v over what each token sees, with `gate` (bf16, NULL: none)
+ * times sigmoid(gate): the out-projection's input. q, gate bf16 [n][q_heads][head_dim], q_heads a multiple of the cache's
+ * heads (up to 64 times); kv head j serves q_heads / heads query heads in a row. Codes and queries are multiplied
+ * exactly, softmax sums are f32, probabilities are rounded to f16 for their products. 16-byte aligned. It uses the
+ * context's scratch (calls on one context must not run concurrently on two streams) and gives the same bits each time.
+ * Launch only. */
+int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
+                 float scale, const void* gate, void* out);
+
 /* ---- graph capture --------------------------------------------------------------------------------------------- */
 
 /* Replaces the capture and replay inside Graphs::run (src/cuda/core.rs:1151-1192); the graph cache around it (keys,

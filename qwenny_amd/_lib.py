@@ -31,6 +31,27 @@ class LoraC(ctypes.Structure):
                 ("rank", ctypes.c_int32), ("tab", P), ("tok_slot", P), ("slot_scale", P)]
 
 
+class KvC(ctypes.Structure):
+    """qh_kv (a layer's paged, quantised KV cache)"""
+
+    _fields_ = [("fmt", ctypes.c_int32), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("pages", S), ("codes", P), ("scales", P)]
+
+
+class AttnRowsC(ctypes.Structure):
+    """qh_attn_rows (the rows of the attention in-projection)"""
+
+    _fields_ = [("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("rot", ctypes.c_int32), ("gated", ctypes.c_int32)]
+
+
+class TreeC(ctypes.Structure):
+    """qh_tree (the sequences of a step)"""
+
+    _fields_ = [("n", S), ("n_seq", ctypes.c_int32), ("max_new", ctypes.c_int32), ("start", P), ("len", P), ("table", P),
+                ("table_ld", S), ("mask", P)]
+
+
 # name -> (restype, argtypes); every symbol include/qwenny_hip.h declares
 SIGNATURES = {
     "qh_last_error": (ctypes.c_char_p, []),
@@ -71,6 +92,13 @@ SIGNATURES = {
     "qh_gemm": (I, [P, P, P, P, S, S, P, S, P, I, P, I]),
     "qh_gemm_noalloc": (I, [P, P, P, P, S, S, P, S, P, I, P, I]),
     "qh_gemm_lora": (I, [P, P, P, P, S, S, P, I, I, ctypes.POINTER(LoraC)]),
+    "qh_kv_sizes": (I, [ctypes.POINTER(KvC), ctypes.POINTER(S), ctypes.POINTER(S)]),
+    "qh_kv_write": (I, [P, ctypes.POINTER(KvC), P, P, P, S]),
+    "qh_kv_read": (I, [P, ctypes.POINTER(KvC), P, S, P, P]),
+    "qh_kv_move": (I, [P, ctypes.POINTER(KvC), P, P, S, P, I]),
+    "qh_attn_prep": (I, [P, P, I, S, ctypes.POINTER(AttnRowsC), P, P, ctypes.c_float, P, P, P, P, ctypes.POINTER(KvC), P,
+                         P, P]),
+    "qh_tree_attn": (I, [P, P, P, I, ctypes.POINTER(KvC), ctypes.POINTER(TreeC), ctypes.c_float, P, P]),
     "qh_put_block": (I, [P, P, P, ctypes.POINTER(QuantC), P, S, P]),
 }
 

@@ -13,7 +13,7 @@ from enum import IntEnum
 
 import numpy as np
 
-from ._lib import MatDesc, QuantC, check, lib
+from ._lib import AttnRowsC, KvC, MatDesc, QuantC, TreeC, check, lib
 
 P = ctypes.c_void_p
 
@@ -188,6 +188,13 @@ class Gemm:
         lc = LoraC(_ptr(xa), split, m_cols, _ptr(b), rank, _ptr(tab), _ptr(tok_slot), _ptr(slot_scale))
         return check(lib().qh_gemm_lora(self._ctx, _stream(stream), w._m, _ptr(x), ldx, n, _ptr(y), int(epi),
                                         int(whole), ctypes.byref(lc)))
+
+    def tree_attn(self, stream, q, q_heads, kv, step, out, gate=None, scale=None):
+        """Attention of a step's tokens over the cache `kv` (KvCache): q bf16 [n][q_heads][head_dim], `step` a TreeStep,
+        out bf16 [n][q_heads * head_dim], times sigmoid(gate) where a gate (bf16, as q) is given; scale: head_dim ** -0.5
+        by default."""
+        s = kv.head_dim ** -0.5 if scale is None else scale
+        check(lib().qh_tree_attn(self._ctx, _stream(stream), _ptr(q), q_heads, kv.c, step.c, s, _ptr(gate), _ptr(out)))
 
     def put_block(self, stream, m, q, zeros, block, rows):
         """Write stored rows `rows` (16) of `q` as the 16-row block `block` of a matrix from Mat.marlin_rows, counting
@@ -420,6 +427,99 @@ def lora_silu(stream, xa, split, m_cols, b_f16, rank, rows, tab, tok_slot, slot_
     src/cuda/qwen/lora.rs:184-187): mid [n][rows / 2] bf16; all device buffers."""
     check(lib().qh_lora_silu(_stream(stream), _ptr(xa), split, m_cols, _ptr(b_f16), rank, rows, _ptr(tab),
                              _ptr(tok_slot), _ptr(slot_scale), n, _ptr(y), ldy or rows, _ptr(mid)))
+
+
+class KvFmt(IntEnum):
+    """Codes of the KV cache: int8, or the 8-bit float of 4 exponent and 3 mantissa bits; a f32 scale per vector."""
+
+    I8 = 1
+    E4M3 = 2
+
+
+class KvCache:
+    """A layer's paged, quantised KV cache over the caller's device buffers (qh_kv): codes u8
+    [pages][heads][2][page * head_dim], scales f32 [pages][heads][2][page]. Slot s is token s % page of page s / page."""
+
+    def __init__(self, fmt, heads, head_dim, page, codes, scales, pages=None):
+        if pages is None:
+            pages = codes.numel() // max(1, heads * 2 * page * head_dim)
+        self.fmt, self.heads, self.head_dim, self.page, self.pages = KvFmt(fmt), heads, head_dim, page, pages
+        self.codes, self.scales = codes, scales
+        self.c = KvC(int(fmt), heads, head_dim, page, pages, _ptr(codes), _ptr(scales))
+        for have, need in zip((codes, scales), KvCache.sizes(fmt, heads, head_dim, page, pages)):
+            if hasattr(have, "numel") and have.numel() * have.element_size() < need:
+                raise ValueError(f"a cache buffer of {have.numel() * have.element_size()} bytes, {need} needed")
+
+    @staticmethod
+    def sizes(fmt, heads, head_dim, page, pages):
+        """(code, scale) bytes of a cache."""
+        a, b = ctypes.c_size_t(), ctypes.c_size_t()
+        check(lib().qh_kv_sizes(KvC(int(fmt), heads, head_dim, page, pages, None, None), ctypes.byref(a), ctypes.byref(b)))
+        return a.value, b.value
+
+    @classmethod
+    def new(cls, fmt, heads, head_dim, page, pages, device="cuda:0"):
+        """A cache in buffers of its own (torch tensors)."""
+        import torch
+
+        cls.sizes(fmt, heads, head_dim, page, pages)
+        return cls(fmt, heads, head_dim, page,
+                   torch.empty((pages, heads, 2, page * head_dim), dtype=torch.uint8, device=device),
+                   torch.empty((pages, heads, 2, page), dtype=torch.float32, device=device))
+
+
+class TreeStep:
+    """The sequences of a step (qh_tree), all device tensors: start int32 [n_seq + 1] (tokens start[b] .. start[b + 1] are
+    sequence b's), len int32 [n_seq] (cached positions before them), table int32 [n_seq][pages] (positions' pages), mask
+    int64 / uint64 [n] (bit j: sees the sequence's j-th token of this step) or None (a chain); no sequence has more than
+    max_new tokens."""
+
+    def __init__(self, n, start, len, table, max_new, mask=None):
+        n_seq, width = table.shape
+        if table.stride(1) != 1 and width > 1:
+            raise ValueError("table: rows must be contiguous")
+        if start.numel() != n_seq + 1 or len.numel() != n_seq or (mask is not None and mask.numel() < n):
+            raise ValueError(f"{n_seq} tables, {start.numel()} starts, {len.numel()} lengths")
+        self._held = (start, len, table, mask)
+        ld = table.stride(0) if n_seq > 1 else width
+        if ld != width:
+            raise ValueError("table: rows must follow one another")
+        self.c = TreeC(n, n_seq, max_new, _ptr(start), _ptr(len), _ptr(table), ld, _ptr(mask))
+
+
+class AttnRows:
+    """The rows of the attention in-projection (qh_attn_rows): q_heads heads of head_dim, each followed by its gate where
+    `gated`, then kv_heads of keys and of values; `rot` dimensions of queries and keys are rotated."""
+
+    def __init__(self, q_heads, kv_heads, head_dim, rot=0, gated=False):
+        self.q_heads, self.kv_heads, self.head_dim, self.rot, self.gated = q_heads, kv_heads, head_dim, rot, bool(gated)
+        self.rows = (q_heads * (2 if gated else 1) + 2 * kv_heads) * head_dim
+        self.c = AttnRowsC(q_heads, kv_heads, head_dim, rot, int(bool(gated)))
+
+
+def attn_prep(stream, x, splits, n, rows, q_w, k_w, inv_freq, pos, q, gate=None, kv=None, slots=None, k=None, v=None,
+              eps=1e-6):
+    """The consumer of the attention in-projection (kernels/qwen.cu:156-202): its partials x [splits][n][rows] summed,
+    queries and keys normed per head (q_w, k_w f32 or None) and rotated to positions pos by pos * inv_freq; q and gate
+    bf16 [n][q_heads][head_dim]; keys and values into `slots` of the cache `kv`, or as bf16 to k, v."""
+    check(lib().qh_attn_prep(_stream(stream), _ptr(x), splits, n, rows.c, _ptr(q_w), _ptr(k_w), eps, _ptr(inv_freq), _ptr(pos),
+                             _ptr(q), _ptr(gate), None if kv is None else kv.c, _ptr(slots), _ptr(k), _ptr(v)))
+
+
+def kv_write(stream, kv, k, v, slots, n):
+    """k, v bf16 [n][heads][head_dim] quantised into the cache's slots (int32 [n], distinct)."""
+    check(lib().qh_kv_write(_stream(stream), kv.c, _ptr(k), _ptr(v), _ptr(slots), n))
+
+
+def kv_read(stream, kv, slots, n, k, v):
+    """The keys and values of slots (int32 [n]) as bf16 [n][heads][head_dim]."""
+    check(lib().qh_kv_read(_stream(stream), kv.c, _ptr(slots), n, _ptr(k), _ptr(v)))
+
+
+def kv_move(stream, kv, src, dst, start, n_seq, n=None):
+    """Codes and scales of slots src to slots dst (int32 [n]), sequence b's moves start[b] .. start[b + 1] read before they
+    are written: an accepted path's slots put together."""
+    check(lib().qh_kv_move(_stream(stream), kv.c, _ptr(src), _ptr(dst), src.numel() if n is None else n, _ptr(start), n_seq))
 
 
 def pack_dense_bf16(w_bf16, order):

@@ -39,6 +39,8 @@ struct qh_ctx {
 };
 
 int qh::ctx_device(const qh_ctx* ctx) { return ctx->device; }
+int qh::ctx_cus(const qh_ctx* ctx) { return ctx->cus; }
+void* qh::ctx_partials(const qh_ctx* ctx) { return ctx->sk_scratch; }
 
 // The context's own launch scratch.
 static Scratch ctx_scratch(const qh_ctx* ctx) {

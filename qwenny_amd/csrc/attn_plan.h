@@ -1,0 +1,59 @@
+// How a step's attention is shared among workgroups (tree_attn.hip), in plain C++: the kernels and a host test make the same
+// plan from the same arrays. Whatever the arrays hold, every index made here lies in its buffer.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+namespace qh {
+
+constexpr int KV_TILE = 64;          // tokens of a tile; pages are a multiple of it
+constexpr int GROUP_TILES = 4;       // tiles of a group, a workgroup's smallest part: one for each of its waves
+constexpr int TREE_MAX_SEQS = 1024;  // sequences of a step
+constexpr int TREE_MAX_NEW = 64;     // tokens of one sequence in a step: a mask is 64 bits
+
+struct TreeArrays {
+    const int32_t* start;  // [n_seq + 1]
+    const int32_t* len;    // [n_seq]
+    int64_t table_ld;      // pages of a table's row
+    int page_shift;
+    int n, n_seq, max_new;
+    int group;  // query heads of a kv head
+};
+
+// A sequence's part of the step: tokens first .. first + news, `old` positions before them, `total` in all; its rows (token,
+// query head of the kv head) in `chunks` of some rows each, its positions in `groups`. `bad`: its numbers do not fit, it gets
+// NaN.
+struct Seq {
+    int first, news, old, total, chunks, groups;
+    bool bad;
+};
+
+constexpr Seq sequence(const TreeArrays& a, int b, int rows) {
+    const int s0 = a.start[b], s1 = a.start[b + 1], len = a.len[b];
+    const int64_t cap = a.table_ld << a.page_shift;
+    const int first = s0 < 0 ? 0 : s0 > a.n ? a.n : s0;
+    const int64_t asked = (int64_t)s1 - s0;
+    int64_t news = (int64_t)s1 - first;
+    news = news < 0 ? 0 : news;
+    news = news > a.n - first ? a.n - first : news;
+    news = news > a.max_new ? a.max_new : news;
+    news = news > cap ? cap : news;
+    int64_t old = len < 0 ? 0 : len;
+    old = old > cap - news ? cap - news : old;
+    const int chunks = ((int)news * a.group + rows - 1) / rows;
+    const int total = (int)(old + news);
+    return Seq{first, (int)news, (int)old, total, chunks,
+               chunks ? (total + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES) : 0,
+               first != s0 || news != asked || old != len};
+}
+
+// `all` groups in a row (sequence by sequence, kv head by kv head, chunk by chunk) in equal parts for `used` <= all
+// workgroups: the first group of workgroup w, the workgroup of group `at`.
+constexpr int first_group(int w, int all, int used) { return (int)((int64_t)w * all / used); }
+constexpr int group_owner(int at, int all, int used) { return (int)((((int64_t)at + 1) * used - 1) / all); }
+
+// Where workgroup w keeps its partial result of the unit (sequence, kv head, chunk) whose groups begin at u0: it has at most
+// two, the unit that its part begins in and the one that it ends in.
+constexpr int partial_slot(int w, int u0, int all, int used) { return 2 * w + (first_group(w, all, used) < u0 ? 1 : 0); }
+
+}  // namespace qh

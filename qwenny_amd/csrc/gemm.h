@@ -16,6 +16,10 @@ int gemm_with_scratch(qh_ctx* ctx, void* stream, const qh_mat* w, const void* x,
 // The device a context was opened on.
 int ctx_device(const qh_ctx* ctx);
 
+// Its compute units, and its scratch for partial results (PF_SK_PART_BYTES, holding nothing between calls).
+int ctx_cus(const qh_ctx* ctx);
+void* ctx_partials(const qh_ctx* ctx);
+
 // Set-up of the allocation-free entry point on `device` (current on the calling thread): resolves the device address
 // of its static scratch once per device and clears it. Called by qh_open.
 int noalloc_init(int device);

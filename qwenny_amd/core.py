@@ -66,11 +66,24 @@ def _ptr(t):
     return int(t)
 
 
+def _current_stream():
+    """torch's current stream of the current device, as an address. The raw query where torch has it: 0.2 us a call,
+    torch.cuda.current_stream() 2.9 us, as much as a launch."""
+    global _current_stream
+    import torch
+
+    torch.cuda.init()
+    raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+    if raw is None or device is None:
+        _current_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+    else:
+        _current_stream = lambda: raw(device())  # noqa: E731
+    return _current_stream()
+
+
 def _stream(s):
     if s is None:
-        import torch
-
-        return torch.cuda.current_stream().cuda_stream
+        return _current_stream()
     if hasattr(s, "cuda_stream"):
         return s.cuda_stream
     return int(s)

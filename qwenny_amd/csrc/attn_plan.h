@@ -7,7 +7,7 @@
 namespace qh {
 
 constexpr int KV_TILE = 64;          // tokens of a tile; pages are a multiple of it
-constexpr int GROUP_TILES = 4;       // tiles of a group, a workgroup's smallest part: one for each of its waves
+constexpr int GROUP_TILES = 8;       // tiles of a group, a workgroup's smallest part: one for each of its waves
 constexpr int TREE_MAX_SEQS = 1024;  // sequences of a step
 constexpr int TREE_MAX_NEW = 64;     // tokens of one sequence in a step: a mask is 64 bits
 
@@ -49,11 +49,32 @@ constexpr Seq sequence(const TreeArrays& a, int b, int rows) {
 
 // `all` groups in a row (sequence by sequence, kv head by kv head, chunk by chunk) in equal parts for `used` <= all
 // workgroups: the first group of workgroup w, the workgroup of group `at`.
-constexpr int first_group(int w, int all, int used) { return (int)((int64_t)w * all / used); }
-constexpr int group_owner(int at, int all, int used) { return (int)((((int64_t)at + 1) * used - 1) / all); }
+// (w all / used and (used (at + 1) - 1) / all, without 64-bit divisions: used <= 1024)
+constexpr int first_group(int w, int all, int used) { return w * (all / used) + w * (all % used) / used; }
+constexpr int group_owner(int at, int all, int used) {
+    int w = (int)((float)at * ((float)used / (float)all));  // off by one at most
+    w = w < 0 ? 0 : w >= used ? used - 1 : w;
+    while (w > 0 && first_group(w, all, used) > at) w--;
+    while (w + 1 < used && first_group(w + 1, all, used) <= at) w++;
+    return w;
+}
 
 // Where workgroup w keeps its partial result of the unit (sequence, kv head, chunk) whose groups begin at u0: it has at most
 // two, the unit that its part begins in and the one that it ends in.
 constexpr int partial_slot(int w, int u0, int all, int used) { return 2 * w + (first_group(w, all, used) < u0 ? 1 : 0); }
+
+// How `parts` partial results of a unit are summed: up to MAX_CLUSTER by the last of all to arrive; more in `of` clusters of
+// `step` neighbours (the last has what is left), then the clusters' sums. The cluster of part i.
+constexpr int MAX_CLUSTER = 32;  // (its square is more than the workgroups of a launch)
+struct Cluster {
+    int first, size, step, of;
+};
+constexpr Cluster cluster(int i, int parts) {
+    int step = parts;
+    if (parts > 16)
+        for (step = 5; step * step < parts;) step++;
+    const int first = i / step * step;
+    return Cluster{first, step < parts - first ? step : parts - first, step, (parts + step - 1) / step};
+}
 
 }  // namespace qh

@@ -28,30 +28,28 @@ struct Seq {
     bool bad;
 };
 
+constexpr int group_count(int total) { return (int)(((unsigned)total + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES)); }
+
+// (`rows`: a power of two)
 constexpr Seq sequence(const TreeArrays& a, int b, int rows) {
     const int s0 = a.start[b], s1 = a.start[b + 1], len = a.len[b];
-    const int64_t cap = a.table_ld << a.page_shift;
-    const int first = s0 < 0 ? 0 : s0 > a.n ? a.n : s0;
-    const int64_t asked = (int64_t)s1 - s0;
-    int64_t news = (int64_t)s1 - first;
-    news = news < 0 ? 0 : news;
-    news = news > a.n - first ? a.n - first : news;
-    news = news > a.max_new ? a.max_new : news;
-    news = news > cap ? cap : news;
-    int64_t old = len < 0 ? 0 : len;
-    old = old > cap - news ? cap - news : old;
-    const int chunks = ((int)news * a.group + rows - 1) / rows;
-    const int total = (int)(old + news);
-    return Seq{first, (int)news, (int)old, total, chunks,
-               chunks ? (total + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES) : 0,
-               first != s0 || news != asked || old != len};
+    const int cap = (int)(a.table_ld << a.page_shift);
+    const int first = s0 < 0 ? 0 : s0 > a.n ? a.n : s0, last = s1 < first ? first : s1 > a.n ? a.n : s1;
+    const int most = a.max_new < cap ? a.max_new : cap, news = last - first < most ? last - first : most;
+    const int old = len < 0 ? 0 : len > cap - news ? cap - news : len, total = old + news;
+    const int chunks = (news * a.group + rows - 1) >> __builtin_ctz(rows);
+    return Seq{first, news, old, total, chunks, chunks ? group_count(total) : 0,
+               first != s0 || last != s1 || news != last - first || old != len};
 }
 
 // `all` groups in a row (sequence by sequence, kv head by kv head, chunk by chunk) in equal parts for `used` <= all
 // workgroups: the first group of workgroup w, the workgroup of group `at`.
 // (w all / used and (used (at + 1) - 1) / all, without 64-bit divisions: used <= 1024)
-constexpr int first_group(int w, int all, int used) { return w * (all / used) + w * (all % used) / used; }
+constexpr int first_group(int w, int all, int used) {
+    return used == all ? w : w * (all / used) + w * (all % used) / used;
+}
 constexpr int group_owner(int at, int all, int used) {
+    if (used == all) return at;
     int w = (int)((float)at * ((float)used / (float)all));  // off by one at most
     w = w < 0 ? 0 : w >= used ? used - 1 : w;
     while (w > 0 && first_group(w, all, used) > at) w--;

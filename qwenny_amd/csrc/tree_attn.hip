@@ -37,7 +37,7 @@ constexpr int BUF_RSRC_WORD3 = 0x00020000;
 constexpr int CPOL_SC1 = 16;
 
 // Workgroups of a CU: what a kernel's registers leave room for.
-constexpr int wgs_per_cu(int d) { return d == 64 ? 2 : 1; }
+constexpr int wgs_per_cu(int d, int r) { return d == 64 && r == 1 ? 2 : 1; }
 
 struct Args {
     const __bf16* q;     // [n][heads][D]
@@ -49,7 +49,7 @@ struct Args {
     const uint64_t* mask;  // [n], or null: a chain
     float scale;           // softmax scale * log2(e)
     uint32_t group_inv;    // 2^20 / group rounded up: (r * group_inv) >> 20 is r / group for the rows r < 64 group <= 4096
-    int32_t row_tiles;     // log2 of a chunk's tiles of 16 rows; the waves share them, and then the cache's tiles
+    int32_t row_tiles;     // log2 of a chunk's tiles of 16 rows
     int32_t fuse;          // partial results are summed by the last workgroup to arrive, else by join_kernel
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
@@ -60,18 +60,25 @@ struct Args {
 // The compiler moves nothing across: left free it converts a whole tile's codes ahead of its products and spills.
 #define HOLD() __builtin_amdgcn_sched_barrier(0)
 
-// eight codes as exact f16 operands
+// A barrier for what the workgroup's waves wrote to LDS; loads and stores to memory stay in flight over it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Eight codes as exact f16 operands: e4m3 by its conversion; an int8 code c = q + 128 is put into f16's low bits as it is,
+// the subnormal number c 2^-24, which the matrix instructions multiply exactly. The products' sums then hold 2^-24 (q + 128):
+// the 128 is taken off by the scores' first value, and from the outputs at the end, beside a sum of the probabilities.
+// (Against codes made whole numbers of, one instruction a pair instead of two.)
 template <int FMT>
 __device__ __forceinline__ h8 operands(uint32_t a, uint32_t b) {
     h2 p[4];
     if constexpr (FMT == QH_KV_I8) {
-        // 0x6400 | code = 1024 + code, then - 1152 (codes are q + 128)
-        const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-        const uint32_t m = 0x64646464u;
-        p[0] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(m, a, 0x04010400u)) + off;
-        p[1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(m, a, 0x04030402u)) + off;
-        p[2] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(m, b, 0x04010400u)) + off;
-        p[3] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(m, b, 0x04030402u)) + off;
+        p[0] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0, a, 0x0c010c00u));
+        p[1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0, a, 0x0c030c02u));
+        p[2] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0, b, 0x0c010c00u));
+        p[3] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0, b, 0x0c030c02u));
     } else {
         p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
         p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
@@ -79,6 +86,22 @@ __device__ __forceinline__ h8 operands(uint32_t a, uint32_t b) {
         p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
     }
     return h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+}
+constexpr int code_exp(int fmt) { return fmt == QH_KV_I8 ? 24 : 0; }  // operands are 2^-this of the codes' values
+
+// A lane's neighbour's value in the wave (DPP): CTRL of quad_perm, row_half_mirror, row_mirror, row_shr, row_bcast.
+template <int CTRL, int ROWS = 15>
+__device__ __forceinline__ int dpp(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 15, false);
+}
+// f over the N = 4, 8 or 16 neighbouring lanes that share a row of queries
+template <int N, class F>
+__device__ __forceinline__ int over_lanes(int v, F&& f) {
+    v = f(v, dpp<0xb1>(v, v));
+    v = f(v, dpp<0x4e>(v, v));
+    if (N > 4) v = f(v, dpp<0x141>(v, v));
+    if (N > 8) v = f(v, dpp<0x140>(v, v));
+    return v;
 }
 
 // the largest / sum over the four lanes that hold one row (lanes l, l ^ 16, l ^ 32, l ^ 48)
@@ -95,27 +118,33 @@ __device__ __forceinline__ float row_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float wave_max(float v) {
+    v = __int_as_float(over_lanes<16>(__float_as_int(v), [](int x, int y) { return __float_as_int(fmaxf(__int_as_float(x), __int_as_float(y))); }));
+    return row_max(v);
+}
 
-// What a workgroup holds in LDS. The queries and the tiles' scales are done with when its waves' results are joined there.
-template <int D>
+__device__ __forceinline__ float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
+// What a workgroup of 16 R rows holds in LDS.
+template <int D, int R>
 struct Shared {
-    static constexpr int C = D / 64, DT = D / 16, HALF = D == 256 ? 8 : DT;
     int32_t base[TREE_MAX_SEQS];  // of each sequence: its first group,
     int32_t who[TREE_MAX_SEQS];   // first token | tokens << 20,
     int32_t old[TREE_MAX_SEQS];   // positions before them | (its numbers do not fit) << 31
     int32_t wave_sum[WAVES];
     int32_t last;
-    float factor[16 * WAVES];
-    f2 wave_ml[WAVES][16];
+    float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
+    f4 largest[16 * R][WAVES / 4];        // each wave's largest score of the row,
+    f4 largest_scale[WAVES / 4];          // and largest scale of its values
+    f4 sums[16 * R][WAVES / 2];           // each wave's sum of the row's probabilities, and of their roundings
+    h8 q[R][D / 64][2][64];
+    float tile_scale[WAVES][2][KV_TILE];
     union {
+        h8 p[WAVES][R][2][64];  // probabilities of each wave's tile
+        f4 half[R][WAVES / 2][64];
         struct {
-            h8 q[WAVES][C][2][64];
-            float tile_scale[WAVES][2][KV_TILE];
-        } in;
-        f4 joined[WAVES][HALF][64];
-        struct {
-            f2 ml[FAN][16];
             float weight[FAN][16];
             f2 row[16];  // the joined maximum and sum
         } parts;
@@ -124,8 +153,8 @@ struct Shared {
 
 // The sequences' places in LDS; returns the number of their groups. Up to 64 sequences each wave makes the whole list for
 // itself, more are shared by the workgroup's threads.
-template <int D>
-__device__ __forceinline__ int plan(const Args& a, Shared<D>& sh) {
+template <int D, int R>
+__device__ __forceinline__ int plan(const Args& a, Shared<D, R>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool few = a.t.n_seq <= 64;
     int before = 0;
@@ -134,25 +163,27 @@ __device__ __forceinline__ int plan(const Args& a, Shared<D>& sh) {
         int v = 0;
         Seq s = {};
         if (b < a.t.n_seq) {
-            s = sequence(a.t, b, 16 << a.row_tiles);
+            s = sequence(a.t, b, 16 * R);
             v = a.kv.heads * s.chunks * s.groups;
         }
         int run = v;  // inclusive over the wave
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(run, o);
-            if (lane >= o) run += up;
-        }
+        run += dpp<0x111>(0, run);
+        run += dpp<0x112>(0, run);
+        run += dpp<0x114>(0, run);
+        run += dpp<0x118>(0, run);
+        run += dpp<0x142, 10>(0, run);
+        run += dpp<0x143, 12>(0, run);
         int sum = __builtin_amdgcn_readlane(run, 63);
         run += before - v;
         if (!few) {
             if (lane == 0) sh.wave_sum[wave] = sum;
-            __syncthreads();
+            lds_barrier();
             sum = 0;
             for (int w = 0; w < WAVES; w++) {
                 if (w < wave) run += sh.wave_sum[w];
                 sum += sh.wave_sum[w];
             }
-            __syncthreads();
+            lds_barrier();
         }
         if (b < a.t.n_seq) {
             sh.base[b] = run;
@@ -161,8 +192,16 @@ __device__ __forceinline__ int plan(const Args& a, Shared<D>& sh) {
         }
         before += sum;
     }
-    if (!few) __syncthreads();
+    if (!few) lds_barrier();
     return __builtin_amdgcn_readfirstlane(before);
+}
+
+// x / y of numbers that all lanes have alike, where the quotient is below 2^20
+__device__ __forceinline__ int divide(int x, int y) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)y));  // off by one at most
+    q -= q * y > x ? 1 : 0;
+    q += x - q * y >= y ? 1 : 0;
+    return __builtin_amdgcn_readfirstlane(q);
 }
 
 // The sequence that group `at` lies in: the last with base <= at (empty ones share their successor's base).
@@ -180,7 +219,7 @@ __device__ __forceinline__ b4 load_gate(const Args& a, size_t at) { return a.gat
 
 // A row's output: four of its dimensions, divided by the sum and gated.
 __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float total, b4 gate) {
-    v *= total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    v *= total > 0.0f || total != total ? __builtin_amdgcn_rcpf(total) : 0.0f;
     if (a.gate) {
 #pragma unroll
         for (int u = 0; u < 4; u++) v[u] *= sigmoid((float)gate[u]);
@@ -191,70 +230,50 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
 // `count` partial results of one unit, those of workgroups w0, w0 + step, .., summed relative to their largest maximum in
 // that order: into the outputs (`out`), or back into the first one's place. (Chunks of 16 rows.)
 template <int D, class Row>
-__device__ __forceinline__ void join_parts(const Args& a, Shared<D>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
+__device__ __forceinline__ void join_parts(const Args& a, Shared<D, 1>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
                                            int count, int live, bool out, Row&& row_of) {
-    constexpr int V = D / 4, ITEMS = (16 * V + THREADS - 1) / THREADS, DEEP = 16 / ITEMS;
+    constexpr int V = D / 4, DEEP = 16;
+    static_assert(THREADS == 16 * FAN);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // what follows from it is made here, not kept in registers over the whole kernel
     auto slot = [&](int i) { return i == 0 ? first_slot : 2 * (w0 + i * step); };
-    f4 sum[ITEMS], in[DEEP][ITEMS];
-    auto load = [&](int i0) {
+    const int row = tid / FAN, part = tid % FAN;  // whose maximum and sum the thread takes
+    f2 ml = {-INFINITY, 0.0f};
+    if (part < count)
+        ml = __builtin_bit_cast(
+            f2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, a.ml_at + ((uint32_t)slot(part) * 16 + row) * 8, 0, CPOL_SC1));
+    f4 in[DEEP];
+    auto load = [&](int e, int i0) {
 #pragma unroll
         for (int k = 0; k < DEEP; k++)
-#pragma unroll
-            for (int j = 0; j < ITEMS; j++) {
-                const int e = j * THREADS + tid;
-                if (i0 + k < count && e < live * V)
-                    in[k][j] = __builtin_bit_cast(
-                        f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (uint32_t)slot(i0 + k) * (16 * D * 4) + e * 16, 0, CPOL_SC1));
-            }
+            if (i0 + k < count && e < live * V)
+                in[k] = __builtin_bit_cast(
+                    f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (uint32_t)slot(i0 + k) * (16 * D * 4) + e * 16, 0, CPOL_SC1));
     };
-    __syncthreads();
-    for (int e = tid; e < count * 16; e += THREADS)
-        sh.parts.ml[e >> 4][e & 15] = __builtin_bit_cast(
-            f2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, a.ml_at + ((uint32_t)slot(e >> 4) * 16 + (e & 15)) * 8, 0, CPOL_SC1));
-    load(0);
-    b4 gate[ITEMS];
-    size_t at[ITEMS];
+    load(tid, 0);
+    float best = ml.x;
 #pragma unroll
-    for (int j = 0; j < ITEMS; j++) {
-        const int e = j * THREADS + tid, r = min(e / V, live - 1);
-        at[j] = row_of(r) + e % V * 4;
-        if (out) gate[j] = load_gate(a, at[j]);
-        sum[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    __syncthreads();
-    if (tid < live) {
-        float best = -INFINITY, total = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < count; i++) best = fmaxf(best, sh.parts.ml[i][tid].x);
-#pragma unroll 4
-        for (int i = 0; i < count; i++) {
-            const f2 v = sh.parts.ml[i][tid];
-            const float by = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - best);
-            total += v.x == -INFINITY ? v.y : v.y * by;  // (without a maximum: 0 or NaN)
-            sh.parts.weight[i][tid] = by;
+    for (int o = 1; o < FAN; o <<= 1) best = fmaxf(best, __shfl_xor(best, o));
+    const float weight = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - best);
+    float total = ml.x == -INFINITY ? ml.y : ml.y * weight;  // (without a maximum: 0 or NaN)
+#pragma unroll
+    for (int o = 1; o < FAN; o <<= 1) total += __shfl_xor(total, o);
+    sh.parts.weight[part][row] = weight;
+    if (part == 0) sh.parts.row[row] = f2{best, total};
+    lds_barrier();
+    for (int e = tid; e < live * V; e += THREADS) {
+        const size_t at = row_of(e / V) + e % V * 4;
+        const b4 gate = out ? load_gate(a, at) : b4{};
+        f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < count; i0 += DEEP) {
+            if (e != tid || i0) load(e, i0);
+#pragma unroll
+            for (int k = 0; k < DEEP; k++)
+                if (i0 + k < count) sum += sh.parts.weight[i0 + k][e / V] * in[k];
         }
-        sh.parts.row[tid] = f2{best, total};
-    }
-    __syncthreads();
-    for (int i0 = 0; i0 < count; i0 += DEEP) {
-#pragma unroll
-        for (int k = 0; k < DEEP; k++)
-#pragma unroll
-            for (int j = 0; j < ITEMS; j++) {
-                const int e = j * THREADS + tid;
-                if (i0 + k < count && e < live * V) sum[j] += sh.parts.weight[i0 + k][e / V] * in[k][j];
-            }
-        if (i0 + DEEP < count) load(i0 + DEEP);
-    }
-#pragma unroll
-    for (int j = 0; j < ITEMS; j++) {
-        const int e = j * THREADS + tid;
-        if (e >= live * V) continue;
-        if (out) put_out(a, at[j], sum[j], sh.parts.row[e / V].y, gate[j]);
+        if (out) put_out(a, at, sum, sh.parts.row[e / V].y, gate);
         else
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, sum[j]), rsrc, (uint32_t)first_slot * (16 * D * 4) + e * 16, 0,
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, sum), rsrc, (uint32_t)first_slot * (16 * D * 4) + e * 16, 0,
                                                    CPOL_SC1);
     }
     if (!out && tid < live)
@@ -265,30 +284,42 @@ __device__ __forceinline__ void join_parts(const Args& a, Shared<D>& sh, __amdgp
 // Whether this workgroup is the last of `of` to come here since the counter was zero; it sets it back to zero.
 __device__ __forceinline__ bool last_of(uint32_t* counter, int of, int32_t* flag) {
     __builtin_amdgcn_s_waitcnt(0);  // this wave's partial has been performed
-    __syncthreads();
+    lds_barrier();
     if (threadIdx.x == 0) {
         const bool l = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(of - 1);
         if (l) (void)__hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = l;
     }
-    __syncthreads();
+    lds_barrier();
     return *flag != 0;
 }
 
-// The work is a row of groups: for each sequence, kv head and chunk of rows, the cache in groups of 8 x 64 tokens. The
+// The work is a row of groups: for each sequence, kv head and chunk of 16 R rows, the cache in groups of 8 x 64 tokens. The
 // workgroups share it in equal parts, across the borders of sequences; consecutive parts on one XCD, whose L2 then serves
-// the chunks that read the same cache. In a workgroup a wave has 16 of the chunk's rows, and takes turns at the cache's
-// tiles with the other waves of these rows; each keeps its own softmax, and they are joined in LDS. What covers a
-// sequence's whole cache is written out, the rest as partial results: at most one at the start of a workgroup's part and
-// one at its end. They are summed in their order by join_kernel, or (`fuse`) here: each workgroup writes its own
-// (device-coherent stores) and counts itself, and the last to arrive sums them; from more than 16 on in two steps,
-// clusters of neighbours and then the clusters' sums. No workgroup waits for another.
-template <int D, int FMT>
-__global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D)) void tree_attn_kernel(const Args a) {
-    constexpr int C = D / 64, DT = D / 16, HALF = Shared<D>::HALF;
-    __shared__ Shared<D> sh;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int all = plan<D>(a, sh), used = min((int)gridDim.x, all);
+// the chunks that read the same cache. In a group each of the eight waves makes the scores of one tile for all rows; the
+// waves agree on the rows' largest scores, put their probabilities into LDS, and each then multiplies all eight tiles' by
+// its own share of the values' dimensions. So a code is read and converted once for all rows, a wave's part of the outputs
+// is small, and there is nothing to join over the waves but the sums. (Each wave with whole rows and tiles of its own, joined
+// over LDS, took 12.0 us against 10.3 for a short sequence, 45 against 33 for 64 drafted tokens at 8,150.) Keys are read a
+// group ahead, values too or while the scores are made.
+// What covers a sequence's whole cache is written out, the rest as partial results: at most one at the start of a
+// workgroup's part and one at its end. They are summed in their order by join_kernel, or (`fuse`) here: each workgroup
+// writes its own (device-coherent stores) and counts itself, and the last to arrive sums them; from more than 16 on in two
+// steps, clusters of neighbours and then the clusters' sums. No workgroup waits for another.
+template <int D, int FMT, int R>
+__global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kernel(const Args a) {
+    // a wave's share of the values: SL sixteenths of the dimensions, of VT of a group's tiles
+    constexpr int C = D / 64, DT = D / 16, ROWS = 16 * R, SPLIT = DT < WAVES ? WAVES / DT : 1, SL = DT * SPLIT / WAVES, VT = WAVES / SPLIT;
+    constexpr int CHAINS = R == 1 ? 2 : 1;  // sums of an output, so that products need not wait for one another
+    constexpr bool EARLY = R == 1 || D < 256;  // registers for a group's values beside its keys
+    constexpr uint32_t NONE = ~0u;
+    __shared__ Shared<D, R> sh;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // all lines of the arguments are fetched at once: each is a trip to memory when first touched
+    const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
+    static_assert(sizeof(Args) > 128);
+    const int all = plan<D, R>(a, sh), used = min((int)gridDim.x, all);
     if (blockIdx.x == 0 && !a.fuse)
         for (int i = threadIdx.x; i <= a.t.n_seq; i += THREADS) a.plan[i] = i < a.t.n_seq ? sh.base[i] : all;
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
@@ -298,30 +329,32 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D)) void tree_attn_kernel(c
     // (what all lanes have alike is said to be so where it comes through LDS or a division: addresses are then scalar)
     const int lo = __builtin_amdgcn_readfirstlane(first_group(w, all, used));
     const int hi = __builtin_amdgcn_readfirstlane(first_group(w + 1, all, used));
-    const int page = 1 << a.kv.page_shift, rows = 16 << a.row_tiles;
-    const int turns = WAVES >> a.row_tiles, turn = wave & (turns - 1), rt = wave >> (3 - a.row_tiles);
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int)PF_SK_PART_BYTES, BUF_RSRC_WORD3);
     for (int at = lo; at < hi;) {
+        // (said anew in each turn, so that nothing that follows is kept in registers across them: most workgroups take one)
+        int tid = threadIdx.x, page_shift = a.kv.page_shift;
+        asm volatile("" : "+v"(tid), "+s"(page_shift));
+        const int lane = tid & 63, col = lane & 15, g = lane >> 4, page_tiles = 1 << (page_shift - 6);
         const int b = find_seq(sh.base, a.t.n_seq, at);
         const int who = __builtin_amdgcn_readfirstlane(sh.who[b]), was = __builtin_amdgcn_readfirstlane(sh.old[b]);
         const int past = at - __builtin_amdgcn_readfirstlane(sh.base[b]);
         const int first = who & 0xfffff, news = who >> 20, old = was & 0x7fffffff, total = old + news;
-        const int chunks = (news * a.t.group + rows - 1) >> (4 + a.row_tiles);
-        const int groups = (total + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES);
-        const int unit = __builtin_amdgcn_readfirstlane(past / groups), g0 = past - unit * groups;
+        const int chunks = (news * a.t.group + ROWS - 1) / ROWS;
+        const int groups = group_count(total), unit = divide(past, groups), g0 = past - unit * groups;
         const int g1 = min(groups, g0 + hi - at);
-        const int head = __builtin_amdgcn_readfirstlane(unit / chunks), row0 = (unit - head * chunks) * rows;
-        const int live = min(rows, news * a.t.group - row0);
-        const int tiles = (total + KV_TILE - 1) / KV_TILE;
-        const int t_first = g0 * GROUP_TILES + turn, t_end = rt * 16 < live ? min(tiles, g1 * GROUP_TILES) : 0;
+        const int head = chunks == 1 ? unit : divide(unit, chunks), row0 = (unit - head * chunks) * ROWS;
+        const int live = min(ROWS, news * a.t.group - row0);
+        const int t_end = min((total + KV_TILE - 1) / KV_TILE, g1 * GROUP_TILES);
 
-        // pages of the wave's tiles, 64 at a time: lane l has its l-th tile's
-        int32_t pages = 0;
-        auto load_pages = [&](int t) {
-            const int mine = t + lane * turns;
-            if (mine < t_end) pages = a.table[(size_t)b * a.t.table_ld + ((mine * KV_TILE) >> a.kv.page_shift)];
+        // where tiles lie, 64 at a time: lane l has the l-th's place in the cache (of its keys) in tiles
+        uint32_t places = 0;
+        auto load_places = [&](int t) {
+            const int mine = min(t + lane, t_end - 1);
+            const int32_t pg = a.table[(size_t)b * a.t.table_ld + (mine >> (page_shift - 6))];
+            places = (((uint32_t)pg * a.kv.heads + head) * 2 << (page_shift - 6)) + (mine & (page_tiles - 1));
+            if (pg < 0 || ((int64_t)pg << page_shift) >= a.kv.slots) places = NONE;
         };
-        load_pages(t_first);
+        load_places(g0 * GROUP_TILES);
 
         auto node_of = [&](int r) { return (int)((uint32_t)r * a.group_inv >> 20); };  // r / group
         // first element of a row's query, gate and output
@@ -331,275 +364,343 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D)) void tree_attn_kernel(c
         };
         // the queries: a thread has 16 dimensions of a row
         constexpr int PER_ROW = D / 16, PASS = THREADS / PER_ROW;
-        const int q_row = threadIdx.x / PER_ROW, q_part = threadIdx.x % PER_ROW;
+        const int q_row = tid / PER_ROW, q_part = tid % PER_ROW;
         b8 raw[2];
         auto load_query = [&](int r) {
             const __bf16* const qp = a.q + row_at(min(r, live - 1)) + q_part * 16;
             raw[0] = *(const b8*)qp, raw[1] = *(const b8*)(qp + 8);
         };
         load_query(q_row);
-        const int my_node = node_of(row0 + min(rt * 16 + col, live - 1));
-        // of its sequence's tokens of this step
-        const uint64_t sees = (a.mask ? a.mask[first + my_node] : ~0ull >> (63 - my_node)) & ~0ull >> (64 - news);
+        uint64_t sees[R];  // of its sequence's tokens of this step
+#pragma unroll
+        for (int rt = 0; rt < R; rt++) {
+            const int node = node_of(row0 + min(rt * 16 + col, live - 1));
+            sees[rt] = (a.mask ? a.mask[first + node] : ~0ull >> (63 - node)) & ~0ull >> (64 - news);
+        }
 
-        u4 kc[4][C], vc[DT];
+        u4 kc[4][C], vc[VT][SL];
         float sk, sv;
-        const uint8_t* block = a.kv.codes;  // a tile's keys; its values lie one block on
-        const float* scales = a.kv.scales;
-        bool none = false;
-        // a page that the cache has not gives NaN
-        auto find = [&](int t, int i) {
-            int64_t pg = __builtin_amdgcn_readlane(pages, i & 63);
-            none = pg < 0 || (pg << a.kv.page_shift) >= a.kv.slots;
-            if (none) pg = 0;
-            const int in = (t * KV_TILE) & (page - 1);
-            block = a.kv.codes + kv_block<D>(a.kv, pg, head, 0) + (size_t)in * D;
-            scales = a.kv.scales + kv_scale(a.kv, pg, head, 0) + in;
-        };
-        const uint32_t k_lane = col * 64 + g * 16;
-        auto load_keys = [&](int t) {  // keys and scales (lane l: token l's)
+        const uint32_t in_tile = col * 64 + g * 16;
+        // the wave's tile's keys and scales (lane l: token l's); a page that the cache has not gives NaN
+        auto load_keys = [&](int gr) {
+            const int t = gr * GROUP_TILES + wave, i = min(t, t_end - 1) - g0 * GROUP_TILES;
+            const uint32_t at = __builtin_amdgcn_readlane(places, i & 63);
+            const bool none = at == NONE;
+            const uint32_t place = none ? 0 : at;
+            const uint8_t* const k = a.kv.codes + (size_t)place * (KV_TILE * D);
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int sub = 0; sub < 4; sub++) kc[sub][c] = *(const u4*)(block + sub * 16 * D + c * 1024 + k_lane);
-            sk = none ? NAN : scales[lane];
-            sv = t * KV_TILE + lane < total ? scales[page + lane] : 0.0f;
+                for (int sub = 0; sub < 4; sub++) kc[sub][c] = *(const u4*)(k + sub * 16 * D + c * 1024 + in_tile);
+            const float* const sc = a.kv.scales + (size_t)place * KV_TILE;
+            sk = none ? NAN : sc[lane];
+            sv = t * KV_TILE + lane < total ? sc[page_tiles * KV_TILE + lane] : 0.0f;
         };
-        auto load_values = [&]() {
-            const uint8_t* const vp = block + ((size_t)D << a.kv.page_shift);
+        const int slice = (wave % (WAVES / SPLIT)) * SL, v_tile = wave / (WAVES / SPLIT) * VT;
+        auto load_values = [&](int gr) {
 #pragma unroll
-            for (int i = 0; i < DT; i++) vc[i] = *(const u4*)(vp + i * 1024 + k_lane);
+            for (int v = 0; v < VT; v++) {
+                const int i = min(gr * GROUP_TILES + v_tile + v, t_end - 1) - g0 * GROUP_TILES;
+                const uint32_t at = __builtin_amdgcn_readlane(places, i & 63);
+                const uint8_t* const p = a.kv.codes + (size_t)((at == NONE ? 0 : at) + page_tiles) * (KV_TILE * D) + slice * 1024;
+#pragma unroll
+                for (int i = 0; i < SL; i++) vc[v][i] = *(const u4*)(p + i * 1024 + in_tile);
+            }
         };
-        if (t_first < t_end) {
-            find(t_first, 0);
-            load_keys(t_first);
-        }
+        load_keys(g0);
+        if (EARLY) load_values(g0);
 
         // the queries, scaled by a power of two into f16's range (the factor goes to the scores)
         for (int r = q_row;;) {
-            float top = 0.0f, odd = 0.0f;
+            // bf16 with the sign taken off compares as a whole number; from 0x7f80 on it is not finite
+            typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+            us2 m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, __builtin_bit_cast(u4, raw[i >> 2])[i & 3] & 0x7fff7fffu));
+            const int top = over_lanes<PER_ROW>(max(m.x, m.y), [](int x, int y) { return max(x, y); });
+            const int e = top < 0x7f80 ? __builtin_amdgcn_frexp_expf(__uint_as_float((uint32_t)top << 16)) - 15 : 0;
+            float sum = 0.0f;
+            h8 q[2];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float v = (float)raw[i >> 3][i & 7];
-                top = fmaxf(top, fabsf(v));
-                odd += v * 0.0f;  // NaN where v is not finite
+                q[i >> 3][i & 7] = (_Float16)__builtin_ldexpf((float)raw[i >> 3][i & 7], -e);
+                if (FMT == QH_KV_I8) sum += (float)q[i >> 3][i & 7];
             }
-#pragma unroll
-            for (int o = 1; o < PER_ROW; o <<= 1) top = fmaxf(top, __shfl_xor(top, o)), odd += __shfl_xor(odd, o);
-            const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-            if (r < rows) {
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    h8 q;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) q[i] = (_Float16)__builtin_ldexpf((float)raw[k][i], -e);
-                    sh.in.q[r >> 4][q_part >> 2][k][(q_part & 3) * 16 + (r & 15)] = q;
+            if (FMT == QH_KV_I8)
+                sum = __int_as_float(over_lanes<PER_ROW>(__float_as_int(sum), [](int x, int y) {
+                    return __float_as_int(__int_as_float(x) + __int_as_float(y));
+                }));
+            if (r < ROWS) {
+                sh.q[r >> 4][q_part >> 2][0][(q_part & 3) * 16 + (r & 15)] = q[0];
+                sh.q[r >> 4][q_part >> 2][1][(q_part & 3) * 16 + (r & 15)] = q[1];
+                if (q_part == 0) {
+                    sh.factor[r] = was < 0 || top >= 0x7f80
+                                       ? NAN
+                                       : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
+                    sh.start[r] = -0x1p-17f * sum;
                 }
-                if (q_part == 0) sh.factor[r] = fmaxf(__builtin_ldexpf(a.scale, e), 1e-37f) + odd + (was < 0 ? NAN : 0.0f);
             }
             r += PASS;
-            if (r - q_row >= rows) break;
+            if (r - q_row >= ROWS) break;
             load_query(r);
         }
-        if (t_first < t_end) load_values();
-        __syncthreads();
-        const float factor = sh.factor[rt * 16 + col];
-        float top = -INFINITY, sum = 0.0f;
-        f4 o[DT];
+        lds_barrier();
+        float factor[R], top[R], sum[R], rounded[R];  // rounded: the sum of the probabilities as they are multiplied
+        f4 o[R][SL][CHAINS];
         float ref = 0x1p-126f;  // the values' scales are taken relative to this power of two: probabilities fit f16
 #pragma unroll
-        for (int i = 0; i < DT; i++) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-
-        for (int t = t_first, it = 1; t < t_end; t += turns, it++) {
-            const int t0 = t * KV_TILE;
-            // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
-            f4 x[4];
+        for (int rt = 0; rt < R; rt++) {
+            factor[rt] = sh.factor[rt * 16 + col];
+            top[rt] = -INFINITY, sum[rt] = rounded[rt] = 0.0f;
 #pragma unroll
-            for (int sub = 0; sub < 4; sub++) x[sub] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < SL; i++)
+#pragma unroll
+                for (int k = 0; k < CHAINS; k++) o[rt][i][k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        for (int gr = g0; gr < g1; gr++) {
+            const int t0 = (gr * GROUP_TILES + wave) * KV_TILE;
+            const bool more = gr + 1 < g1;
+            // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
+            f4 x[R][4];
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) {
+                const float start = FMT == QH_KV_I8 ? sh.start[rt * 16 + col] : 0.0f;
+#pragma unroll
+                for (int sub = 0; sub < 4; sub++) x[rt][sub] = f4{start, start, start, start};
+            }
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const h8 q0 = sh.in.q[rt][c][0][lane], q1 = sh.in.q[rt][c][1][lane];
 #pragma unroll
-                for (int sub = 0; sub < 4; sub++) {
-                    const h8 k0 = operands<FMT>(kc[sub][c].x, kc[sub][c].y), k1 = operands<FMT>(kc[sub][c].z, kc[sub][c].w);
-                    x[sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q0, x[sub], 0, 0, 0);
-                    x[sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q1, x[sub], 0, 0, 0);
+                for (int k = 0; k < 2; k++) {
+                    h8 q[R], codes[4];
+#pragma unroll
+                    for (int rt = 0; rt < R; rt++) q[rt] = sh.q[rt][c][k][lane];
+#pragma unroll
+                    for (int sub = 0; sub < 4; sub++) codes[sub] = operands<FMT>(kc[sub][c][2 * k], kc[sub][c][2 * k + 1]);
+#pragma unroll
+                    for (int rt = 0; rt < R; rt++)
+#pragma unroll
+                        for (int sub = 0; sub < 4; sub++)
+                            x[rt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[sub], q[rt], x[rt][sub], 0, 0, 0);
                 }
                 HOLD();
             }
+            if (!EARLY) load_values(gr);
+
+            // the scores' and the values' scales, as the lanes need them
+            float(&ts)[2][KV_TILE] = sh.tile_scale[wave];
+            ts[0][lane] = sk;
+            ts[1][lane] = sv;
+            float most = 0.0f;
+            if (__any(sv > ref && sv < INFINITY)) most = wave_max(sv < INFINITY ? sv : 0.0f);
+            __builtin_amdgcn_wave_barrier();
+            const bool whole = t0 + KV_TILE <= old;  // every row sees every token
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) {
+                uint64_t seen = 0;  // bit i: the row sees token t0 + i
+                if (!whole) {
+                    const int node = t0 - old;  // above -64
+                    seen = node >= 64 ? 0 : node >= 0 ? sees[rt] >> node : sees[rt] << -node | ((1ull << -node) - 1);
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int sub = 0; sub < 4; sub++) {
+                    x[rt][sub] *= *(const f4*)&ts[0][sub * 16 + g * 4];
+                    if (!whole) {
+                        const uint32_t bits = (uint32_t)(seen >> (sub * 16 + g * 4));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[rt][sub][i] = bits & (1u << i) ? x[rt][sub][i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[rt][sub][i]);
+                }
+                mx = row_max(mx);
+                if (g == 0) ((float*)sh.largest[rt * 16 + col])[wave] = mx;
+            }
+            if (lane == 0) ((float*)sh.largest_scale)[wave] = most;
+            HOLD();
+            lds_barrier();
 
             // the values' scales relative to ref; ref grows to the largest finite one's power of two
+            f4 lg = sh.largest_scale[0], lg2 = sh.largest_scale[1];
+            most = fmaxf(fmaxf(fmaxf(lg.x, lg.y), fmaxf(lg.z, lg.w)), fmaxf(fmaxf(lg2.x, lg2.y), fmaxf(lg2.z, lg2.w)));
             float grow = 1.0f;
-            if (__any(sv > ref && sv < INFINITY)) {
-                float m = sv < INFINITY ? sv : 0.0f;
-                for (int of = 32; of; of >>= 1) m = fmaxf(m, __shfl_xor(m, of));
-                const float next = __builtin_ldexpf(1.0f, min(__builtin_amdgcn_frexp_expf(m), 127));
-                grow = ref * (1.0f / next);
-                ref = next;
+            if (__any(most > ref)) {
+                const int e = min(__builtin_amdgcn_frexp_expf(most), 127);
+                grow = __builtin_ldexpf(ref, -e);
+                ref = __builtin_ldexpf(1.0f, e);
             }
-            float(&ts)[2][KV_TILE] = sh.in.tile_scale[wave];
-            ts[0][lane] = sk;
-            ts[1][lane] = sv * (1.0f / ref);
-            const bool more = t + turns < t_end;
+            const float inv_ref = __builtin_amdgcn_rcpf(ref);  // (exact: a power of two)
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) {
+                lg = sh.largest[rt * 16 + col][0], lg2 = sh.largest[rt * 16 + col][1];
+                const float next = fmaxf(top[rt], fmaxf(fmaxf(fmaxf(lg.x, lg.y), fmaxf(lg.z, lg.w)),
+                                                        fmaxf(fmaxf(lg2.x, lg2.y), fmaxf(lg2.z, lg2.w))));
+                // the maximum is followed only where it has grown by more than 2^8 (the sums and f16 hold that)
+                float by = grow;
+                if (__any((next - top[rt]) * factor[rt] > 8.0f)) {
+                    const float al = next > top[rt] ? __builtin_amdgcn_exp2f((top[rt] - next) * factor[rt]) : 1.0f;
+                    sum[rt] *= al;
+                    top[rt] = next;
+                    by *= al;
+                }
+                if (gr != g0 && __any(by != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < SL; i++)
+#pragma unroll
+                        for (int k = 0; k < CHAINS; k++) o[rt][i][k] *= by;
+                    rounded[rt] *= by;
+                }
+                const float off = top[rt] == -INFINITY ? 0.0f : top[rt];
+                h8 p[2];
+#pragma unroll
+                for (int sub = 0; sub < 4; sub++) {
+                    const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4] * inv_ref;
+                    float pv[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float pr = __builtin_amdgcn_exp2f((x[rt][sub][i] - off) * factor[rt]);
+                        pv[i] = pr * vs[i];
+                        if (!whole) pv[i] = x[rt][sub][i] == -INFINITY ? 0.0f : pv[i];
+                        sum[rt] += pr;
+                    }
+                    const h2 a0 = __builtin_convertvector((f2{pv[0], pv[1]}), h2);
+                    const h2 a1 = __builtin_convertvector((f2{pv[2], pv[3]}), h2);
+                    if (FMT == QH_KV_I8) {
+                        const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+                        rounded[rt] = __builtin_amdgcn_fdot2(a0, one, rounded[rt], false);
+                        rounded[rt] = __builtin_amdgcn_fdot2(a1, one, rounded[rt], false);
+                    }
+                    h8& to = p[sub >> 1];
+                    const int k = (sub & 1) * 4;
+                    to[k] = a0.x, to[k + 1] = a0.y, to[k + 2] = a1.x, to[k + 3] = a1.y;
+                }
+                sh.p[wave][rt][0][lane] = p[0];
+                sh.p[wave][rt][1][lane] = p[1];
+                HOLD();
+            }
             if (more) {
-                if ((it & 63) == 0) load_pages(t + turns);
-                find(t + turns, it);
-                load_keys(t + turns);
+                const int i = (gr + 1 - g0) & 7;
+                if (i == 0) load_places((gr + 1) * GROUP_TILES);
+                load_keys(gr + 1);
             }
-            HOLD();
-            __builtin_amdgcn_wave_barrier();
+            lds_barrier();
 
-            h8 p[2];
-            const bool whole = t0 + KV_TILE <= old;  // every row sees every token
-            uint64_t seen = 0;                       // bit i: the row sees token t0 + i
-            if (!whole) {
-                const int node = t0 - old;  // above -64
-                seen = node >= 64 ? 0 : node >= 0 ? sees >> node : sees << -node | ((1ull << -node) - 1);
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int sub = 0; sub < 4; sub++) {
-                x[sub] *= *(const f4*)&ts[0][sub * 16 + g * 4];
-                if (!whole) {
-                    const uint32_t bits = (uint32_t)(seen >> (sub * 16 + g * 4));
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[sub][i] = bits & (1u << i) ? x[sub][i] : -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[sub][i]);
-            }
-            // the maximum is followed only where it has grown by more than 2^8 (the sums and f16 hold that)
-            const float next = fmaxf(top, row_max(mx));
-            float by = grow;
-            if (__any((next - top) * factor > 8.0f)) {
-                const float al = next > top ? __builtin_amdgcn_exp2f((top - next) * factor) : 1.0f;
-                sum *= al;
-                top = next;
-                by *= al;
-            }
-            if (t != t_first && __any(by != 1.0f))
-#pragma unroll
-                for (int i = 0; i < DT; i++) o[i] *= by;
-            const float off = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int sub = 0; sub < 4; sub++) {
-                const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4];
-                float pv[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float pr = __builtin_amdgcn_exp2f((x[sub][i] - off) * factor);
-                    pv[i] = pr * vs[i];
-                    if (!whole) pv[i] = x[sub][i] == -INFINITY ? 0.0f : pv[i];
-                    sum += pr;
-                }
-                const h2 a0 = __builtin_convertvector((f2{pv[0], pv[1]}), h2);
-                const h2 a1 = __builtin_convertvector((f2{pv[2], pv[3]}), h2);
-                h8& to = p[sub >> 1];
-                const int k = (sub & 1) * 4;
-                to[k] = a0.x, to[k + 1] = a0.y, to[k + 2] = a1.x, to[k + 3] = a1.y;
-            }
-            HOLD();
-            if (t0 + KV_TILE > total) {  // codes that no token of this sequence wrote may be anything: none are multiplied
-                u4 keep;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int have = total - (t0 + k * 16 + g * 4);
-                    keep[k] = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * have)) - 1;
-                }
-#pragma unroll
-                for (int i = 0; i < DT; i++) vc[i] &= keep;
-            }
             // o^T += v^T p^T: the k index of both operands runs over tokens 16 w + 4 g + j, as the scores lie
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const h8 v0 = operands<FMT>(vc[i].x, vc[i].y), v1 = operands<FMT>(vc[i].z, vc[i].w);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[0], o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[1], o[i], 0, 0, 0);
-                if (i % 4 == 3) HOLD();
+            for (int v = 0; v < VT; v++) {
+                const int t = gr * GROUP_TILES + v_tile + v;
+                if (t < t_end) {
+                    if ((t + 1) * KV_TILE > total) {  // codes that no token of this sequence wrote may be anything
+                        u4 keep;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int have = total - (t * KV_TILE + k * 16 + g * 4);
+                            keep[k] = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+                        }
+#pragma unroll
+                        for (int i = 0; i < SL; i++) vc[v][i] &= keep;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        h8 codes[SL];
+#pragma unroll
+                        for (int i = 0; i < SL; i++) codes[i] = operands<FMT>(vc[v][i][2 * k], vc[v][i][2 * k + 1]);
+#pragma unroll
+                        for (int rt = 0; rt < R; rt++) {
+                            const h8 p = sh.p[v_tile + v][rt][k][lane];
+#pragma unroll
+                            for (int i = 0; i < SL; i++)
+                                o[rt][i][k % CHAINS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[i], p, o[rt][i][k % CHAINS], 0, 0, 0);
+                        }
+                    }
+                }
             }
-            if (more) load_values();
+            if (EARLY && more) load_values(gr + 1);
         }
 
-        // the waves' results joined, and written out or as a partial result
+        // the waves' sums joined, and the outputs written, or a partial result
         const bool direct = g0 == 0 && g1 == groups;
         const int slot = 2 * w + (at != lo);
-        {
-            int el = lane;
-            asm volatile("" : "+v"(el));  // as in join_parts
-            const int col = el & 15, g = el >> 4, r = rt * 16 + col;
-            const bool mine = r < live;
-            const size_t out_at = row_at(min(r, live - 1));
-            const float l = row_sum(sum), m = top == -INFINITY ? -INFINITY : top * factor;
-            float best = m, total_sum = l, by = ref;
-            auto put = [&](int i, f4 v, b4 gate) {
-                const int d = i * 16 + g * 4;
-                if (direct) put_out(a, out_at + d, v, total_sum, gate);
-                else
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rsrc, (uint32_t)((slot * rows + r) * D + d) * 4, 0,
-                                                           CPOL_SC1);
-            };
-            if (turns > 1) {
-                if (g == 0) sh.wave_ml[wave][col] = f2{m, l};
-                __syncthreads();
-                f2 ml[WAVES];
 #pragma unroll
-                for (int k = 0; k < WAVES; k++) ml[k] = sh.wave_ml[(wave & -turns) + (k & (turns - 1))][col];
-                best = -INFINITY, total_sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < WAVES; k++) best = fmaxf(best, ml[k].x);
-#pragma unroll
-                for (int k = 0; k < WAVES; k++)  // (without a maximum: 0 or NaN)
-                    if (k < turns) total_sum += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * __builtin_amdgcn_exp2f(ml[k].x - best);
-                by *= m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - best);
-#pragma unroll
-                for (int h = 0; h < DT / HALF; h++) {
-                    if (h) __syncthreads();
-#pragma unroll
-                    for (int i = 0; i < HALF; i++)
-                        if (mine) sh.joined[wave][i][el] = m == -INFINITY ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o[h * HALF + i] * by;
-                    __syncthreads();
-                    if (mine)
-                        for (int i = turn; i < HALF; i += turns) {
-                            const b4 gate = direct ? load_gate(a, out_at + (h * HALF + i) * 16 + g * 4) : b4{};
-                            f4 v = {0.0f, 0.0f, 0.0f, 0.0f}, u[WAVES];
-#pragma unroll
-                            for (int k = 0; k < WAVES; k++) u[k] = sh.joined[(wave & -turns) + (k & (turns - 1))][i][el];
-#pragma unroll
-                            for (int k = 0; k < WAVES; k++) v += k < turns ? u[k] : f4{0.0f, 0.0f, 0.0f, 0.0f};
-                            put(h * HALF + i, v, gate);
-                        }
-                }
-            } else if (mine) {
-#pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    const b4 gate = direct ? load_gate(a, out_at + i * 16 + g * 4) : b4{};
-                    put(i, m == -INFINITY ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o[i] * by, gate);
-                }
-            }
-            if (!direct && turn == 0 && g == 0 && mine)
-                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, (f2{best, total_sum})), rsrc,
-                                                      a.ml_at + (uint32_t)(slot * rows + r) * 8, 0, CPOL_SC1);
+        for (int rt = 0; rt < R; rt++) {
+            const f2 s = {row_sum(sum[rt]), FMT == QH_KV_I8 ? row_sum(rounded[rt]) : 0.0f};
+            if (g == 0) ((f2*)sh.sums[rt * 16 + col])[wave] = s;
         }
-        if (!direct && a.fuse) {
-            const int u0 = at - g0, w0 = group_owner(u0, all, used), parts = group_owner(u0 + groups - 1, all, used) - w0 + 1;
-            const Cluster k = cluster(w - w0, parts);
-            const int kw = w0 + k.first, k_slot = partial_slot(kw, u0, all, used);
-            // the cluster's parts, then the clusters' sums; the last of either to arrive goes on
-            int from = kw, first_slot = k_slot, step = 1, count = k.size;
-            uint32_t* counter = a.count + k_slot;
-            for (bool out = k.of == 1;;) {
-                if (count > 1) {
-                    if (!last_of(counter, count, &sh.last)) break;
-                    join_parts<D>(a, sh, rsrc, first_slot, from, step, count, live, out, row_at);
-                }
-                if (out) break;
-                from = w0, first_slot = partial_slot(w0, u0, all, used), step = k.step, count = k.of;
-                counter = a.count + 2 * gridDim.x + w0;
-                out = true;
+        b4 gate[R][SL];
+        if (direct)
+#pragma unroll
+            for (int rt = 0; rt < R; rt++)
+#pragma unroll
+                for (int i = 0; i < SL; i++) gate[rt][i] = load_gate(a, row_at(min(rt * 16 + col, live - 1)) + (slice + i) * 16 + g * 4);
+        lds_barrier();
+#pragma unroll
+        for (int rt = 0; rt < R; rt++) {
+            f4 s = sh.sums[rt * 16 + col][0];
+#pragma unroll
+            for (int k = 1; k < WAVES / 2; k++) s += sh.sums[rt * 16 + col][k];
+            sum[rt] = s.x + s.z;
+            const float back = -128.0f * (s.y + s.w);
+#pragma unroll
+            for (int i = 0; i < SL; i++) {
+                f4 v = o[rt][i][0];
+                if (CHAINS > 1) v += o[rt][i][CHAINS - 1];
+                if (FMT == QH_KV_I8) v = v * 0x1p24f + back / SPLIT;
+                o[rt][i][0] = v * ref;
             }
         }
-        __syncthreads();
+        if (SPLIT > 1) {  // two waves have the same dimensions, of different tiles
+            if (wave >= WAVES / SPLIT)
+#pragma unroll
+                for (int rt = 0; rt < R; rt++) sh.half[rt][wave - WAVES / 2][lane] = o[rt][0][0];
+            lds_barrier();
+            if (wave < WAVES / SPLIT)
+#pragma unroll
+                for (int rt = 0; rt < R; rt++) o[rt][0][0] += sh.half[rt][wave][lane];
+        }
+        if (SPLIT == 1 || wave < WAVES / SPLIT)
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) {
+                const int r = rt * 16 + col;
+                if (r >= live) continue;
+                if (direct) {
+#pragma unroll
+                    for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt], gate[rt][i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < SL; i++)
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, o[rt][i][0]), rsrc,
+                                                               (uint32_t)((slot * ROWS + r) * D + (slice + i) * 16 + g * 4) * 4, 0, CPOL_SC1);
+                    if (wave == 0 && g == 0)
+                        __builtin_amdgcn_raw_buffer_store_b64(
+                            __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * factor[rt], sum[rt]})), rsrc,
+                            a.ml_at + (uint32_t)(slot * ROWS + r) * 8, 0, CPOL_SC1);
+                }
+            }
+        if constexpr (R == 1) {
+            if (!direct && a.fuse) {
+                const int u0 = at - g0, w0 = group_owner(u0, all, used), parts = group_owner(u0 + groups - 1, all, used) - w0 + 1;
+                const Cluster k = cluster(w - w0, parts);
+                const int kw = w0 + k.first, k_slot = partial_slot(kw, u0, all, used);
+                // the cluster's parts, then the clusters' sums; the last of either to arrive goes on
+                int from = kw, first_slot = k_slot, step = 1, count = k.size;
+                uint32_t* counter = a.count + k_slot;
+                for (bool out = k.of == 1;;) {
+                    if (count > 1) {
+                        if (!last_of(counter, count, &sh.last)) break;
+                        join_parts<D>(a, sh, rsrc, first_slot, from, step, count, live, out, row_at);
+                    }
+                    if (out) break;
+                    from = w0, first_slot = partial_slot(w0, u0, all, used), step = k.step, count = k.of;
+                    counter = a.count + 2 * gridDim.x + w0;
+                    out = true;
+                }
+            }
+        }
         at += g1 - g0;
+        if (at < hi) lds_barrier();
     }
 }
 
@@ -658,7 +759,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
         if (i0 + SETS * DEEP < parts) load(i0 + SETS * DEEP);
     }
     sums[set][v4] = v;
-    __syncthreads();
+    lds_barrier();
     if (set) return;
     for (int k = 1; k < SETS; k++) v += sums[k][v4];
     put_out(a, at, v, total, gate);
@@ -666,7 +767,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
 
 template <int D, int FMT>
 void launch(hipStream_t stream, const Args& a, int grid, bool join) {
-    hipLaunchKernelGGL((tree_attn_kernel<D, FMT>), dim3(grid), dim3(THREADS), 0, stream, a);
+    auto* f = a.row_tiles == 0 ? tree_attn_kernel<D, FMT, 1> : tree_attn_kernel<D, FMT, 2>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(THREADS), 0, stream, a);
     if (join) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.t.n * a.kv.heads * a.t.group)), dim3(256), 0, stream, a, grid);
 }
 
@@ -695,11 +797,11 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
         return fail(QH_EINVAL, "tree_attn: tables of %zu pages of %d tokens (1 to 2^30 positions)", step->table_ld, kv->page);
     const int group = q_heads / kv->heads;
     const int64_t groups = (cap + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES);  // of the longest sequence there can be
-    const int64_t most = (int64_t)(ctx ? ctx_cus(ctx) : 1) * wgs_per_cu(kv->head_dim);
+    const int64_t most = (int64_t)(ctx ? ctx_cus(ctx) : 1) * wgs_per_cu(kv->head_dim, 1);
     auto units_of = [&](int rt) { return (int64_t)kv->heads * ((step->max_new * group + (16 << rt) - 1) >> (4 + rt)); };
-    // A chunk's rows: all of them, up to 128, while that leaves work for every CU.
+    // A chunk's rows: all of them, up to 32, while that leaves work for every CU.
     int rt = 0;
-    while (rt < 3 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= most) rt++;
+    while (rt < 1 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= most) rt++;
     const int rows = 16 << rt;
     const int64_t units = units_of(rt);
     if (units * step->n_seq > 0x7fffffff / groups)

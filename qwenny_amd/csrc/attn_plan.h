@@ -7,7 +7,7 @@
 namespace qh {
 
 constexpr int KV_TILE = 64;          // tokens of a tile; pages are a multiple of it
-constexpr int GROUP_TILES = 8;       // tiles of a group, a workgroup's smallest part: one for each of its waves
+constexpr int GROUP_TILES = 4;       // tiles of a group, a workgroup's smallest part: one for each of its waves
 constexpr int TREE_MAX_SEQS = 1024;  // sequences of a step
 constexpr int TREE_MAX_NEW = 64;     // tokens of one sequence in a step: a mask is 64 bits
 
@@ -28,17 +28,21 @@ struct Seq {
     bool bad;
 };
 
-constexpr int group_count(int total) { return (int)(((unsigned)total + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES)); }
+// groups of `total` positions; `wide`: groups of twice the tiles, where there are enough for every workgroup
+constexpr int group_count(int total, bool wide = false) {
+    const unsigned size = KV_TILE * GROUP_TILES << (wide ? 1 : 0);
+    return (int)(((unsigned)total + size - 1) / size);
+}
 
 // (`rows`: a power of two)
-constexpr Seq sequence(const TreeArrays& a, int b, int rows) {
+constexpr Seq sequence(const TreeArrays& a, int b, int rows, bool wide = false) {
     const int s0 = a.start[b], s1 = a.start[b + 1], len = a.len[b];
     const int cap = (int)(a.table_ld << a.page_shift);
     const int first = s0 < 0 ? 0 : s0 > a.n ? a.n : s0, last = s1 < first ? first : s1 > a.n ? a.n : s1;
     const int most = a.max_new < cap ? a.max_new : cap, news = last - first < most ? last - first : most;
     const int old = len < 0 ? 0 : len > cap - news ? cap - news : len, total = old + news;
     const int chunks = (news * a.group + rows - 1) >> __builtin_ctz(rows);
-    return Seq{first, news, old, total, chunks, chunks ? group_count(total) : 0,
+    return Seq{first, news, old, total, chunks, chunks ? group_count(total, wide) : 0,
                first != s0 || last != s1 || news != last - first || old != len};
 }
 
@@ -61,16 +65,16 @@ constexpr int group_owner(int at, int all, int used) {
 // two, the unit that its part begins in and the one that it ends in.
 constexpr int partial_slot(int w, int u0, int all, int used) { return 2 * w + (first_group(w, all, used) < u0 ? 1 : 0); }
 
-// How `parts` partial results of a unit are summed: up to MAX_CLUSTER by the last of all to arrive; more in `of` clusters of
+// How `parts` partial results of a unit are summed: few by the last of all to arrive; more in `of` clusters of
 // `step` neighbours (the last has what is left), then the clusters' sums. The cluster of part i.
-constexpr int MAX_CLUSTER = 32;  // (its square is more than the workgroups of a launch)
+constexpr int MAX_CLUSTER = 32;  // (its square is no less than the workgroups of a launch)
 struct Cluster {
     int first, size, step, of;
 };
 constexpr Cluster cluster(int i, int parts) {
     int step = parts;
-    if (parts > 16)
-        for (step = 5; step * step < parts;) step++;
+    if (parts > 24)
+        for (step = 2; step * step < parts;) step++;
     const int first = i / step * step;
     return Cluster{first, step < parts - first ? step : parts - first, step, (parts + step - 1) / step};
 }

@@ -53,7 +53,7 @@ struct Args {
     int32_t fuse;          // partial results are summed by the last workgroup to arrive, else by join_kernel
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
-    int32_t* plan;         // [n_seq + 1]: base of each sequence's groups, then their number (for join_kernel)
+    int32_t* plan;         // [n_seq + 2]: base of each sequence's groups, their number, and whether they are wide (for join_kernel)
     uint32_t* count;       // [3 * workgroups] arrivals, zero between launches: of clusters by slot, then of units
 };
 
@@ -123,6 +123,14 @@ __device__ __forceinline__ float wave_max(float v) {
     return row_max(v);
 }
 
+// f over the 32 lanes of each half of the wave
+template <class F>
+__device__ __forceinline__ float lanes32(F&& f, float v) {
+    v = __int_as_float(over_lanes<16>(__float_as_int(v), [&](int x, int y) { return __float_as_int(f(__int_as_float(x), __int_as_float(y))); }));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
@@ -130,10 +138,10 @@ __device__ __forceinline__ float sigmoid(float x) {
 // What a workgroup of 16 R rows holds in LDS.
 template <int D, int R>
 struct Shared {
-    int32_t base[TREE_MAX_SEQS];  // of each sequence: its first group,
+    int32_t base[2][TREE_MAX_SEQS];  // of each sequence: its first group (of 4, of 8 tiles),
     int32_t who[TREE_MAX_SEQS];   // first token | tokens << 20,
     int32_t old[TREE_MAX_SEQS];   // positions before them | (its numbers do not fit) << 31
-    int32_t wave_sum[WAVES];
+    int32_t wave_sum[2][WAVES];
     int32_t last;
     float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
     f4 largest[16 * R][WAVES / 4];        // each wave's largest score of the row,
@@ -151,49 +159,59 @@ struct Shared {
     };
 };
 
-// The sequences' places in LDS; returns the number of their groups. Up to 64 sequences each wave makes the whole list for
-// itself, more are shared by the workgroup's threads.
+// The sequences' places in LDS, and the number of their groups: of four tiles in .x, of eight in .y. Up to 64 sequences each
+// wave makes the whole list for itself, more are shared by the workgroup's threads.
+struct Totals {
+    int narrow, wide;
+};
 template <int D, int R>
-__device__ __forceinline__ int plan(const Args& a, Shared<D, R>& sh) {
+__device__ __forceinline__ Totals plan(const Args& a, Shared<D, R>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool few = a.t.n_seq <= 64;
-    int before = 0;
+    int before[2] = {0, 0};
     for (int c = 0; c < a.t.n_seq; c += THREADS) {
         const int b = c + (few ? lane : (int)threadIdx.x);
-        int v = 0;
+        int v[2] = {0, 0}, run[2], sum[2];
         Seq s = {};
         if (b < a.t.n_seq) {
             s = sequence(a.t, b, 16 * R);
-            v = a.kv.heads * s.chunks * s.groups;
+            v[0] = a.kv.heads * s.chunks * s.groups;
+            v[1] = a.kv.heads * s.chunks * ((s.groups + 1) >> 1);
         }
-        int run = v;  // inclusive over the wave
-        run += dpp<0x111>(0, run);
-        run += dpp<0x112>(0, run);
-        run += dpp<0x114>(0, run);
-        run += dpp<0x118>(0, run);
-        run += dpp<0x142, 10>(0, run);
-        run += dpp<0x143, 12>(0, run);
-        int sum = __builtin_amdgcn_readlane(run, 63);
-        run += before - v;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            run[k] = v[k];  // inclusive over the wave
+            run[k] += dpp<0x111>(0, run[k]);
+            run[k] += dpp<0x112>(0, run[k]);
+            run[k] += dpp<0x114>(0, run[k]);
+            run[k] += dpp<0x118>(0, run[k]);
+            run[k] += dpp<0x142, 10>(0, run[k]);
+            run[k] += dpp<0x143, 12>(0, run[k]);
+            sum[k] = __builtin_amdgcn_readlane(run[k], 63);
+            run[k] += before[k] - v[k];
+        }
         if (!few) {
-            if (lane == 0) sh.wave_sum[wave] = sum;
+            if (lane == 0) sh.wave_sum[0][wave] = sum[0], sh.wave_sum[1][wave] = sum[1];
             lds_barrier();
-            sum = 0;
-            for (int w = 0; w < WAVES; w++) {
-                if (w < wave) run += sh.wave_sum[w];
-                sum += sh.wave_sum[w];
-            }
+            sum[0] = sum[1] = 0;
+            for (int w = 0; w < WAVES; w++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if (w < wave) run[k] += sh.wave_sum[k][w];
+                    sum[k] += sh.wave_sum[k][w];
+                }
             lds_barrier();
         }
         if (b < a.t.n_seq) {
-            sh.base[b] = run;
+            sh.base[0][b] = run[0];
+            sh.base[1][b] = run[1];
             sh.who[b] = s.first | s.news << 20;
             sh.old[b] = s.old | (s.bad ? 1 << 31 : 0);
         }
-        before += sum;
+        before[0] += sum[0], before[1] += sum[1];
     }
     if (!few) lds_barrier();
-    return __builtin_amdgcn_readfirstlane(before);
+    return Totals{__builtin_amdgcn_readfirstlane(before[0]), __builtin_amdgcn_readfirstlane(before[1])};
 }
 
 // x / y of numbers that all lanes have alike, where the quotient is below 2^20
@@ -232,44 +250,58 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
 template <int D, class Row>
 __device__ __forceinline__ void join_parts(const Args& a, Shared<D, 1>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
                                            int count, int live, bool out, Row&& row_of) {
-    constexpr int V = D / 4, DEEP = 16;
-    static_assert(THREADS == 16 * FAN);
+    constexpr int V = D / 4, DEEP = 24;
+    static_assert(FAN == 32);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // what follows from it is made here, not kept in registers over the whole kernel
     auto slot = [&](int i) { return i == 0 ? first_slot : 2 * (w0 + i * step); };
-    const int row = tid / FAN, part = tid % FAN;  // whose maximum and sum the thread takes
-    f2 ml = {-INFINITY, 0.0f};
-    if (part < count)
-        ml = __builtin_bit_cast(
-            f2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, a.ml_at + ((uint32_t)slot(part) * 16 + row) * 8, 0, CPOL_SC1));
+    const int part = tid % FAN;  // whose maxima and sums the thread takes, of every PASS-th row
+    constexpr int PASS = THREADS / FAN;
+    f2 ml[16 / PASS];
+#pragma unroll
+    for (int k = 0; k < 16 / PASS; k++) {
+        ml[k] = f2{-INFINITY, 0.0f};
+        if (part < count)
+            ml[k] = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(
+                                               rsrc, a.ml_at + ((uint32_t)slot(part) * 16 + k * PASS + tid / FAN) * 8, 0, CPOL_SC1));
+    }
+    // (rows that are not there are loads past the buffer's end: they read nothing)
     f4 in[DEEP];
+    constexpr uint32_t PAST = 0x40000000;
+    static_assert(PF_SK_PART_BYTES <= PAST);
     auto load = [&](int e, int i0) {
+        const uint32_t at = e < live * V ? e * 16 : PAST;
 #pragma unroll
         for (int k = 0; k < DEEP; k++)
-            if (i0 + k < count && e < live * V)
+            if (i0 + k < count)
                 in[k] = __builtin_bit_cast(
-                    f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (uint32_t)slot(i0 + k) * (16 * D * 4) + e * 16, 0, CPOL_SC1));
+                    f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, slot(i0 + k) * (16 * D * 4), CPOL_SC1));
     };
+    auto place = [&](int e) { return row_of(min(e / V, live - 1)) + e % V * 4; };
+    b4 gate = out ? load_gate(a, place(tid)) : b4{};
     load(tid, 0);
-    float best = ml.x;
 #pragma unroll
-    for (int o = 1; o < FAN; o <<= 1) best = fmaxf(best, __shfl_xor(best, o));
-    const float weight = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - best);
-    float total = ml.x == -INFINITY ? ml.y : ml.y * weight;  // (without a maximum: 0 or NaN)
-#pragma unroll
-    for (int o = 1; o < FAN; o <<= 1) total += __shfl_xor(total, o);
-    sh.parts.weight[part][row] = weight;
-    if (part == 0) sh.parts.row[row] = f2{best, total};
+    for (int k = 0; k < 16 / PASS; k++) {
+        const int row = k * PASS + tid / FAN;
+        const float best = lanes32([](float x, float y) { return fmaxf(x, y); }, ml[k].x);
+        const float weight = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - best);
+        // (without a maximum: 0 or NaN)
+        const float total = lanes32([](float x, float y) { return x + y; }, ml[k].x == -INFINITY ? ml[k].y : ml[k].y * weight);
+        sh.parts.weight[part][row] = weight;
+        if (part == 0) sh.parts.row[row] = f2{best, total};
+    }
     lds_barrier();
     for (int e = tid; e < live * V; e += THREADS) {
-        const size_t at = row_of(e / V) + e % V * 4;
-        const b4 gate = out ? load_gate(a, at) : b4{};
+        const size_t at = place(e);
+        if (e != tid && out) gate = load_gate(a, at);
         f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int i0 = 0; i0 < count; i0 += DEEP) {
             if (e != tid || i0) load(e, i0);
+            int there = count;
+            asm volatile("" : "+s"(there));  // compared anew: the loads' comparisons kept would be two registers each
 #pragma unroll
             for (int k = 0; k < DEEP; k++)
-                if (i0 + k < count) sum += sh.parts.weight[i0 + k][e / V] * in[k];
+                if (i0 + k < there) sum += sh.parts.weight[i0 + k][e / V] * in[k];
         }
         if (out) put_out(a, at, sum, sh.parts.row[e / V].y, gate);
         else
@@ -294,9 +326,9 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int of, int32_t* flag
     return *flag != 0;
 }
 
-// The work is a row of groups: for each sequence, kv head and chunk of 16 R rows, the cache in groups of 8 x 64 tokens. The
+// The work is a row of groups: for each sequence, kv head and chunk of 16 R rows, the cache in groups of 4 x 64 tokens. The
 // workgroups share it in equal parts, across the borders of sequences; consecutive parts on one XCD, whose L2 then serves
-// the chunks that read the same cache. In a group each of the eight waves makes the scores of one tile for all rows; the
+// the chunks that read the same cache. Eight tiles at a time, each of the eight waves makes the scores of one tile for all rows; the
 // waves agree on the rows' largest scores, put their probabilities into LDS, and each then multiplies all eight tiles' by
 // its own share of the values' dimensions. So a code is read and converted once for all rows, a wave's part of the outputs
 // is small, and there is nothing to join over the waves but the sums. (Each wave with whole rows and tiles of its own, joined
@@ -319,9 +351,14 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
     const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
     static_assert(sizeof(Args) > 128);
-    const int all = plan<D, R>(a, sh), used = min((int)gridDim.x, all);
+    // groups of four tiles where there are few, so that they reach more CUs; of eight where a workgroup has several, so that
+    // its waves' turns are whole
+    const Totals totals = plan<D, R>(a, sh);
+    const bool wide = totals.narrow > (int)gridDim.x;
+    const int all = wide ? totals.wide : totals.narrow, used = min((int)gridDim.x, all), group_tiles = GROUP_TILES << (wide ? 1 : 0);
     if (blockIdx.x == 0 && !a.fuse)
-        for (int i = threadIdx.x; i <= a.t.n_seq; i += THREADS) a.plan[i] = i < a.t.n_seq ? sh.base[i] : all;
+        for (int i = threadIdx.x; i <= a.t.n_seq + 1; i += THREADS)
+            a.plan[i] = i < a.t.n_seq ? sh.base[wide][i] : i == a.t.n_seq ? all : (int)wide;
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
     const int xcd = blockIdx.x & 7, at_xcd = blockIdx.x >> 3;
     if (at_xcd >= (used >> 3) + (xcd < (used & 7) ? 1 : 0)) return;
@@ -335,16 +372,16 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
         int tid = threadIdx.x, page_shift = a.kv.page_shift;
         asm volatile("" : "+v"(tid), "+s"(page_shift));
         const int lane = tid & 63, col = lane & 15, g = lane >> 4, page_tiles = 1 << (page_shift - 6);
-        const int b = find_seq(sh.base, a.t.n_seq, at);
+        const int b = find_seq(sh.base[wide], a.t.n_seq, at);
         const int who = __builtin_amdgcn_readfirstlane(sh.who[b]), was = __builtin_amdgcn_readfirstlane(sh.old[b]);
-        const int past = at - __builtin_amdgcn_readfirstlane(sh.base[b]);
+        const int past = at - __builtin_amdgcn_readfirstlane(sh.base[wide][b]);
         const int first = who & 0xfffff, news = who >> 20, old = was & 0x7fffffff, total = old + news;
         const int chunks = (news * a.t.group + ROWS - 1) / ROWS;
-        const int groups = group_count(total), unit = divide(past, groups), g0 = past - unit * groups;
+        const int groups = group_count(total, wide), unit = divide(past, groups), g0 = past - unit * groups;
         const int g1 = min(groups, g0 + hi - at);
         const int head = chunks == 1 ? unit : divide(unit, chunks), row0 = (unit - head * chunks) * ROWS;
         const int live = min(ROWS, news * a.t.group - row0);
-        const int t_end = min((total + KV_TILE - 1) / KV_TILE, g1 * GROUP_TILES);
+        const int t_end = min((total + KV_TILE - 1) / KV_TILE, g1 * group_tiles);
 
         // where tiles lie, 64 at a time: lane l has the l-th's place in the cache (of its keys) in tiles
         uint32_t places = 0;
@@ -354,7 +391,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
             places = (((uint32_t)pg * a.kv.heads + head) * 2 << (page_shift - 6)) + (mine & (page_tiles - 1));
             if (pg < 0 || ((int64_t)pg << page_shift) >= a.kv.slots) places = NONE;
         };
-        load_places(g0 * GROUP_TILES);
+        load_places(g0 * group_tiles);
 
         auto node_of = [&](int r) { return (int)((uint32_t)r * a.group_inv >> 20); };  // r / group
         // first element of a row's query, gate and output
@@ -381,34 +418,42 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
         u4 kc[4][C], vc[VT][SL];
         float sk, sv;
         const uint32_t in_tile = col * 64 + g * 16;
+        // 1 KiB pieces of a tile, as buffer loads: of a tile that is not there they read nothing
+        auto tile_at = [&](uint32_t place, int from, bool there) {
+            return __builtin_amdgcn_make_buffer_rsrc(a.kv.codes + (size_t)place * (KV_TILE * D) + from, 0, there ? KV_TILE * D - from : 0,
+                                                     BUF_RSRC_WORD3);
+        };
+        auto piece = [&](__amdgpu_buffer_rsrc_t tile, int at) {
+            return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, 0));
+        };
         // the wave's tile's keys and scales (lane l: token l's); a page that the cache has not gives NaN
-        auto load_keys = [&](int gr) {
-            const int t = gr * GROUP_TILES + wave, i = min(t, t_end - 1) - g0 * GROUP_TILES;
-            const uint32_t at = __builtin_amdgcn_readlane(places, i & 63);
+        auto load_keys = [&](int t8) {
+            const int t = t8 + wave;
+            const uint32_t at = __builtin_amdgcn_readlane(places, (t - g0 * group_tiles) & 63);
             const bool none = at == NONE;
             const uint32_t place = none ? 0 : at;
-            const uint8_t* const k = a.kv.codes + (size_t)place * (KV_TILE * D);
+            const auto tile = tile_at(place, 0, t < t_end);
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int sub = 0; sub < 4; sub++) kc[sub][c] = *(const u4*)(k + sub * 16 * D + c * 1024 + in_tile);
+                for (int sub = 0; sub < 4; sub++) kc[sub][c] = piece(tile, sub * 16 * D + c * 1024);
             const float* const sc = a.kv.scales + (size_t)place * KV_TILE;
             sk = none ? NAN : sc[lane];
             sv = t * KV_TILE + lane < total ? sc[page_tiles * KV_TILE + lane] : 0.0f;
         };
         const int slice = (wave % (WAVES / SPLIT)) * SL, v_tile = wave / (WAVES / SPLIT) * VT;
-        auto load_values = [&](int gr) {
+        auto load_values = [&](int t8) {
 #pragma unroll
             for (int v = 0; v < VT; v++) {
-                const int i = min(gr * GROUP_TILES + v_tile + v, t_end - 1) - g0 * GROUP_TILES;
-                const uint32_t at = __builtin_amdgcn_readlane(places, i & 63);
-                const uint8_t* const p = a.kv.codes + (size_t)((at == NONE ? 0 : at) + page_tiles) * (KV_TILE * D) + slice * 1024;
+                const int t = t8 + v_tile + v;
+                const uint32_t at = __builtin_amdgcn_readlane(places, (t - g0 * group_tiles) & 63);
+                const auto tile = tile_at((at == NONE ? 0 : at) + page_tiles, slice * 1024, t < t_end);
 #pragma unroll
-                for (int i = 0; i < SL; i++) vc[v][i] = *(const u4*)(p + i * 1024 + in_tile);
+                for (int i = 0; i < SL; i++) vc[v][i] = piece(tile, i * 1024);
             }
         };
-        load_keys(g0);
-        if (EARLY) load_values(g0);
+        load_keys(g0 * group_tiles);
+        if (EARLY) load_values(g0 * group_tiles);
 
         // the queries, scaled by a power of two into f16's range (the factor goes to the scores)
         for (int r = q_row;;) {
@@ -459,9 +504,9 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 for (int k = 0; k < CHAINS; k++) o[rt][i][k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        for (int gr = g0; gr < g1; gr++) {
-            const int t0 = (gr * GROUP_TILES + wave) * KV_TILE;
-            const bool more = gr + 1 < g1;
+        for (int t8 = g0 * group_tiles; t8 < t_end; t8 += WAVES) {
+            const int t0 = (t8 + wave) * KV_TILE;
+            const bool more = t8 + WAVES < t_end, own = t8 + wave < t_end;
             // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
             f4 x[R][4];
 #pragma unroll
@@ -487,20 +532,20 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 }
                 HOLD();
             }
-            if (!EARLY) load_values(gr);
+            if (!EARLY) load_values(t8);
 
             // the scores' and the values' scales, as the lanes need them
             float(&ts)[2][KV_TILE] = sh.tile_scale[wave];
             ts[0][lane] = sk;
             ts[1][lane] = sv;
             float most = 0.0f;
-            if (__any(sv > ref && sv < INFINITY)) most = wave_max(sv < INFINITY ? sv : 0.0f);
+            if (own && __any(sv > ref && sv < INFINITY)) most = wave_max(sv < INFINITY ? sv : 0.0f);
             __builtin_amdgcn_wave_barrier();
-            const bool whole = t0 + KV_TILE <= old;  // every row sees every token
+            const bool whole = own && t0 + KV_TILE <= old;  // every row sees every token
 #pragma unroll
             for (int rt = 0; rt < R; rt++) {
                 uint64_t seen = 0;  // bit i: the row sees token t0 + i
-                if (!whole) {
+                if (own && !whole) {
                     const int node = t0 - old;  // above -64
                     seen = node >= 64 ? 0 : node >= 0 ? sees[rt] >> node : sees[rt] << -node | ((1ull << -node) - 1);
                 }
@@ -546,7 +591,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                     top[rt] = next;
                     by *= al;
                 }
-                if (gr != g0 && __any(by != 1.0f)) {
+                if (t8 != g0 * group_tiles && __any(by != 1.0f)) {
 #pragma unroll
                     for (int i = 0; i < SL; i++)
 #pragma unroll
@@ -582,16 +627,15 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 HOLD();
             }
             if (more) {
-                const int i = (gr + 1 - g0) & 7;
-                if (i == 0) load_places((gr + 1) * GROUP_TILES);
-                load_keys(gr + 1);
+                if (((t8 + WAVES - g0 * group_tiles) & 63) == 0) load_places(t8 + WAVES);
+                load_keys(t8 + WAVES);
             }
             lds_barrier();
 
             // o^T += v^T p^T: the k index of both operands runs over tokens 16 w + 4 g + j, as the scores lie
 #pragma unroll
             for (int v = 0; v < VT; v++) {
-                const int t = gr * GROUP_TILES + v_tile + v;
+                const int t = t8 + v_tile + v;
                 if (t < t_end) {
                     if ((t + 1) * KV_TILE > total) {  // codes that no token of this sequence wrote may be anything
                         u4 keep;
@@ -618,7 +662,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                     }
                 }
             }
-            if (EARLY && more) load_values(gr + 1);
+            if (EARLY && more) load_values(t8 + WAVES);
         }
 
         // the waves' sums joined, and the outputs written, or a partial result
@@ -714,8 +758,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
     const int token = blockIdx.x / heads, h = blockIdx.x - token * heads, head = h / a.t.group;
     const int lane = threadIdx.x & 63, v4 = threadIdx.x % V, set = threadIdx.x / V;
     const int all = a.plan[a.t.n_seq], used = min(grid, all);
+    const bool wide = a.plan[a.t.n_seq + 1] != 0;
     const int b = max(0, find_seq(a.t.start, a.t.n_seq, token));  // the last sequence with start <= token
-    const Seq s = sequence(a.t, b, rows);
+    const Seq s = sequence(a.t, b, rows, wide);
     const int node = token - s.first;
     if (node < 0 || node >= s.news) return;
     const int r = node * a.t.group + h - head * a.t.group;
@@ -797,11 +842,11 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
         return fail(QH_EINVAL, "tree_attn: tables of %zu pages of %d tokens (1 to 2^30 positions)", step->table_ld, kv->page);
     const int group = q_heads / kv->heads;
     const int64_t groups = (cap + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES);  // of the longest sequence there can be
-    const int64_t most = (int64_t)(ctx ? ctx_cus(ctx) : 1) * wgs_per_cu(kv->head_dim, 1);
+    const int64_t cus = ctx ? ctx_cus(ctx) : 1;
     auto units_of = [&](int rt) { return (int64_t)kv->heads * ((step->max_new * group + (16 << rt) - 1) >> (4 + rt)); };
     // A chunk's rows: all of them, up to 32, while that leaves work for every CU.
     int rt = 0;
-    while (rt < 1 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= most) rt++;
+    while (rt < 1 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= cus) rt++;
     const int rows = 16 << rt;
     const int64_t units = units_of(rt);
     if (units * step->n_seq > 0x7fffffff / groups)
@@ -814,10 +859,10 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     a.mask = step->mask;
     a.group_inv = ((1u << 20) + group - 1) / group;
     a.scale = scale * 1.4426950408889634f;
-    const int grid = (int)std::min({most, units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
+    const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt), units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
     static_assert(3 * MAX_CLUSTER * MAX_CLUSTER <= PF_SK_ITEMS_MAX);
     const size_t part = (size_t)2 * grid * rows * kv->head_dim * 4, ml = (size_t)2 * grid * rows * 8;
-    if (part + ml + (TREE_MAX_SEQS + 1) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
+    if (part + ml + (TREE_MAX_SEQS + 2) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
     a.row_tiles = rt;
     a.part = (float*)ctx_partials(ctx);
     a.ml_at = (int32_t)part;

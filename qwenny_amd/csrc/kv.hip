@@ -18,42 +18,77 @@ using namespace qh;
 namespace {
 
 constexpr int WAVES = 4;
+constexpr int BATCH = 64, BATCH_WAVES = 16;  // tokens of a workgroup that turns values over in LDS, and its waves
 
+// f over the wave's 64 lanes: within rows of 16 by DPP, then over the rows
+template <class F>
+__device__ __forceinline__ uint32_t over_wave(uint32_t v, F&& f) {
+    auto step = [&](auto ctrl) { v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 15, 15, false)); };
+    step(std::integral_constant<int, 0xb1>{});   // quad_perm 1 0 3 2
+    step(std::integral_constant<int, 0x4e>{});   // quad_perm 2 3 0 1
+    step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    step(std::integral_constant<int, 0x140>{});  // row_mirror
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(a[0], a[1]);
+    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(a[0], a[1]);
+}
 __device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return __uint_as_float(
+        over_wave(__float_as_uint(v), [](uint32_t x, uint32_t y) { return __float_as_uint(__uint_as_float(x) + __uint_as_float(y)); }));
 }
 
-__device__ __forceinline__ float quotient_to_odd(float x, float s) {
-    const float y = x / s, r = fmaf(-y, s, x);
+// x / s rounded to odd: of the two neighbours of the quotient the one with its last bit set, unless it is exact. `r`: 1 / s to
+// a unit in the last place; the quotient made with it is one of the neighbours.
+__device__ __forceinline__ float quotient_to_odd(float x, float s, float r) {
+    float y = x * r;
+    y = fmaf(fmaf(-y, s, x), r, y);
+    const float left = fmaf(-y, s, x);
     uint32_t u = __float_as_uint(y);
-    if (r != 0.0f && y != 0.0f && !(u & 1)) u += (r < 0.0f) == (y < 0.0f) ? 1 : -1;
+    if (left != 0.0f && y != 0.0f && !(u & 1)) u += (left < 0.0f) == (y < 0.0f) ? 1 : -1;
     return __uint_as_float(u);
 }
 
-// The codes of a wave's vector (V values a lane) and its scale; not finite: scale NaN, codes of zero.
-template <int FMT, int V>
-__device__ __forceinline__ float quantise(const float (&x)[V], uint8_t (&code)[V]) {
-    float top = 0.0f, odd = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; i++) top = fmaxf(top, fabsf(x[i])), odd += x[i] * 0.0f;
-    top = wave_max(top);
-    odd = wave_sum(odd);
+// The codes of a wave's N vectors (V values a lane) and their scales; not finite: scale NaN, codes of zero. (The vectors'
+// steps wait for one another less side by side.)
+template <int FMT, int N, int V>
+__device__ __forceinline__ void quantise(const float (&x)[N][V], uint8_t (&code)[N][V], float (&s)[N]) {
     constexpr float most = FMT == QH_KV_I8 ? 127.0f : 448.0f;
-    float s = top / most;
-    if (!(odd == 0.0f)) s = NAN;
+    uint32_t bits[N];  // magnitudes compare as whole numbers; from 0x7f800000 on they are not finite
+    bool small = false;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        float y = s > 0.0f ? quotient_to_odd(x[i], s) : 0.0f;
-        y = fminf(fmaxf(y, -most), most);
-        if constexpr (FMT == QH_KV_I8) code[i] = (uint8_t)((int)rintf(y) + 128);
-        else code[i] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+    for (int n = 0; n < N; n++) {
+        bits[n] = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) bits[n] = max(bits[n], __float_as_uint(x[n][i]) & 0x7fffffffu);
     }
-    return s;
+#pragma unroll
+    for (int n = 0; n < N; n++) bits[n] = over_wave(bits[n], [](uint32_t x, uint32_t y) { return max(x, y); });
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        s[n] = bits[n] >= 0x7f800000u ? NAN : __uint_as_float(bits[n]) / most;
+        small |= !(s[n] >= 0x1p-126f);  // (or NaN) its reciprocal may not be a number
+    }
+    auto put = [&](int n, int i, float y) {
+        y = fminf(fmaxf(y, -most), most);
+        if constexpr (FMT == QH_KV_I8) code[n][i] = (uint8_t)((int)rintf(y) + 128);
+        else code[n][i] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+    };
+    if (!__any(small)) {
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float r = __builtin_amdgcn_rcpf(s[n]);
+#pragma unroll
+            for (int i = 0; i < V; i++) put(n, i, quotient_to_odd(x[n][i], s[n], r));
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                put(n, i, !(s[n] > 0.0f) ? 0.0f
+                          : s[n] >= 0x1p-126f ? quotient_to_odd(x[n][i], s[n], __builtin_amdgcn_rcpf(s[n])) : x[n][i] / s[n]);
+    }
 }
 
 template <int FMT>
@@ -62,12 +97,10 @@ __device__ __forceinline__ float code_value(uint32_t code) {
     else return __builtin_amdgcn_cvt_f32_fp8(code, 0);
 }
 
-// A wave's vector (lane l holds dimensions V l ..) into one slot as a key (which = 0) or value (1).
-template <int D, int FMT, int V>
-__device__ __forceinline__ void store(const Kv& kv, int64_t slot, int head, int which, const float (&x)[V], int lane) {
+// A wave's vector's codes (lane l holds dimensions V l ..) and scale into one slot as a key (which = 0) or value (1).
+template <int D, int V>
+__device__ __forceinline__ void store(const Kv& kv, int64_t slot, int head, int which, const uint8_t (&code)[V], float s, int lane) {
     if (slot < 0 || slot >= kv.slots) return;
-    uint8_t code[V];
-    const float s = quantise<FMT>(x, code);
     const int64_t page = slot >> kv.page_shift;
     const uint32_t t = (uint32_t)slot & ((1u << kv.page_shift) - 1), d = lane * V;
     uint8_t* const to = kv.codes + kv_block<D>(kv, page, head, which);
@@ -83,6 +116,13 @@ __device__ __forceinline__ void store(const Kv& kv, int64_t slot, int head, int 
     }
     if (lane == 0) kv.scales[kv_scale(kv, page, head, which) + t] = s;
 }
+template <int D, int FMT, int V>
+__device__ __forceinline__ void quantise_into(const Kv& kv, int64_t slot, int head, int which, const float (&x)[V], int lane) {
+    uint8_t code[1][V];
+    float s[1];
+    quantise<FMT, 1, V>(*(const float(*)[1][V])&x, code, s);
+    store<D, V>(kv, slot, head, which, code[0], s[0], lane);
+}
 
 template <int V>
 struct Vec {
@@ -94,6 +134,24 @@ struct Vec<1> {
     typedef float f __attribute__((ext_vector_type(1)));
     typedef __bf16 b __attribute__((ext_vector_type(1)));
 };
+
+// One head of one token's partials, summed in their order: V values a lane, up to eight partials in flight.
+template <int V>
+__device__ __forceinline__ void head_sum(const float* __restrict__ x, int splits, int64_t stride, int lane, float (&y)[V]) {
+    typedef typename Vec<V>::f vec;
+    vec sum = __builtin_nontemporal_load((const vec*)(x + lane * V));
+    for (int s0 = 1; s0 < splits; s0 += 8) {
+        vec p[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (s0 + j < splits) p[j] = __builtin_nontemporal_load((const vec*)(x + (s0 + j) * stride + lane * V));
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (s0 + j < splits) sum += p[j];
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = sum[i];
+}
 
 // a wave for each (token, kv head, keys or values)
 template <int D, int FMT>
@@ -109,7 +167,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_write_kernel(Kv kv, const __bf1
     float x[V];
 #pragma unroll
     for (int j = 0; j < V; j++) x[j] = (float)in[j];
-    store<D, FMT, V>(kv, slots[t], (int)(th - t * kv.heads), which, x, lane);
+    quantise_into<D, FMT, V>(kv, slots[t], (int)(th - t * kv.heads), which, x, lane);
 }
 
 template <int D, int FMT>
@@ -135,6 +193,167 @@ __global__ __launch_bounds__(64 * WAVES) void kv_read_kernel(Kv kv, const int32_
         for (int j = 0; j < V; j++) y[j] = (__bf16)(code_value<FMT>(from[which ? v_byte<D>(t, d + j) : k_byte<D>(t, d + j)]) * s);
     }
     *(typename Vec<V>::b*)((which ? v : k) + th * D + lane * V) = y;
+}
+
+// Where a batch kernel's values come from: bf16, or the in-projection's partials (f32, summed in their order).
+struct Source {
+    const __bf16* bf16;
+    const float* x;
+    int splits;
+    int64_t stride, ld;  // of a partial, of a token
+    int col;             // of the first head's values
+};
+
+// 64 tokens of one kv head, keys (which = 0) or values, for many tokens at a time (prompts). A value's codes lie 64 bytes
+// from dimension to dimension, four tokens side by side: written vector by vector they are single bytes, 16.0 us for 2048
+// tokens of 4 x 256. Here the codes of 64 tokens are put into LDS and turned over: a thread writes four tokens' codes of four
+// dimensions, 16 threads the 64 bytes of a dimension.
+// `which0`: 0 for keys and values, 1 for values alone.
+template <int D, int FMT, bool PARTIALS>
+__global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv, Source keys, Source values,
+                                                                          const int32_t* __restrict__ slots, int n, int which0) {
+    constexpr int V = D / 64, EACH = BATCH / BATCH_WAVES, ROW = D / 4 + 1;
+    __shared__ uint32_t codes[BATCH][ROW];
+    __shared__ __align__(4) uint8_t from[BATCH_WAVES][BATCH];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t0 = blockIdx.x * BATCH;
+    const int which = which0 | (blockIdx.y & (1 - which0)), head = blockIdx.y >> (1 - which0);
+    const Source& src = which ? values : keys;
+    float x[EACH][V];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int t = min(t0 + wave + i * BATCH_WAVES, n - 1);
+        if constexpr (PARTIALS) {
+            head_sum<V>(src.x + t * src.ld + src.col + head * D, src.splits, src.stride, lane, x[i]);
+        } else {
+            const auto in = *(const typename Vec<V>::b*)(src.bf16 + ((int64_t)t * kv.heads + head) * D + lane * V);
+#pragma unroll
+            for (int j = 0; j < V; j++) x[i][j] = (float)in[j];
+        }
+    }
+    const int mine = t0 + lane < n ? slots[t0 + lane] : -1;  // lane l: the l-th token's slot
+    const bool in_cache = mine >= 0 && mine < kv.slots;
+    uint8_t code[EACH][V];
+    float s[EACH];
+    quantise<FMT>(x, code, s);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int e = wave + i * BATCH_WAVES, slot = __builtin_amdgcn_readlane(mine, e);
+        if (which == 0) {
+            store<D, V>(kv, slot, head, 0, code[i], s[i], lane);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) ((uint8_t*)codes[e])[lane * V + j] = code[i][j];
+        if (lane == 0 && slot >= 0 && slot < kv.slots)
+            kv.scales[kv_scale(kv, slot >> kv.page_shift, head, 1) + (slot & ((1 << kv.page_shift) - 1))] = s[i];
+    }
+    if (which == 0) return;
+    __syncthreads();
+    // one of the cache's tiles after the other, that of the first token left
+    for (uint64_t left = __ballot(in_cache); left;) {
+        const int tile = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)left) - 1) >> 6;
+        const bool here = in_cache && mine >> 6 == tile;
+        left &= ~__ballot(here);
+        from[wave][lane] = 255;
+        __builtin_amdgcn_wave_barrier();
+        if (here) from[wave][mine & 63] = (uint8_t)lane;
+        __builtin_amdgcn_wave_barrier();
+        const int slot0 = tile << 6;
+        uint8_t* const to = kv.codes + kv_block<D>(kv, slot0 >> kv.page_shift, head, 1) + (size_t)(slot0 & ((1 << kv.page_shift) - 1)) * D;
+        const int p = lane & 15;  // bytes 4 p .. of a dimension: tokens 16 (p % 4) + 4 (p / 4) ..
+        const uint32_t who = *(const uint32_t*)&from[wave][(p & 3) * 16 + (p >> 2) * 4];
+        if (who == ~0u) continue;
+        const bool all = !((who & 0x80808080u));
+        for (int dg = threadIdx.x >> 4; dg < D / 4; dg += 4 * BATCH_WAVES) {
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) c[j] = codes[who >> (8 * j) & 63][dg];
+            // bytes turned over: o[d] = the four tokens' byte d
+            const uint32_t a0 = __builtin_amdgcn_perm(c[1], c[0], 0x05010400u), a1 = __builtin_amdgcn_perm(c[1], c[0], 0x07030602u);
+            const uint32_t b0 = __builtin_amdgcn_perm(c[3], c[2], 0x05010400u), b1 = __builtin_amdgcn_perm(c[3], c[2], 0x07030602u);
+            const uint32_t o[4] = {__builtin_amdgcn_perm(b0, a0, 0x05040100u), __builtin_amdgcn_perm(b0, a0, 0x07060302u),
+                                   __builtin_amdgcn_perm(b1, a1, 0x05040100u), __builtin_amdgcn_perm(b1, a1, 0x07060302u)};
+            uint8_t* const at = to + dg * 256 + p * 4;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                if (all) *(uint32_t*)(at + d * 64) = o[d];
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (!(who >> (8 * j) & 0x80)) at[d * 64 + j] = (uint8_t)(o[d] >> (8 * j));
+            }
+        }
+    }
+}
+
+// The same tokens read back: a tile's values go into LDS whole, each wave then takes its tokens' bytes out of them.
+template <int D, int FMT>
+__global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, const int32_t* __restrict__ slots, int n,
+                                                                         __bf16* __restrict__ k, __bf16* __restrict__ v) {
+    constexpr int V = D / 64, EACH = BATCH / BATCH_WAVES, ROW = 17;  // words of a dimension's 64 bytes, and one
+    __shared__ uint32_t tile_codes[D * ROW];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t0 = blockIdx.x * BATCH, which = blockIdx.y & 1, head = blockIdx.y >> 1;
+    const uint32_t in_page = (1u << kv.page_shift) - 1;
+    const int mine = t0 + lane < n ? slots[t0 + lane] : -1;
+    const bool in_cache = mine >= 0 && mine < kv.slots;
+    const float scale = in_cache ? kv.scales[kv_scale(kv, mine >> kv.page_shift, head, which) + (mine & in_page)] : 0.0f;
+    __bf16* const out = (which ? v : k) + ((int64_t)t0 * kv.heads + head) * D + lane * V;
+    auto put = [&](int e, const uint8_t (&c)[V]) {
+        const float s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), e));
+        typename Vec<V>::b y;
+#pragma unroll
+        for (int j = 0; j < V; j++) y[j] = (__bf16)(code_value<FMT>(c[j]) * s);
+        *(typename Vec<V>::b*)(out + (int64_t)e * kv.heads * D) = y;
+    };
+    typename Vec<V>::b zero;
+#pragma unroll
+    for (int j = 0; j < V; j++) zero[j] = (__bf16)0.0f;
+    const uint64_t there = __ballot(in_cache);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int e = wave * EACH + i;
+        if (t0 + e < n && !(there >> e & 1)) *(typename Vec<V>::b*)(out + (int64_t)e * kv.heads * D) = zero;
+    }
+    if (which == 0) {
+        uint8_t c[EACH][V];
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int slot = __builtin_amdgcn_readlane(in_cache ? mine : 0, wave * EACH + i);
+            const uint8_t* const at = kv.codes + kv_block<D>(kv, slot >> kv.page_shift, head, 0) + k_byte<D>(slot & in_page, lane * V);
+            typedef uint8_t bytes __attribute__((ext_vector_type(V)));
+            const bytes b = *(const bytes*)at;
+#pragma unroll
+            for (int j = 0; j < V; j++) c[i][j] = b[j];
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++)
+            if (there >> (wave * EACH + i) & 1) put(wave * EACH + i, c[i]);
+        return;
+    }
+    for (uint64_t left = there; left;) {
+        const int tile = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)left) - 1) >> 6, slot0 = tile << 6;
+        const uint64_t here = __ballot(in_cache && mine >> 6 == tile);
+        left &= ~here;
+        const uint8_t* const block = kv.codes + kv_block<D>(kv, slot0 >> kv.page_shift, head, 1) + (size_t)(slot0 & in_page) * D;
+        for (int i = threadIdx.x; i < D * 4; i += 64 * BATCH_WAVES) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const u4 w = *(const u4*)(block + i * 16);
+            uint32_t* const to = tile_codes + (i >> 2) * ROW + (i & 3) * 4;
+            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int e = wave * EACH + i;
+            if (!(here >> e & 1)) continue;
+            const uint32_t t = __builtin_amdgcn_readlane(mine, e) & 63, byte = v_byte<D>(t, 0);
+            uint8_t c[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) c[j] = ((const uint8_t*)(tile_codes + (lane * V + j) * ROW))[byte];
+            put(e, c);
+        }
+        if (left) __syncthreads();
+    }
 }
 
 // a workgroup for each (sequence, kv head, keys or values): 64 moves at a time read into LDS, then written
@@ -188,25 +407,8 @@ struct Prep {
     __bf16 *q, *gate, *k, *v;
     Kv kv;
     const int32_t* slots;
+    int heads;  // heads of a token that the kernel takes: the values' last, or without them
 };
-
-// One head of one token's partials, summed in their order: V values a lane, up to eight partials in flight.
-template <int V>
-__device__ __forceinline__ void head_sum(const float* __restrict__ x, int splits, int64_t stride, int lane, float (&y)[V]) {
-    typedef typename Vec<V>::f vec;
-    vec sum = *(const vec*)(x + lane * V);
-    for (int s0 = 1; s0 < splits; s0 += 8) {
-        vec p[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (s0 + j < splits) p[j] = *(const vec*)(x + (s0 + j) * stride + lane * V);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (s0 + j < splits) sum += p[j];
-    }
-#pragma unroll
-    for (int i = 0; i < V; i++) y[i] = sum[i];
-}
 
 template <int V>
 __device__ __forceinline__ void put(__bf16* to, const float (&y)[V], int lane) {
@@ -226,21 +428,33 @@ __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
     __shared__ float rows[WAVES][D];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = a.rot / 2;
     const int64_t t = blockIdx.x;
+    const int per = a.gated ? 2 : 1, heads = a.heads;
+    const int64_t ld = (int64_t)(a.q_heads * per + 2 * a.kv_heads) * D, stride = a.n * ld;
+    const int share = (heads + gridDim.y - 1) / gridDim.y, h1 = min(heads, (int)(blockIdx.y + 1) * share);
+    // a head's sums, with a query's those of its gate, are read while the head before is worked on
+    float next[V], next_gate[V];
+    auto read = [&](int h) {
+        const bool is_q = h < a.q_heads;
+        const float* const x = a.x + t * ld + (int64_t)(is_q ? h * per : h - a.q_heads + a.q_heads * per) * D;
+        head_sum<V>(x, a.splits, stride, lane, next);
+        if (is_q && a.gated) head_sum<V>(x + D, a.splits, stride, lane, next_gate);
+    };
+    const int h0 = blockIdx.y * share + wave;
+    if (h0 < h1) read(h0);
     if ((int)threadIdx.x < half) {
         const double turns = (double)a.pos[t] * (double)a.inv_freq[threadIdx.x] * 0.15915494309189535;
         const float part = (float)(turns - rint(turns));
         sincospif(2.0f * part, &sn[threadIdx.x], &cs[threadIdx.x]);
     }
-    __syncthreads();
-    const int per = a.gated ? 2 : 1, heads = a.q_heads + 2 * a.kv_heads;
-    const int64_t ld = (int64_t)(a.q_heads * per + 2 * a.kv_heads) * D, stride = a.n * ld;
-    const int share = (heads + gridDim.y - 1) / gridDim.y, h1 = min(heads, (int)(blockIdx.y + 1) * share);
-    for (int h = blockIdx.y * share + wave; h < h1; h += WAVES) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");  // (the reads stay in flight over the barrier)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    for (int h = h0; h < h1; h += WAVES) {
         const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
-        const int col = is_q ? h * per : h - a.q_heads + a.q_heads * per;
-        const float* const x = a.x + t * ld + (int64_t)col * D;
-        float y[V];
-        head_sum<V>(x, a.splits, stride, lane, y);
+        float y[V], gate[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) y[i] = next[i], gate[i] = next_gate[i];
+        if (h + WAVES < h1) read(h + WAVES);
         const float* const w = is_q ? a.q_w : is_k ? a.k_w : nullptr;
         if (w) {
             float ss = 0.0f;
@@ -264,15 +478,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
         }
         if (is_q) {
             put<V>(a.q + (t * a.q_heads + h) * D, y, lane);
-            if (a.gated) {
-                head_sum<V>(x + D, a.splits, stride, lane, y);
-                put<V>(a.gate + (t * a.q_heads + h) * D, y, lane);
-            }
+            if (a.gated) put<V>(a.gate + (t * a.q_heads + h) * D, gate, lane);
             continue;
         }
         const int head = h - a.q_heads - (is_k ? 0 : a.kv_heads);
         if constexpr (FMT == 0) put<V>((is_k ? a.k : a.v) + (t * a.kv_heads + head) * D, y, lane);
-        else store<D, FMT, V>(a.kv, a.slots[t], head, is_k ? 0 : 1, y, lane);
+        else quantise_into<D, FMT, V>(a.kv, a.slots[t], head, is_k ? 0 : 1, y, lane);
     }
 }
 
@@ -289,6 +500,7 @@ int launched(const char* who) {
 }
 
 constexpr size_t MAX_TOKENS = (size_t)1 << 20;  // of one call
+constexpr size_t BATCH_FROM = 64;               // tokens from which the batch kernels take over: a whole batch
 
 }  // namespace
 
@@ -314,6 +526,13 @@ extern "C" int qh_kv_write(void* stream, const qh_kv* kv, const void* k_bf16, co
     const dim3 grid((unsigned)((vectors + WAVES - 1) / WAVES));
     by_dim(kv->head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
+        if (n >= BATCH_FROM) {
+            const Source ks = {(const __bf16*)k_bf16}, vs = {(const __bf16*)v_bf16};
+            auto* f = kv->fmt == QH_KV_I8 ? kv_write_batch_kernel<D, QH_KV_I8, false> : kv_write_batch_kernel<D, QH_KV_E4M3, false>;
+            hipLaunchKernelGGL(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream, c,
+                               ks, vs, slots, (int)n, 0);
+            return;
+        }
         auto* f = kv->fmt == QH_KV_I8 ? kv_write_kernel<D, QH_KV_I8> : kv_write_kernel<D, QH_KV_E4M3>;
         hipLaunchKernelGGL(f, grid, dim3(64 * WAVES), 0, (hipStream_t)stream, c, (const __bf16*)k_bf16, (const __bf16*)v_bf16,
                            slots, vectors);
@@ -332,6 +551,12 @@ extern "C" int qh_kv_read(void* stream, const qh_kv* kv, const int32_t* slots, s
     const dim3 grid((unsigned)((vectors + WAVES - 1) / WAVES));
     by_dim(kv->head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
+        if (n >= BATCH_FROM) {
+            auto* f = kv->fmt == QH_KV_I8 ? kv_read_batch_kernel<D, QH_KV_I8> : kv_read_batch_kernel<D, QH_KV_E4M3>;
+            hipLaunchKernelGGL(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream, c,
+                               slots, (int)n, (__bf16*)k_bf16, (__bf16*)v_bf16);
+            return;
+        }
         auto* f = kv->fmt == QH_KV_I8 ? kv_read_kernel<D, QH_KV_I8> : kv_read_kernel<D, QH_KV_E4M3>;
         hipLaunchKernelGGL(f, grid, dim3(64 * WAVES), 0, (hipStream_t)stream, c, slots, vectors, (__bf16*)k_bf16, (__bf16*)v_bf16);
     });
@@ -378,12 +603,20 @@ extern "C" int qh_attn_prep(void* stream, const float* x, int splits, size_t n, 
     a.x = x, a.splits = splits, a.n = (int64_t)n, a.q_heads = rows->q_heads, a.kv_heads = rows->kv_heads, a.rot = rows->rot;
     a.gated = rows->gated != 0, a.q_w = q_w, a.k_w = k_w, a.inv_freq = inv_freq, a.eps = eps, a.pos = pos, a.slots = slots;
     a.q = (__bf16*)q, a.gate = (__bf16*)gate, a.k = (__bf16*)k, a.v = (__bf16*)v;
-    const int heads = rows->q_heads + 2 * rows->kv_heads;
+    // into the cache, many tokens' values are turned over by the batch kernel
+    const bool batch = kv && n >= BATCH_FROM;
+    const int heads = a.heads = rows->q_heads + (batch ? 1 : 2) * rows->kv_heads;
     const unsigned shares = n >= 512 ? 1 : (heads + WAVES - 1) / WAVES;
     by_dim(D, [&](auto d) {
         constexpr int DD = decltype(d)::value;
         auto* f = !kv ? attn_prep_kernel<DD, 0> : kv->fmt == QH_KV_I8 ? attn_prep_kernel<DD, QH_KV_I8> : attn_prep_kernel<DD, QH_KV_E4M3>;
         hipLaunchKernelGGL(f, dim3((unsigned)n, shares), dim3(64 * WAVES), 0, (hipStream_t)stream, a);
+        if (!batch) return;
+        const int64_t ld = (int64_t)(rows->q_heads * (a.gated ? 2 : 1) + 2 * rows->kv_heads) * D;
+        const Source vs = {nullptr, x, splits, (int64_t)n * ld, ld, (int)(ld - (int64_t)rows->kv_heads * D)};
+        auto* fv = kv->fmt == QH_KV_I8 ? kv_write_batch_kernel<DD, QH_KV_I8, true> : kv_write_batch_kernel<DD, QH_KV_E4M3, true>;
+        hipLaunchKernelGGL(fv, dim3((unsigned)((n + BATCH - 1) / BATCH), rows->kv_heads), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream,
+                           a.kv, vs, vs, slots, (int)n, 1);
     });
     return launched("attn_prep");
 }

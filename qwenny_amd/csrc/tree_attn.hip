@@ -504,7 +504,12 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 for (int k = 0; k < CHAINS; k++) o[rt][i][k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+        const int whole_lane = lane;
         for (int t8 = g0 * group_tiles; t8 < t_end; t8 += WAVES) {
+            // (said anew here and behind the loop: what follows from it would be kept in registers otherwise, and they run out)
+            int said = whole_lane;
+            asm volatile("" : "+v"(said));
+            const int lane = said, col = lane & 15, g = lane >> 4;
             const int t0 = (t8 + wave) * KV_TILE;
             const bool more = t8 + WAVES < t_end, own = t8 + wave < t_end;
             // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
@@ -668,61 +673,66 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
         // the waves' sums joined, and the outputs written, or a partial result
         const bool direct = g0 == 0 && g1 == groups;
         const int slot = 2 * w + (at != lo);
-#pragma unroll
-        for (int rt = 0; rt < R; rt++) {
-            const f2 s = {row_sum(sum[rt]), FMT == QH_KV_I8 ? row_sum(rounded[rt]) : 0.0f};
-            if (g == 0) ((f2*)sh.sums[rt * 16 + col])[wave] = s;
-        }
-        b4 gate[R][SL];
-        if (direct)
-#pragma unroll
-            for (int rt = 0; rt < R; rt++)
-#pragma unroll
-                for (int i = 0; i < SL; i++) gate[rt][i] = load_gate(a, row_at(min(rt * 16 + col, live - 1)) + (slice + i) * 16 + g * 4);
-        lds_barrier();
-#pragma unroll
-        for (int rt = 0; rt < R; rt++) {
-            f4 s = sh.sums[rt * 16 + col][0];
-#pragma unroll
-            for (int k = 1; k < WAVES / 2; k++) s += sh.sums[rt * 16 + col][k];
-            sum[rt] = s.x + s.z;
-            const float back = -128.0f * (s.y + s.w);
-#pragma unroll
-            for (int i = 0; i < SL; i++) {
-                f4 v = o[rt][i][0];
-                if (CHAINS > 1) v += o[rt][i][CHAINS - 1];
-                if (FMT == QH_KV_I8) v = v * 0x1p24f + back / SPLIT;
-                o[rt][i][0] = v * ref;
-            }
-        }
-        if (SPLIT > 1) {  // two waves have the same dimensions, of different tiles
-            if (wave >= WAVES / SPLIT)
-#pragma unroll
-                for (int rt = 0; rt < R; rt++) sh.half[rt][wave - WAVES / 2][lane] = o[rt][0][0];
-            lds_barrier();
-            if (wave < WAVES / SPLIT)
-#pragma unroll
-                for (int rt = 0; rt < R; rt++) o[rt][0][0] += sh.half[rt][wave][lane];
-        }
-        if (SPLIT == 1 || wave < WAVES / SPLIT)
+        {
+            int said = whole_lane;
+            asm volatile("" : "+v"(said));
+            const int lane = said, col = lane & 15, g = lane >> 4;
 #pragma unroll
             for (int rt = 0; rt < R; rt++) {
-                const int r = rt * 16 + col;
-                if (r >= live) continue;
-                if (direct) {
+                const f2 s = {row_sum(sum[rt]), FMT == QH_KV_I8 ? row_sum(rounded[rt]) : 0.0f};
+                if (g == 0) ((f2*)sh.sums[rt * 16 + col])[wave] = s;
+            }
+            b4 gate[R][SL];
+            if (direct)
 #pragma unroll
-                    for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt], gate[rt][i]);
-                } else {
+                for (int rt = 0; rt < R; rt++)
 #pragma unroll
-                    for (int i = 0; i < SL; i++)
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, o[rt][i][0]), rsrc,
-                                                               (uint32_t)((slot * ROWS + r) * D + (slice + i) * 16 + g * 4) * 4, 0, CPOL_SC1);
-                    if (wave == 0 && g == 0)
-                        __builtin_amdgcn_raw_buffer_store_b64(
-                            __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * factor[rt], sum[rt]})), rsrc,
-                            a.ml_at + (uint32_t)(slot * ROWS + r) * 8, 0, CPOL_SC1);
+                    for (int i = 0; i < SL; i++) gate[rt][i] = load_gate(a, row_at(min(rt * 16 + col, live - 1)) + (slice + i) * 16 + g * 4);
+            lds_barrier();
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) {
+                f4 s = sh.sums[rt * 16 + col][0];
+#pragma unroll
+                for (int k = 1; k < WAVES / 2; k++) s += sh.sums[rt * 16 + col][k];
+                sum[rt] = s.x + s.z;
+                const float back = -128.0f * (s.y + s.w);
+#pragma unroll
+                for (int i = 0; i < SL; i++) {
+                    f4 v = o[rt][i][0];
+                    if (CHAINS > 1) v += o[rt][i][CHAINS - 1];
+                    if (FMT == QH_KV_I8) v = v * 0x1p24f + back / SPLIT;
+                    o[rt][i][0] = v * ref;
                 }
             }
+            if (SPLIT > 1) {  // two waves have the same dimensions, of different tiles
+                if (wave >= WAVES / SPLIT)
+#pragma unroll
+                    for (int rt = 0; rt < R; rt++) sh.half[rt][wave - WAVES / 2][lane] = o[rt][0][0];
+                lds_barrier();
+                if (wave < WAVES / SPLIT)
+#pragma unroll
+                    for (int rt = 0; rt < R; rt++) o[rt][0][0] += sh.half[rt][wave][lane];
+            }
+            if (SPLIT == 1 || wave < WAVES / SPLIT)
+#pragma unroll
+                for (int rt = 0; rt < R; rt++) {
+                    const int r = rt * 16 + col;
+                    if (r >= live) continue;
+                    if (direct) {
+#pragma unroll
+                        for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt], gate[rt][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < SL; i++)
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, o[rt][i][0]), rsrc,
+                                                                   (uint32_t)((slot * ROWS + r) * D + (slice + i) * 16 + g * 4) * 4, 0, CPOL_SC1);
+                        if (wave == 0 && g == 0)
+                            __builtin_amdgcn_raw_buffer_store_b64(
+                                __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * factor[rt], sum[rt]})), rsrc,
+                                a.ml_at + (uint32_t)(slot * ROWS + r) * 8, 0, CPOL_SC1);
+                    }
+                }
+        }
         if constexpr (R == 1) {
             if (!direct && a.fuse) {
                 const int u0 = at - g0, w0 = group_owner(u0, all, used), parts = group_owner(u0 + groups - 1, all, used) - w0 + 1;

@@ -61,6 +61,12 @@ constexpr int group_owner(int at, int all, int used) {
     return w;
 }
 
+// The workgroups that take part of `grid`. One sequence's units are all alike: each gets as many workgroups as any, so that no
+// workgroup has parts of two.
+constexpr int used_workgroups(int grid, int all, int n_seq, int units) {
+    return all <= grid ? all : n_seq == 1 && units <= grid ? units * (grid / units) : grid;
+}
+
 // Where workgroup w keeps its partial result of the unit (sequence, kv head, chunk) whose groups begin at u0: it has at most
 // two, the unit that its part begins in and the one that it ends in.
 constexpr int partial_slot(int w, int u0, int all, int used) { return 2 * w + (first_group(w, all, used) < u0 ? 1 : 0); }

@@ -31,6 +31,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 8, THREADS = 64 * WAVES;  // of a workgroup: two waves a SIMD
 constexpr int FAN = MAX_CLUSTER;
+constexpr int PLAN_HEAD = 4;
 
 // buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of agent-coherent loads and stores
 constexpr int BUF_RSRC_WORD3 = 0x00020000;
@@ -53,7 +54,7 @@ struct Args {
     int32_t fuse;          // partial results are summed by the last workgroup to arrive, else by join_kernel
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
-    int32_t* plan;         // [n_seq + 2]: base of each sequence's groups, their number, and whether they are wide (for join_kernel)
+    int32_t* plan;         // for join_kernel: groups, workgroups, whether the groups are wide; each sequence's first group
     uint32_t* count;       // [3 * workgroups] arrivals, zero between launches: of clusters by slot, then of units
 };
 
@@ -123,10 +124,14 @@ __device__ __forceinline__ float wave_max(float v) {
     return row_max(v);
 }
 
-// f over the 32 lanes of each half of the wave
+// f over the 16 lanes of each quarter of the wave, over the 32 of each half
+template <class F>
+__device__ __forceinline__ float lanes16(F&& f, float v) {
+    return __int_as_float(over_lanes<16>(__float_as_int(v), [&](int x, int y) { return __float_as_int(f(__int_as_float(x), __int_as_float(y))); }));
+}
 template <class F>
 __device__ __forceinline__ float lanes32(F&& f, float v) {
-    v = __int_as_float(over_lanes<16>(__float_as_int(v), [&](int x, int y) { return __float_as_int(f(__int_as_float(x), __int_as_float(y))); }));
+    v = lanes16(f, v);
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
@@ -162,21 +167,22 @@ struct Shared {
 // The sequences' places in LDS, and the number of their groups: of four tiles in .x, of eight in .y. Up to 64 sequences each
 // wave makes the whole list for itself, more are shared by the workgroup's threads.
 struct Totals {
-    int narrow, wide;
+    int narrow, wide, units;  // (units: of the first sequence)
 };
 template <int D, int R>
 __device__ __forceinline__ Totals plan(const Args& a, Shared<D, R>& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool few = a.t.n_seq <= 64;
-    int before[2] = {0, 0};
+    int before[2] = {0, 0}, units = 0;
     for (int c = 0; c < a.t.n_seq; c += THREADS) {
         const int b = c + (few ? lane : (int)threadIdx.x);
         int v[2] = {0, 0}, run[2], sum[2];
         Seq s = {};
         if (b < a.t.n_seq) {
             s = sequence(a.t, b, 16 * R);
-            v[0] = a.kv.heads * s.chunks * s.groups;
-            v[1] = a.kv.heads * s.chunks * ((s.groups + 1) >> 1);
+            units = a.kv.heads * s.chunks;
+            v[0] = units * s.groups;
+            v[1] = units * ((s.groups + 1) >> 1);
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
@@ -211,7 +217,7 @@ __device__ __forceinline__ Totals plan(const Args& a, Shared<D, R>& sh) {
         before[0] += sum[0], before[1] += sum[1];
     }
     if (!few) lds_barrier();
-    return Totals{__builtin_amdgcn_readfirstlane(before[0]), __builtin_amdgcn_readfirstlane(before[1])};
+    return Totals{__builtin_amdgcn_readfirstlane(before[0]), __builtin_amdgcn_readfirstlane(before[1]), __builtin_amdgcn_readfirstlane(units)};
 }
 
 // x / y of numbers that all lanes have alike, where the quotient is below 2^20
@@ -355,10 +361,12 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
     // its waves' turns are whole
     const Totals totals = plan<D, R>(a, sh);
     const bool wide = totals.narrow > (int)gridDim.x;
-    const int all = wide ? totals.wide : totals.narrow, used = min((int)gridDim.x, all), group_tiles = GROUP_TILES << (wide ? 1 : 0);
-    if (blockIdx.x == 0 && !a.fuse)
-        for (int i = threadIdx.x; i <= a.t.n_seq + 1; i += THREADS)
-            a.plan[i] = i < a.t.n_seq ? sh.base[wide][i] : i == a.t.n_seq ? all : (int)wide;
+    const int all = wide ? totals.wide : totals.narrow, group_tiles = GROUP_TILES << (wide ? 1 : 0);
+    const int used = used_workgroups(gridDim.x, all, a.t.n_seq, totals.units);
+    if (blockIdx.x == 0 && !a.fuse) {
+        if (threadIdx.x == 0) a.plan[0] = all, a.plan[1] = used, a.plan[2] = wide;
+        for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) a.plan[PLAN_HEAD + i] = sh.base[wide][i];
+    }
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
     const int xcd = blockIdx.x & 7, at_xcd = blockIdx.x >> 3;
     if (at_xcd >= (used >> 3) + (xcd < (used & 7) ? 1 : 0)) return;
@@ -758,23 +766,41 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
     }
 }
 
-// The partial results of the rows whose cache several workgroups shared, a workgroup per row: D / 4 threads hold four
-// dimensions each, 1024 / D such sets take partials in turn, relative to the largest maximum, and are summed in LDS.
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
-    constexpr int V = D / 4, SETS = 256 / V, DEEP = 8;
+// The partial results of the rows whose cache several workgroups shared: a workgroup takes W dimensions of a row, each thread
+// four; the sets of W / 4 threads take partials in turn, relative to the largest maximum, and are summed in LDS. Bound by its
+// trips to memory: the plan, the partials. W is 64 for few rows (of 64 partials 4.6 us against 5.5 with whole rows), and whole
+// rows for many (1536 rows of 5 partials: 8 us against 21).
+template <int D, int W>
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+    constexpr int V = W / 4, SETS = 256 / V, DEEP = 4;
     __shared__ f4 sums[SETS][V];
     const int heads = a.kv.heads * a.t.group, rows = 16 << a.row_tiles;
     const int token = blockIdx.x / heads, h = blockIdx.x - token * heads, head = h / a.t.group;
-    const int lane = threadIdx.x & 63, v4 = threadIdx.x % V, set = threadIdx.x / V;
-    const int all = a.plan[a.t.n_seq], used = min(grid, all);
-    const bool wide = a.plan[a.t.n_seq + 1] != 0;
-    const int b = max(0, find_seq(a.t.start, a.t.n_seq, token));  // the last sequence with start <= token
-    const Seq s = sequence(a.t, b, rows, wide);
+    const int lane = threadIdx.x & 63, set = threadIdx.x / V, d = blockIdx.y * W + threadIdx.x % V * 4;
+    const size_t at = (size_t)blockIdx.x * D + d;
+    const b4 gate = load_gate(a, at);
+    const int all = a.plan[0], used = a.plan[1];
+    const bool wide = a.plan[2] != 0;
+    // the last sequence with start <= token; up to 64 sequences all their numbers are read at once
+    Seq s;
+    int base;
+    if (a.t.n_seq <= 64) {
+        const int mine = min(lane, a.t.n_seq - 1);
+        const Seq one = sequence(a.t, mine, rows, wide);
+        const int first = a.plan[PLAN_HEAD + mine];
+        const int b = max(0, __popcll(__ballot(lane < a.t.n_seq && a.t.start[mine] <= token)) - 1);
+        s.first = __builtin_amdgcn_readlane(one.first, b), s.news = __builtin_amdgcn_readlane(one.news, b);
+        s.chunks = __builtin_amdgcn_readlane(one.chunks, b), s.groups = __builtin_amdgcn_readlane(one.groups, b);
+        base = __builtin_amdgcn_readlane(first, b);
+    } else {
+        const int b = max(0, find_seq(a.t.start, a.t.n_seq, token));
+        s = sequence(a.t, b, rows, wide);
+        base = a.plan[PLAN_HEAD + b];
+    }
     const int node = token - s.first;
     if (node < 0 || node >= s.news) return;
     const int r = node * a.t.group + h - head * a.t.group;
-    const int u0 = a.plan[b] + (head * s.chunks + (r >> (4 + a.row_tiles))) * s.groups, u1 = u0 + s.groups;
+    const int u0 = base + (head * s.chunks + (r >> (4 + a.row_tiles))) * s.groups, u1 = u0 + s.groups;
     const int w0 = group_owner(u0, all, used), parts = group_owner(u1 - 1, all, used) - w0 + 1;
     if (parts == 1) return;  // one workgroup wrote the row
     const int first_slot = partial_slot(w0, u0, all, used), in = r & (rows - 1);
@@ -788,13 +814,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
             const int i = i0 + k * SETS;
             if (i < parts) {
                 m[k] = ml[slot(i)].x;
-                y[k] = *(const f4*)(a.part + slot(i) * D + v4 * 4);
+                y[k] = *(const f4*)(a.part + slot(i) * D + d);
             }
         }
     };
     load(set);
-    const size_t at = (size_t)blockIdx.x * D + v4 * 4;
-    const b4 gate = load_gate(a, at);
     f2 mine = lane < parts ? ml[slot(lane)] : f2{-INFINITY, 0.0f};
     for (int i = lane + 64; i < parts; i += 64) {
         const f2 u = ml[slot(i)];
@@ -803,20 +827,25 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int grid) {
                  (u.x == -INFINITY ? u.y : u.y * __builtin_amdgcn_exp2f(u.x - best));
         mine.x = best;
     }
-    float best = mine.x;
-    for (int o = 32; o; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+    const float best = wave_max(mine.x);
     float total = mine.x == -INFINITY ? mine.y : mine.y * __builtin_amdgcn_exp2f(mine.x - best);
-    for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+    total = row_sum(lanes16([](float x, float y) { return x + y; }, total));
     for (int i0 = set; i0 < parts; i0 += SETS * DEEP) {
 #pragma unroll
         for (int k = 0; k < DEEP; k++)
             if (i0 + k * SETS < parts) v += (m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - best)) * y[k];
         if (i0 + SETS * DEEP < parts) load(i0 + SETS * DEEP);
     }
-    sums[set][v4] = v;
-    lds_barrier();
+    sums[set][threadIdx.x % V] = v;
+    __syncthreads();
     if (set) return;
-    for (int k = 1; k < SETS; k++) v += sums[k][v4];
+    const int there = min(parts, SETS);
+    f4 u[SETS];
+#pragma unroll
+    for (int k = 1; k < SETS; k++) u[k] = sums[k][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < SETS; k++)
+        if (k < there) v += u[k];
     put_out(a, at, v, total, gate);
 }
 
@@ -824,7 +853,10 @@ template <int D, int FMT>
 void launch(hipStream_t stream, const Args& a, int grid, bool join) {
     auto* f = a.row_tiles == 0 ? tree_attn_kernel<D, FMT, 1> : tree_attn_kernel<D, FMT, 2>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(THREADS), 0, stream, a);
-    if (join) hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.t.n * a.kv.heads * a.t.group)), dim3(256), 0, stream, a, grid);
+    if (!join) return;
+    const unsigned rows = (unsigned)(a.t.n * a.kv.heads * a.t.group);
+    if (rows <= 512) hipLaunchKernelGGL((join_kernel<D, 64>), dim3(rows, D / 64), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((join_kernel<D, D>), dim3(rows), dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -872,7 +904,7 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt), units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
     static_assert(3 * MAX_CLUSTER * MAX_CLUSTER <= PF_SK_ITEMS_MAX);
     const size_t part = (size_t)2 * grid * rows * kv->head_dim * 4, ml = (size_t)2 * grid * rows * 8;
-    if (part + ml + (TREE_MAX_SEQS + 2) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
+    if (part + ml + (TREE_MAX_SEQS + PLAN_HEAD) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
     a.row_tiles = rt;
     a.part = (float*)ctx_partials(ctx);
     a.ml_at = (int32_t)part;

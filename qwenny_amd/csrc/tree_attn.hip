@@ -29,7 +29,6 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 8, THREADS = 64 * WAVES;  // of a workgroup: two waves a SIMD
 constexpr int FAN = MAX_CLUSTER;
 constexpr int PLAN_HEAD = 4;
 
@@ -38,7 +37,7 @@ constexpr int BUF_RSRC_WORD3 = 0x00020000;
 constexpr int CPOL_SC1 = 16;
 
 // Workgroups of a CU: what a kernel's registers leave room for.
-constexpr int wgs_per_cu(int d, int r) { return d == 64 && r == 1 ? 2 : 1; }
+constexpr int wgs_per_cu(int d, int r, int w) { return w == 8 ? (d == 64 && r == 1 ? 2 : 1) : d == 64 ? (r == 1 ? 4 : 3) : d == 128 && r == 1 ? 3 : 2; }
 
 struct Args {
     const __bf16* q;     // [n][heads][D]
@@ -141,22 +140,23 @@ __device__ __forceinline__ float sigmoid(float x) {
 }
 
 // What a workgroup of 16 R rows holds in LDS.
-template <int D, int R>
+template <int D, int R, int W>
 struct Shared {
     int32_t base[2][TREE_MAX_SEQS];  // of each sequence: its first group (of 4, of 8 tiles),
     int32_t who[TREE_MAX_SEQS];   // first token | tokens << 20,
     int32_t old[TREE_MAX_SEQS];   // positions before them | (its numbers do not fit) << 31
-    int32_t wave_sum[2][WAVES];
+    int32_t wave_sum[2][W];
     int32_t last;
     float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
-    f4 largest[16 * R][WAVES / 4];        // each wave's largest score of the row,
-    f4 largest_scale[WAVES / 4];          // and largest scale of its values
-    f4 sums[16 * R][WAVES / 2];           // each wave's sum of the row's probabilities, and of their roundings
+    uint64_t sees[16 * R];                // which of its sequence's tokens of this step a row sees
+    f4 largest[16 * R][W / 4];            // each wave's largest score of the row,
+    f4 largest_scale[W / 4];              // and largest scale of its values
+    f4 sums[16 * R][W / 2];               // each wave's sum of the row's probabilities, and of their roundings
     h8 q[R][D / 64][2][64];
-    float tile_scale[WAVES][2][KV_TILE];
+    float tile_scale[W][2][KV_TILE];
     union {
-        h8 p[WAVES][R][2][64];  // probabilities of each wave's tile
-        f4 half[R][WAVES / 2][64];
+        h8 p[W][R][2][64];  // probabilities of each wave's tile
+        f4 half[R][W / 2][64];
         struct {
             float weight[FAN][16];
             f2 row[16];  // the joined maximum and sum
@@ -169,8 +169,9 @@ struct Shared {
 struct Totals {
     int narrow, wide, units;  // (units: of the first sequence)
 };
-template <int D, int R>
-__device__ __forceinline__ Totals plan(const Args& a, Shared<D, R>& sh) {
+template <int D, int R, int W>
+__device__ __forceinline__ Totals plan(const Args& a, Shared<D, R, W>& sh) {
+    constexpr int THREADS = 64 * W;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool few = a.t.n_seq <= 64;
     int before[2] = {0, 0}, units = 0;
@@ -200,7 +201,7 @@ __device__ __forceinline__ Totals plan(const Args& a, Shared<D, R>& sh) {
             if (lane == 0) sh.wave_sum[0][wave] = sum[0], sh.wave_sum[1][wave] = sum[1];
             lds_barrier();
             sum[0] = sum[1] = 0;
-            for (int w = 0; w < WAVES; w++)
+            for (int w = 0; w < W; w++)
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     if (w < wave) run[k] += sh.wave_sum[k][w];
@@ -253,10 +254,10 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
 
 // `count` partial results of one unit, those of workgroups w0, w0 + step, .., summed relative to their largest maximum in
 // that order: into the outputs (`out`), or back into the first one's place. (Chunks of 16 rows.)
-template <int D, class Row>
-__device__ __forceinline__ void join_parts(const Args& a, Shared<D, 1>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
+template <int D, int W, class Row>
+__device__ __forceinline__ void join_parts(const Args& a, Shared<D, 1, W>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
                                            int count, int live, bool out, Row&& row_of) {
-    constexpr int V = D / 4, DEEP = 24;
+    constexpr int V = D / 4, DEEP = 24, THREADS = 64 * W;
     static_assert(FAN == 32);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // what follows from it is made here, not kept in registers over the whole kernel
@@ -344,14 +345,15 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int of, int32_t* flag
 // workgroup's part and one at its end. They are summed in their order by join_kernel, or (`fuse`) here: each workgroup
 // writes its own (device-coherent stores) and counts itself, and the last to arrive sums them; from more than 16 on in two
 // steps, clusters of neighbours and then the clusters' sums. No workgroup waits for another.
-template <int D, int FMT, int R>
-__global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kernel(const Args a) {
+template <int D, int FMT, int R, int W>
+__global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args a) {
+    constexpr int WAVES = W, THREADS = 64 * W;
     // a wave's share of the values: SL sixteenths of the dimensions, of VT of a group's tiles
     constexpr int C = D / 64, DT = D / 16, ROWS = 16 * R, SPLIT = DT < WAVES ? WAVES / DT : 1, SL = DT * SPLIT / WAVES, VT = WAVES / SPLIT;
     constexpr int CHAINS = R == 1 ? 2 : 1;  // sums of an output, so that products need not wait for one another
     constexpr bool EARLY = R == 1 || D < 256;  // registers for a group's values beside its keys
     constexpr uint32_t NONE = ~0u;
-    __shared__ Shared<D, R> sh;
+    __shared__ Shared<D, R, W> sh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // all lines of the arguments are fetched at once: each is a trip to memory when first touched
     const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
     static_assert(sizeof(Args) > 128);
     // groups of four tiles where there are few, so that they reach more CUs; of eight where a workgroup has several, so that
     // its waves' turns are whole
-    const Totals totals = plan<D, R>(a, sh);
+    const Totals totals = plan<D, R, W>(a, sh);
     const bool wide = totals.narrow > (int)gridDim.x;
     const int all = wide ? totals.wide : totals.narrow, group_tiles = GROUP_TILES << (wide ? 1 : 0);
     const int used = used_workgroups(gridDim.x, all, a.t.n_seq, totals.units);
@@ -411,17 +413,14 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
         constexpr int PER_ROW = D / 16, PASS = THREADS / PER_ROW;
         const int q_row = tid / PER_ROW, q_part = tid % PER_ROW;
         b8 raw[2];
+        uint64_t mask;
         auto load_query = [&](int r) {
-            const __bf16* const qp = a.q + row_at(min(r, live - 1)) + q_part * 16;
+            const int row = min(r, live - 1), node = node_of(row0 + row);
+            const __bf16* const qp = a.q + row_at(row) + q_part * 16;
             raw[0] = *(const b8*)qp, raw[1] = *(const b8*)(qp + 8);
+            mask = a.mask ? a.mask[first + node] : ~0ull >> (63 - node);
         };
         load_query(q_row);
-        uint64_t sees[R];  // of its sequence's tokens of this step
-#pragma unroll
-        for (int rt = 0; rt < R; rt++) {
-            const int node = node_of(row0 + min(rt * 16 + col, live - 1));
-            sees[rt] = (a.mask ? a.mask[first + node] : ~0ull >> (63 - node)) & ~0ull >> (64 - news);
-        }
 
         u4 kc[4][C], vc[VT][SL];
         float sk, sv;
@@ -492,6 +491,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                                        ? NAN
                                        : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
                     sh.start[r] = -0x1p-17f * sum;
+                    sh.sees[r] = mask & ~0ull >> (64 - news);
                 }
             }
             r += PASS;
@@ -499,12 +499,11 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
             load_query(r);
         }
         lds_barrier();
-        float factor[R], top[R], sum[R], rounded[R];  // rounded: the sum of the probabilities as they are multiplied
+        float top[R], sum[R], rounded[R];  // rounded: the sum of the probabilities as they are multiplied
         f4 o[R][SL][CHAINS];
         float ref = 0x1p-126f;  // the values' scales are taken relative to this power of two: probabilities fit f16
 #pragma unroll
         for (int rt = 0; rt < R; rt++) {
-            factor[rt] = sh.factor[rt * 16 + col];
             top[rt] = -INFINITY, sum[rt] = rounded[rt] = 0.0f;
 #pragma unroll
             for (int i = 0; i < SL; i++)
@@ -560,7 +559,8 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 uint64_t seen = 0;  // bit i: the row sees token t0 + i
                 if (own && !whole) {
                     const int node = t0 - old;  // above -64
-                    seen = node >= 64 ? 0 : node >= 0 ? sees[rt] >> node : sees[rt] << -node | ((1ull << -node) - 1);
+                    const uint64_t sees = sh.sees[rt * 16 + col];
+                    seen = node >= 64 ? 0 : node >= 0 ? sees >> node : sees << -node | ((1ull << -node) - 1);
                 }
                 float mx = -INFINITY;
 #pragma unroll
@@ -582,8 +582,13 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
             lds_barrier();
 
             // the values' scales relative to ref; ref grows to the largest finite one's power of two
-            f4 lg = sh.largest_scale[0], lg2 = sh.largest_scale[1];
-            most = fmaxf(fmaxf(fmaxf(lg.x, lg.y), fmaxf(lg.z, lg.w)), fmaxf(fmaxf(lg2.x, lg2.y), fmaxf(lg2.z, lg2.w)));
+            const auto over = [](const f4(&v)[W / 4]) {
+                float m = fmaxf(fmaxf(v[0].x, v[0].y), fmaxf(v[0].z, v[0].w));
+#pragma unroll
+                for (int k = 1; k < W / 4; k++) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+                return m;
+            };
+            most = over(sh.largest_scale);
             float grow = 1.0f;
             if (__any(most > ref)) {
                 const int e = min(__builtin_amdgcn_frexp_expf(most), 127);
@@ -593,13 +598,12 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
             const float inv_ref = __builtin_amdgcn_rcpf(ref);  // (exact: a power of two)
 #pragma unroll
             for (int rt = 0; rt < R; rt++) {
-                lg = sh.largest[rt * 16 + col][0], lg2 = sh.largest[rt * 16 + col][1];
-                const float next = fmaxf(top[rt], fmaxf(fmaxf(fmaxf(lg.x, lg.y), fmaxf(lg.z, lg.w)),
-                                                        fmaxf(fmaxf(lg2.x, lg2.y), fmaxf(lg2.z, lg2.w))));
+                const float next = fmaxf(top[rt], over(sh.largest[rt * 16 + col]));
+                const float factor = sh.factor[rt * 16 + col];
                 // the maximum is followed only where it has grown by more than 2^8 (the sums and f16 hold that)
                 float by = grow;
-                if (__any((next - top[rt]) * factor[rt] > 8.0f)) {
-                    const float al = next > top[rt] ? __builtin_amdgcn_exp2f((top[rt] - next) * factor[rt]) : 1.0f;
+                if (__any((next - top[rt]) * factor > 8.0f)) {
+                    const float al = next > top[rt] ? __builtin_amdgcn_exp2f((top[rt] - next) * factor) : 1.0f;
                     sum[rt] *= al;
                     top[rt] = next;
                     by *= al;
@@ -619,7 +623,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                     float pv[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float pr = __builtin_amdgcn_exp2f((x[rt][sub][i] - off) * factor[rt]);
+                        const float pr = __builtin_amdgcn_exp2f((x[rt][sub][i] - off) * factor);
                         pv[i] = pr * vs[i];
                         if (!whole) pv[i] = x[rt][sub][i] == -INFINITY ? 0.0f : pv[i];
                         sum[rt] += pr;
@@ -690,8 +694,9 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 const f2 s = {row_sum(sum[rt]), FMT == QH_KV_I8 ? row_sum(rounded[rt]) : 0.0f};
                 if (g == 0) ((f2*)sh.sums[rt * 16 + col])[wave] = s;
             }
+            constexpr bool AHEAD = R * SL <= 4;  // (registers)
             b4 gate[R][SL];
-            if (direct)
+            if (AHEAD && direct)
 #pragma unroll
                 for (int rt = 0; rt < R; rt++)
 #pragma unroll
@@ -728,7 +733,8 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                     if (r >= live) continue;
                     if (direct) {
 #pragma unroll
-                        for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt], gate[rt][i]);
+                        for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt],
+                                AHEAD ? gate[rt][i] : load_gate(a, row_at(r) + (slice + i) * 16 + g * 4));
                     } else {
 #pragma unroll
                         for (int i = 0; i < SL; i++)
@@ -736,7 +742,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                                                                    (uint32_t)((slot * ROWS + r) * D + (slice + i) * 16 + g * 4) * 4, 0, CPOL_SC1);
                         if (wave == 0 && g == 0)
                             __builtin_amdgcn_raw_buffer_store_b64(
-                                __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * factor[rt], sum[rt]})), rsrc,
+                                __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * sh.factor[r], sum[rt]})), rsrc,
                                 a.ml_at + (uint32_t)(slot * ROWS + r) * 8, 0, CPOL_SC1);
                     }
                 }
@@ -752,7 +758,7 @@ __global__ __launch_bounds__(THREADS, 2 * wgs_per_cu(D, R)) void tree_attn_kerne
                 for (bool out = k.of == 1;;) {
                     if (count > 1) {
                         if (!last_of(counter, count, &sh.last)) break;
-                        join_parts<D>(a, sh, rsrc, first_slot, from, step, count, live, out, row_at);
+                        join_parts<D, W>(a, sh, rsrc, first_slot, from, step, count, live, out, row_at);
                     }
                     if (out) break;
                     from = w0, first_slot = partial_slot(w0, u0, all, used), step = k.step, count = k.of;
@@ -850,9 +856,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 }
 
 template <int D, int FMT>
-void launch(hipStream_t stream, const Args& a, int grid, bool join) {
-    auto* f = a.row_tiles == 0 ? tree_attn_kernel<D, FMT, 1> : tree_attn_kernel<D, FMT, 2>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(THREADS), 0, stream, a);
+void launch(hipStream_t stream, const Args& a, int waves, int grid, bool join) {
+    auto* f = a.row_tiles == 0 ? (waves == 8 ? tree_attn_kernel<D, FMT, 1, 8> : tree_attn_kernel<D, FMT, 1, 4>)
+                               : waves == 8 ? tree_attn_kernel<D, FMT, 2, 8> : tree_attn_kernel<D, FMT, 2, 4>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(64 * waves), 0, stream, a);
     if (!join) return;
     const unsigned rows = (unsigned)(a.t.n * a.kv.heads * a.t.group);
     if (rows <= 512) hipLaunchKernelGGL((join_kernel<D, 64>), dim3(rows, D / 64), dim3(256), 0, stream, a);
@@ -890,6 +897,13 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     int rt = 0;
     while (rt < 1 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= cus) rt++;
     const int rows = 16 << rt;
+    // Workgroups of eight waves, or twice as many of four: those start sooner (4,099 positions of 32 x 128: 10.1 us against 11.5,
+    // of 24 x 256 13.5 against 13.8) and are out of step with one another, so that one's products run beside another's softmax
+    // (8 sequences of 8 tokens, 32 x 128: 20.6 against 27.9; 64 tokens at 8,150, 24 x 256: 43.0 against 46.0), but they leave
+    // twice the partial results (131,000 positions 61.7 against 59.6, 5 tokens at 32,700 27.8 against 24.1).
+    const int64_t total = units_of(rt) * step->n_seq * groups;
+    const bool four = rt == 0 ? total <= cus : kv->head_dim < 256 || (step->max_new * group > 128 && total >= 4 * cus);
+    const int waves = four ? 4 : 8;
     const int64_t units = units_of(rt);
     if (units * step->n_seq > 0x7fffffff / groups)
         return fail(QH_EINVAL, "tree_attn: %d sequences of up to %lld positions are too many for one call", step->n_seq, (long long)cap);
@@ -901,7 +915,7 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     a.mask = step->mask;
     a.group_inv = ((1u << 20) + group - 1) / group;
     a.scale = scale * 1.4426950408889634f;
-    const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt), units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
+    const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt, waves), units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
     static_assert(3 * MAX_CLUSTER * MAX_CLUSTER <= PF_SK_ITEMS_MAX);
     const size_t part = (size_t)2 * grid * rows * kv->head_dim * 4, ml = (size_t)2 * grid * rows * 8;
     if (part + ml + (TREE_MAX_SEQS + PLAN_HEAD) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
@@ -913,8 +927,8 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     a.fuse = rt == 0;
     const bool join = !a.fuse && groups > 1 && grid > 1;
     auto go = [&](auto d) {
-        if (kv->fmt == QH_KV_I8) launch<decltype(d)::value, QH_KV_I8>((hipStream_t)stream, a, grid, join);
-        else launch<decltype(d)::value, QH_KV_E4M3>((hipStream_t)stream, a, grid, join);
+        if (kv->fmt == QH_KV_I8) launch<decltype(d)::value, QH_KV_I8>((hipStream_t)stream, a, waves, grid, join);
+        else launch<decltype(d)::value, QH_KV_E4M3>((hipStream_t)stream, a, waves, grid, join);
     };
     if (kv->head_dim == 64) go(std::integral_constant<int, 64>{});
     else if (kv->head_dim == 128) go(std::integral_constant<int, 128>{});

@@ -346,7 +346,7 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int of, int32_t* flag
 // writes its own (device-coherent stores) and counts itself, and the last to arrive sums them; from more than 16 on in two
 // steps, clusters of neighbours and then the clusters' sums. No workgroup waits for another.
 template <int D, int FMT, int R, int W>
-__global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args a) {
+__global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args args) {
     constexpr int WAVES = W, THREADS = 64 * W;
     // a wave's share of the values: SL sixteenths of the dimensions, of VT of a group's tiles
     constexpr int C = D / 64, DT = D / 16, ROWS = 16 * R, SPLIT = DT < WAVES ? WAVES / DT : 1, SL = DT * SPLIT / WAVES, VT = WAVES / SPLIT;
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     constexpr bool EARLY = R == 1 || D < 256;  // registers for a group's values beside its keys
     constexpr uint32_t NONE = ~0u;
     __shared__ Shared<D, R, W> sh;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Args& a = args;
     // all lines of the arguments are fetched at once: each is a trip to memory when first touched
     const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
@@ -363,24 +363,29 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     // its waves' turns are whole
     const Totals totals = plan<D, R, W>(a, sh);
     const bool wide = totals.narrow > (int)gridDim.x;
-    const int all = wide ? totals.wide : totals.narrow, group_tiles = GROUP_TILES << (wide ? 1 : 0);
-    const int used = used_workgroups(gridDim.x, all, a.t.n_seq, totals.units);
+    const int groups_in_all = wide ? totals.wide : totals.narrow;
+    const int workgroups = __builtin_amdgcn_readfirstlane(used_workgroups(gridDim.x, groups_in_all, a.t.n_seq, totals.units));
     if (blockIdx.x == 0 && !a.fuse) {
-        if (threadIdx.x == 0) a.plan[0] = all, a.plan[1] = used, a.plan[2] = wide;
+        if (threadIdx.x == 0) a.plan[0] = groups_in_all, a.plan[1] = workgroups, a.plan[2] = wide;
         for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) a.plan[PLAN_HEAD + i] = sh.base[wide][i];
     }
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
     const int xcd = blockIdx.x & 7, at_xcd = blockIdx.x >> 3;
-    if (at_xcd >= (used >> 3) + (xcd < (used & 7) ? 1 : 0)) return;
-    const int w = xcd * (used >> 3) + min(xcd, used & 7) + at_xcd;
+    if (at_xcd >= (workgroups >> 3) + (xcd < (workgroups & 7) ? 1 : 0)) return;
+    const int workgroup = xcd * (workgroups >> 3) + min(xcd, workgroups & 7) + at_xcd;
     // (what all lanes have alike is said to be so where it comes through LDS or a division: addresses are then scalar)
-    const int lo = __builtin_amdgcn_readfirstlane(first_group(w, all, used));
-    const int hi = __builtin_amdgcn_readfirstlane(first_group(w + 1, all, used));
+    const int lo = __builtin_amdgcn_readfirstlane(first_group(workgroup, groups_in_all, workgroups));
+    const int hi = __builtin_amdgcn_readfirstlane(first_group(workgroup + 1, groups_in_all, workgroups));
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int)PF_SK_PART_BYTES, BUF_RSRC_WORD3);
     for (int at = lo; at < hi;) {
-        // (said anew in each turn, so that nothing that follows is kept in registers across them: most workgroups take one)
-        int tid = threadIdx.x, page_shift = a.kv.page_shift;
-        asm volatile("" : "+v"(tid), "+s"(page_shift));
+        // (said anew in each turn, so that nothing that follows is kept in registers across them: most workgroups take one. The
+        // arguments are read again where they are used.)
+        int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        int all = groups_in_all, used = workgroups, w = __builtin_amdgcn_readfirstlane(workgroup), group_tiles = __builtin_amdgcn_readfirstlane(GROUP_TILES << (wide ? 1 : 0));
+        const auto* again = line;
+        asm volatile("" : "+v"(tid), "+s"(wave), "+s"(all), "+s"(used), "+s"(w), "+s"(group_tiles), "+s"(again));
+        const Args& a = *(const Args*)again;
+        const int page_shift = a.kv.page_shift;
         const int lane = tid & 63, col = lane & 15, g = lane >> 4, page_tiles = 1 << (page_shift - 6);
         const int b = find_seq(sh.base[wide], a.t.n_seq, at);
         const int who = __builtin_amdgcn_readfirstlane(sh.who[b]), was = __builtin_amdgcn_readfirstlane(sh.old[b]);

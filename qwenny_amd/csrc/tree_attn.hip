@@ -891,6 +891,8 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(QH_EINVAL, "tree_attn: scale %g must be positive", scale);
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)gate % 16)
         return fail(QH_EINVAL, "tree_attn: q, gate and out must be 16-byte aligned");
+    if ((uint64_t)a.kv.slots / KV_TILE * 2 * kv->heads >= 0xffffffffu)  // (a tile's place is a 32-bit number)
+        return fail(QH_EINVAL, "tree_attn: a cache of %zu pages of %d tokens of %d heads is too large", kv->pages, kv->page, kv->heads);
     const int64_t cap = (int64_t)step->table_ld * kv->page;  // positions that a table can name
     if (step->table_ld < 1 || step->table_ld > ((size_t)1 << 30) / kv->page)
         return fail(QH_EINVAL, "tree_attn: tables of %zu pages of %d tokens (1 to 2^30 positions)", step->table_ld, kv->page);

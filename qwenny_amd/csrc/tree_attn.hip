@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                                                      BUF_RSRC_WORD3);
         };
         auto piece = [&](__amdgpu_buffer_rsrc_t tile, int at) {
-            return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, 0));
+            return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, R == 1 ? 2 : 0));
         };
         // the wave's tile's keys and scales (lane l: token l's); a page that the cache has not gives NaN
         auto load_keys = [&](int t8) {

@@ -67,6 +67,14 @@ def _ptr(t):
         return int(t)
 
 
+def _ptrs(*tensors):
+    """_ptr of each: a call's tensors at once, which takes half the time of one by one."""
+    try:
+        return [t if t is None else t.data_ptr() for t in tensors]
+    except AttributeError:
+        return [_ptr(t) for t in tensors]
+
+
 _raw_stream = None  # () -> torch's current stream of the current device, as an address
 
 
@@ -210,7 +218,8 @@ class Gemm:
         out bf16 [n][q_heads * head_dim], times sigmoid(gate) where a gate (bf16, as q) is given; scale: head_dim ** -0.5
         by default."""
         s = kv.head_dim ** -0.5 if scale is None else scale
-        check(lib().qh_tree_attn(self._ctx, _stream(stream), _ptr(q), q_heads, kv.c, step.c, s, _ptr(gate), _ptr(out)))
+        q, gate, out = _ptrs(q, gate, out)
+        check(lib().qh_tree_attn(self._ctx, _stream(stream), q, q_heads, kv.c, step.c, s, gate, out))
 
     def put_block(self, stream, m, q, zeros, block, rows):
         """Write stored rows `rows` (16) of `q` as the 16-row block `block` of a matrix from Mat.marlin_rows, counting
@@ -518,24 +527,28 @@ def attn_prep(stream, x, splits, n, rows, q_w, k_w, inv_freq, pos, q, gate=None,
     """The consumer of the attention in-projection (kernels/qwen.cu:156-202): its partials x [splits][n][rows] summed,
     queries and keys normed per head (q_w, k_w f32 or None) and rotated to positions pos by pos * inv_freq; q and gate
     bf16 [n][q_heads][head_dim]; keys and values into `slots` of the cache `kv`, or as bf16 to k, v."""
-    check(lib().qh_attn_prep(_stream(stream), _ptr(x), splits, n, rows.c, _ptr(q_w), _ptr(k_w), eps, _ptr(inv_freq), _ptr(pos),
-                             _ptr(q), _ptr(gate), None if kv is None else kv.c, _ptr(slots), _ptr(k), _ptr(v)))
+    x, q_w, k_w, inv_freq, pos, q, gate, slots, k, v = _ptrs(x, q_w, k_w, inv_freq, pos, q, gate, slots, k, v)
+    check(lib().qh_attn_prep(_stream(stream), x, splits, n, rows.c, q_w, k_w, eps, inv_freq, pos, q, gate,
+                             None if kv is None else kv.c, slots, k, v))
 
 
 def kv_write(stream, kv, k, v, slots, n):
     """k, v bf16 [n][heads][head_dim] quantised into the cache's slots (int32 [n], distinct)."""
-    check(lib().qh_kv_write(_stream(stream), kv.c, _ptr(k), _ptr(v), _ptr(slots), n))
+    check(lib().qh_kv_write(_stream(stream), kv.c, *_ptrs(k, v, slots), n))
 
 
 def kv_read(stream, kv, slots, n, k, v):
     """The keys and values of slots (int32 [n]) as bf16 [n][heads][head_dim]."""
-    check(lib().qh_kv_read(_stream(stream), kv.c, _ptr(slots), n, _ptr(k), _ptr(v)))
+    slots, k, v = _ptrs(slots, k, v)
+    check(lib().qh_kv_read(_stream(stream), kv.c, slots, n, k, v))
 
 
 def kv_move(stream, kv, src, dst, start, n_seq, n=None):
     """Codes and scales of slots src to slots dst (int32 [n]), sequence b's moves start[b] .. start[b + 1] read before they
     are written: an accepted path's slots put together."""
-    check(lib().qh_kv_move(_stream(stream), kv.c, _ptr(src), _ptr(dst), src.numel() if n is None else n, _ptr(start), n_seq))
+    n = src.numel() if n is None else n
+    src, dst, start = _ptrs(src, dst, start)
+    check(lib().qh_kv_move(_stream(stream), kv.c, src, dst, n, start, n_seq))
 
 
 def pack_dense_bf16(w_bf16, order):

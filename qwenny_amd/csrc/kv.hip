@@ -460,7 +460,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; i++) ss += y[i] * y[i];
-            const float r = 1.0f / sqrtf(wave_sum(ss) / (float)D + a.eps);
+            // (rsqrt to a unit in the last place: below the rounding of the mean's own sum)
+            const float r = __builtin_amdgcn_rsqf(wave_sum(ss) * (1.0f / D) + a.eps);
 #pragma unroll
             for (int i = 0; i < V; i++) y[i] = w[lane * V + i] * (y[i] * r);
         }

@@ -10,6 +10,7 @@ constexpr int KV_TILE = 64;          // tokens of a tile; pages are a multiple o
 constexpr int GROUP_TILES = 4;       // tiles of a group, a workgroup's smallest part: one for each of its waves
 constexpr int TREE_MAX_SEQS = 1024;  // sequences of a step
 constexpr int TREE_MAX_NEW = 64;     // tokens of one sequence in a step: a mask is 64 bits
+constexpr int TREE_MAX_WGS = 1024;   // workgroups of a launch
 
 struct TreeArrays {
     const int32_t* start;  // [n_seq + 1]
@@ -48,7 +49,7 @@ constexpr Seq sequence(const TreeArrays& a, int b, int rows, bool wide = false) 
 
 // `all` groups in a row (sequence by sequence, kv head by kv head, chunk by chunk) in equal parts for `used` <= all
 // workgroups: the first group of workgroup w, the workgroup of group `at`.
-// (w all / used and (used (at + 1) - 1) / all, without 64-bit divisions: used <= 1024)
+// (w all / used and (used (at + 1) - 1) / all, without 64-bit divisions: used <= TREE_MAX_WGS)
 constexpr int first_group(int w, int all, int used) {
     return used == all ? w : w * (all / used) + w * (all % used) / used;
 }
@@ -70,19 +71,5 @@ constexpr int used_workgroups(int grid, int all, int n_seq, int units) {
 // Where workgroup w keeps its partial result of the unit (sequence, kv head, chunk) whose groups begin at u0: it has at most
 // two, the unit that its part begins in and the one that it ends in.
 constexpr int partial_slot(int w, int u0, int all, int used) { return 2 * w + (first_group(w, all, used) < u0 ? 1 : 0); }
-
-// How `parts` partial results of a unit are summed: few by the last of all to arrive; more in `of` clusters of
-// `step` neighbours (the last has what is left), then the clusters' sums. The cluster of part i.
-constexpr int MAX_CLUSTER = 32;  // (its square is no less than the workgroups of a launch)
-struct Cluster {
-    int first, size, step, of;
-};
-constexpr Cluster cluster(int i, int parts) {
-    int step = parts;
-    if (parts > 24)
-        for (step = 2; step * step < parts;) step++;
-    const int first = i / step * step;
-    return Cluster{first, step < parts - first ? step : parts - first, step, (parts + step - 1) / step};
-}
 
 }  // namespace qh

@@ -26,18 +26,16 @@ typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int FAN = MAX_CLUSTER;
 constexpr int PLAN_HEAD = 4;
 
-// buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of agent-coherent loads and stores
+// buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of loads past the caches
 constexpr int BUF_RSRC_WORD3 = 0x00020000;
-constexpr int CPOL_SC1 = 16;
+constexpr int CPOL_NT = 2;
 
 // Workgroups of a CU: what a kernel's registers leave room for.
-constexpr int wgs_per_cu(int d, int r, int w) { return w == 8 ? (d == 64 && r == 1 ? 2 : 1) : d == 64 ? (r == 1 ? 4 : 3) : d == 128 && r == 1 ? 3 : 2; }
+constexpr int wgs_per_cu(int d, int r, int w) { return w == 8 ? 1 : d == 64 ? (r == 1 ? 4 : 3) : d == 128 && r == 1 ? 3 : 2; }
 
 struct Args {
     const __bf16* q;     // [n][heads][D]
@@ -50,11 +48,9 @@ struct Args {
     float scale;           // softmax scale * log2(e)
     uint32_t group_inv;    // 2^20 / group rounded up: (r * group_inv) >> 20 is r / group for the rows r < 64 group <= 4096
     int32_t row_tiles;     // log2 of a chunk's tiles of 16 rows
-    int32_t fuse;          // partial results are summed by the last workgroup to arrive, else by join_kernel
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
     int32_t* plan;         // for join_kernel: groups, workgroups, whether the groups are wide; each sequence's first group
-    uint32_t* count;       // [3 * workgroups] arrivals, zero between launches: of clusters by slot, then of units
 };
 
 // The compiler moves nothing across: left free it converts a whole tile's codes ahead of its products and spills.
@@ -123,18 +119,11 @@ __device__ __forceinline__ float wave_max(float v) {
     return row_max(v);
 }
 
-// f over the 16 lanes of each quarter of the wave, over the 32 of each half
+// f over the 16 lanes of each quarter of the wave
 template <class F>
 __device__ __forceinline__ float lanes16(F&& f, float v) {
     return __int_as_float(over_lanes<16>(__float_as_int(v), [&](int x, int y) { return __float_as_int(f(__int_as_float(x), __int_as_float(y))); }));
 }
-template <class F>
-__device__ __forceinline__ float lanes32(F&& f, float v) {
-    v = lanes16(f, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-
 __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
@@ -146,7 +135,6 @@ struct Shared {
     int32_t who[TREE_MAX_SEQS];   // first token | tokens << 20,
     int32_t old[TREE_MAX_SEQS];   // positions before them | (its numbers do not fit) << 31
     int32_t wave_sum[2][W];
-    int32_t last;
     float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
     uint64_t sees[16 * R];                // which of its sequence's tokens of this step a row sees
     f4 largest[16 * R][W / 4];            // each wave's largest score of the row,
@@ -154,14 +142,7 @@ struct Shared {
     f4 sums[16 * R][W / 2];               // each wave's sum of the row's probabilities, and of their roundings
     h8 q[R][D / 64][2][64];
     float tile_scale[W][2][KV_TILE];
-    union {
-        h8 p[W][R][2][64];  // probabilities of each wave's tile
-        f4 half[R][W / 2][64];
-        struct {
-            float weight[FAN][16];
-            f2 row[16];  // the joined maximum and sum
-        } parts;
-    };
+    h8 p[W][R][2][64];  // probabilities of each wave's tile
 };
 
 // The sequences' places in LDS, and the number of their groups: of four tiles in .x, of eight in .y. Up to 64 sequences each
@@ -252,104 +233,22 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
     *(b4*)(a.out + at) = __builtin_convertvector(v, b4);
 }
 
-// `count` partial results of one unit, those of workgroups w0, w0 + step, .., summed relative to their largest maximum in
-// that order: into the outputs (`out`), or back into the first one's place. (Chunks of 16 rows.)
-template <int D, int W, class Row>
-__device__ __forceinline__ void join_parts(const Args& a, Shared<D, 1, W>& sh, __amdgpu_buffer_rsrc_t rsrc, int first_slot, int w0, int step,
-                                           int count, int live, bool out, Row&& row_of) {
-    constexpr int V = D / 4, DEEP = 24, THREADS = 64 * W;
-    static_assert(FAN == 32);
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));  // what follows from it is made here, not kept in registers over the whole kernel
-    auto slot = [&](int i) { return i == 0 ? first_slot : 2 * (w0 + i * step); };
-    const int part = tid % FAN;  // whose maxima and sums the thread takes, of every PASS-th row
-    constexpr int PASS = THREADS / FAN;
-    f2 ml[16 / PASS];
-#pragma unroll
-    for (int k = 0; k < 16 / PASS; k++) {
-        ml[k] = f2{-INFINITY, 0.0f};
-        if (part < count)
-            ml[k] = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(
-                                               rsrc, a.ml_at + ((uint32_t)slot(part) * 16 + k * PASS + tid / FAN) * 8, 0, CPOL_SC1));
-    }
-    // (rows that are not there are loads past the buffer's end: they read nothing)
-    f4 in[DEEP];
-    constexpr uint32_t PAST = 0x40000000;
-    static_assert(PF_SK_PART_BYTES <= PAST);
-    auto load = [&](int e, int i0) {
-        const uint32_t at = e < live * V ? e * 16 : PAST;
-#pragma unroll
-        for (int k = 0; k < DEEP; k++)
-            if (i0 + k < count)
-                in[k] = __builtin_bit_cast(
-                    f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, slot(i0 + k) * (16 * D * 4), CPOL_SC1));
-    };
-    auto place = [&](int e) { return row_of(min(e / V, live - 1)) + e % V * 4; };
-    b4 gate = out ? load_gate(a, place(tid)) : b4{};
-    load(tid, 0);
-#pragma unroll
-    for (int k = 0; k < 16 / PASS; k++) {
-        const int row = k * PASS + tid / FAN;
-        const float best = lanes32([](float x, float y) { return fmaxf(x, y); }, ml[k].x);
-        const float weight = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - best);
-        // (without a maximum: 0 or NaN)
-        const float total = lanes32([](float x, float y) { return x + y; }, ml[k].x == -INFINITY ? ml[k].y : ml[k].y * weight);
-        sh.parts.weight[part][row] = weight;
-        if (part == 0) sh.parts.row[row] = f2{best, total};
-    }
-    lds_barrier();
-    for (int e = tid; e < live * V; e += THREADS) {
-        const size_t at = place(e);
-        if (e != tid && out) gate = load_gate(a, at);
-        f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i0 = 0; i0 < count; i0 += DEEP) {
-            if (e != tid || i0) load(e, i0);
-            int there = count;
-            asm volatile("" : "+s"(there));  // compared anew: the loads' comparisons kept would be two registers each
-#pragma unroll
-            for (int k = 0; k < DEEP; k++)
-                if (i0 + k < there) sum += sh.parts.weight[i0 + k][e / V] * in[k];
-        }
-        if (out) put_out(a, at, sum, sh.parts.row[e / V].y, gate);
-        else
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, sum), rsrc, (uint32_t)first_slot * (16 * D * 4) + e * 16, 0,
-                                                   CPOL_SC1);
-    }
-    if (!out && tid < live)
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, sh.parts.row[tid]), rsrc,
-                                              a.ml_at + ((uint32_t)first_slot * 16 + tid) * 8, 0, CPOL_SC1);
-}
-
-// Whether this workgroup is the last of `of` to come here since the counter was zero; it sets it back to zero.
-__device__ __forceinline__ bool last_of(uint32_t* counter, int of, int32_t* flag) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's partial has been performed
-    lds_barrier();
-    if (threadIdx.x == 0) {
-        const bool l = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(of - 1);
-        if (l) (void)__hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = l;
-    }
-    lds_barrier();
-    return *flag != 0;
-}
-
 // The work is a row of groups: for each sequence, kv head and chunk of 16 R rows, the cache in groups of 4 x 64 tokens. The
 // workgroups share it in equal parts, across the borders of sequences; consecutive parts on one XCD, whose L2 then serves
-// the chunks that read the same cache. Eight tiles at a time, each of the eight waves makes the scores of one tile for all rows; the
-// waves agree on the rows' largest scores, put their probabilities into LDS, and each then multiplies all eight tiles' by
+// the chunks that read the same cache. A tile for each wave at a time, a wave makes the scores of its own for all rows; the
+// waves agree on the rows' largest scores, put their probabilities into LDS, and each then multiplies those of all tiles by
 // its own share of the values' dimensions. So a code is read and converted once for all rows, a wave's part of the outputs
 // is small, and there is nothing to join over the waves but the sums. (Each wave with whole rows and tiles of its own, joined
 // over LDS, took 12.0 us against 10.3 for a short sequence, 45 against 33 for 64 drafted tokens at 8,150.) Keys are read a
 // group ahead, values too or while the scores are made.
-// What covers a sequence's whole cache is written out, the rest as partial results: at most one at the start of a
-// workgroup's part and one at its end. They are summed in their order by join_kernel, or (`fuse`) here: each workgroup
-// writes its own (device-coherent stores) and counts itself, and the last to arrive sums them; from more than 16 on in two
-// steps, clusters of neighbours and then the clusters' sums. No workgroup waits for another.
+// What covers a sequence's whole cache is written out, the rest as partial results for join_kernel: at most one at the start
+// of a workgroup's part and one at its end. (Summed by the last workgroup of a row to arrive instead, without a second launch:
+// one workgroup reads them all then, and waits for stores and counters first. One token at 4,099 positions 13.7 us against
+// 12.8, at 16,000 18.7 against 15.3, at 131,000 54.5 against 51.9.)
 template <int D, int FMT, int R, int W>
 __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args args) {
-    constexpr int WAVES = W, THREADS = 64 * W;
-    // a wave's share of the values: SL sixteenths of the dimensions, of VT of a group's tiles
-    constexpr int C = D / 64, DT = D / 16, ROWS = 16 * R, SPLIT = DT < WAVES ? WAVES / DT : 1, SL = DT * SPLIT / WAVES, VT = WAVES / SPLIT;
+    constexpr int THREADS = 64 * W;
+    constexpr int C = D / 64, ROWS = 16 * R, SL = D / 16 / W;  // SL: sixteenths of the dimensions that a wave multiplies
     constexpr int CHAINS = R == 1 ? 2 : 1;  // sums of an output, so that products need not wait for one another
     constexpr bool EARLY = R == 1 || D < 256;  // registers for a group's values beside its keys
     constexpr uint32_t NONE = ~0u;
@@ -359,13 +258,13 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
     static_assert(sizeof(Args) > 128);
-    // groups of four tiles where there are few, so that they reach more CUs; of eight where a workgroup has several, so that
-    // its waves' turns are whole
+    // groups of four tiles where there are few, so that they reach more CUs; of eight where a workgroup has several: the parts are
+    // then whole turns of eight waves too
     const Totals totals = plan<D, R, W>(a, sh);
     const bool wide = totals.narrow > (int)gridDim.x;
     const int groups_in_all = wide ? totals.wide : totals.narrow;
     const int workgroups = __builtin_amdgcn_readfirstlane(used_workgroups(gridDim.x, groups_in_all, a.t.n_seq, totals.units));
-    if (blockIdx.x == 0 && !a.fuse) {
+    if (blockIdx.x == 0) {
         if (threadIdx.x == 0) a.plan[0] = groups_in_all, a.plan[1] = workgroups, a.plan[2] = wide;
         for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) a.plan[PLAN_HEAD + i] = sh.base[wide][i];
     }
@@ -376,7 +275,6 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     // (what all lanes have alike is said to be so where it comes through LDS or a division: addresses are then scalar)
     const int lo = __builtin_amdgcn_readfirstlane(first_group(workgroup, groups_in_all, workgroups));
     const int hi = __builtin_amdgcn_readfirstlane(first_group(workgroup + 1, groups_in_all, workgroups));
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int)PF_SK_PART_BYTES, BUF_RSRC_WORD3);
     for (int at = lo; at < hi;) {
         // (said anew in each turn, so that nothing that follows is kept in registers across them: most workgroups take one. The
         // arguments are read again where they are used.)
@@ -427,7 +325,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
         };
         load_query(q_row);
 
-        u4 kc[4][C], vc[VT][SL];
+        u4 kc[4][C], vc[W][SL];
         float sk, sv;
         const uint32_t in_tile = col * 64 + g * 16;
         // 1 KiB pieces of a tile, as buffer loads: of a tile that is not there they read nothing
@@ -436,11 +334,11 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                                                      BUF_RSRC_WORD3);
         };
         auto piece = [&](__amdgpu_buffer_rsrc_t tile, int at) {
-            return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, R == 1 ? 2 : 0));
+            return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, R == 1 ? CPOL_NT : 0));
         };
         // the wave's tile's keys and scales (lane l: token l's); a page that the cache has not gives NaN
-        auto load_keys = [&](int t8) {
-            const int t = t8 + wave;
+        auto load_keys = [&](int turn) {
+            const int t = turn + wave;
             const uint32_t at = __builtin_amdgcn_readlane(places, (t - g0 * group_tiles) & 63);
             const bool none = at == NONE;
             const uint32_t place = none ? 0 : at;
@@ -453,11 +351,11 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             sk = none ? NAN : sc[lane];
             sv = t * KV_TILE + lane < total ? sc[page_tiles * KV_TILE + lane] : 0.0f;
         };
-        const int slice = (wave % (WAVES / SPLIT)) * SL, v_tile = wave / (WAVES / SPLIT) * VT;
-        auto load_values = [&](int t8) {
+        const int slice = wave * SL;
+        auto load_values = [&](int turn) {
 #pragma unroll
-            for (int v = 0; v < VT; v++) {
-                const int t = t8 + v_tile + v;
+            for (int v = 0; v < W; v++) {
+                const int t = turn + v;
                 const uint32_t at = __builtin_amdgcn_readlane(places, (t - g0 * group_tiles) & 63);
                 const auto tile = tile_at((at == NONE ? 0 : at) + page_tiles, slice * 1024, t < t_end);
 #pragma unroll
@@ -517,13 +415,13 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
         }
 
         const int whole_lane = lane;
-        for (int t8 = g0 * group_tiles; t8 < t_end; t8 += WAVES) {
+        for (int turn = g0 * group_tiles; turn < t_end; turn += W) {
             // (said anew here and behind the loop: what follows from it would be kept in registers otherwise, and they run out)
             int said = whole_lane;
             asm volatile("" : "+v"(said));
             const int lane = said, col = lane & 15, g = lane >> 4;
-            const int t0 = (t8 + wave) * KV_TILE;
-            const bool more = t8 + WAVES < t_end, own = t8 + wave < t_end;
+            const int t0 = (turn + wave) * KV_TILE;
+            const bool more = turn + W < t_end, own = turn + wave < t_end;
             // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
             f4 x[R][4];
 #pragma unroll
@@ -549,7 +447,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 }
                 HOLD();
             }
-            if (!EARLY) load_values(t8);
+            if (!EARLY) load_values(turn);
 
             // the scores' and the values' scales, as the lanes need them
             float(&ts)[2][KV_TILE] = sh.tile_scale[wave];
@@ -613,7 +511,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                     top[rt] = next;
                     by *= al;
                 }
-                if (t8 != g0 * group_tiles && __any(by != 1.0f)) {
+                if (turn != g0 * group_tiles && __any(by != 1.0f)) {
 #pragma unroll
                     for (int i = 0; i < SL; i++)
 #pragma unroll
@@ -649,15 +547,15 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 HOLD();
             }
             if (more) {
-                if (((t8 + WAVES - g0 * group_tiles) & 63) == 0) load_places(t8 + WAVES);
-                load_keys(t8 + WAVES);
+                if (((turn + W - g0 * group_tiles) & 63) == 0) load_places(turn + W);
+                load_keys(turn + W);
             }
             lds_barrier();
 
             // o^T += v^T p^T: the k index of both operands runs over tokens 16 w + 4 g + j, as the scores lie
 #pragma unroll
-            for (int v = 0; v < VT; v++) {
-                const int t = t8 + v_tile + v;
+            for (int v = 0; v < W; v++) {
+                const int t = turn + v;
                 if (t < t_end) {
                     if ((t + 1) * KV_TILE > total) {  // codes that no token of this sequence wrote may be anything
                         u4 keep;
@@ -676,7 +574,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                         for (int i = 0; i < SL; i++) codes[i] = operands<FMT>(vc[v][i][2 * k], vc[v][i][2 * k + 1]);
 #pragma unroll
                         for (int rt = 0; rt < R; rt++) {
-                            const h8 p = sh.p[v_tile + v][rt][k][lane];
+                            const h8 p = sh.p[v][rt][k][lane];
 #pragma unroll
                             for (int i = 0; i < SL; i++)
                                 o[rt][i][k % CHAINS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[i], p, o[rt][i][k % CHAINS], 0, 0, 0);
@@ -684,7 +582,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                     }
                 }
             }
-            if (EARLY && more) load_values(t8 + WAVES);
+            if (EARLY && more) load_values(turn + W);
         }
 
         // the waves' sums joined, and the outputs written, or a partial result
@@ -711,27 +609,17 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             for (int rt = 0; rt < R; rt++) {
                 f4 s = sh.sums[rt * 16 + col][0];
 #pragma unroll
-                for (int k = 1; k < WAVES / 2; k++) s += sh.sums[rt * 16 + col][k];
+                for (int k = 1; k < W / 2; k++) s += sh.sums[rt * 16 + col][k];
                 sum[rt] = s.x + s.z;
                 const float back = -128.0f * (s.y + s.w);
 #pragma unroll
                 for (int i = 0; i < SL; i++) {
                     f4 v = o[rt][i][0];
                     if (CHAINS > 1) v += o[rt][i][CHAINS - 1];
-                    if (FMT == QH_KV_I8) v = v * 0x1p24f + back / SPLIT;
+                    if (FMT == QH_KV_I8) v = v * 0x1p24f + back;
                     o[rt][i][0] = v * ref;
                 }
             }
-            if (SPLIT > 1) {  // two waves have the same dimensions, of different tiles
-                if (wave >= WAVES / SPLIT)
-#pragma unroll
-                    for (int rt = 0; rt < R; rt++) sh.half[rt][wave - WAVES / 2][lane] = o[rt][0][0];
-                lds_barrier();
-                if (wave < WAVES / SPLIT)
-#pragma unroll
-                    for (int rt = 0; rt < R; rt++) o[rt][0][0] += sh.half[rt][wave][lane];
-            }
-            if (SPLIT == 1 || wave < WAVES / SPLIT)
 #pragma unroll
                 for (int rt = 0; rt < R; rt++) {
                     const int r = rt * 16 + col;
@@ -741,36 +629,14 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                         for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt],
                                 AHEAD ? gate[rt][i] : load_gate(a, row_at(r) + (slice + i) * 16 + g * 4));
                     } else {
+                        const uint32_t row = slot * ROWS + r;
 #pragma unroll
-                        for (int i = 0; i < SL; i++)
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, o[rt][i][0]), rsrc,
-                                                                   (uint32_t)((slot * ROWS + r) * D + (slice + i) * 16 + g * 4) * 4, 0, CPOL_SC1);
+                        for (int i = 0; i < SL; i++) *(f4*)(a.part + row * D + (slice + i) * 16 + g * 4) = o[rt][i][0];
                         if (wave == 0 && g == 0)
-                            __builtin_amdgcn_raw_buffer_store_b64(
-                                __builtin_bit_cast(u2, (f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * sh.factor[r], sum[rt]})), rsrc,
-                                a.ml_at + (uint32_t)(slot * ROWS + r) * 8, 0, CPOL_SC1);
+                            ((f2*)((uint8_t*)a.part + a.ml_at))[row] =
+                                f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * sh.factor[r], sum[rt]};
                     }
                 }
-        }
-        if constexpr (R == 1) {
-            if (!direct && a.fuse) {
-                const int u0 = at - g0, w0 = group_owner(u0, all, used), parts = group_owner(u0 + groups - 1, all, used) - w0 + 1;
-                const Cluster k = cluster(w - w0, parts);
-                const int kw = w0 + k.first, k_slot = partial_slot(kw, u0, all, used);
-                // the cluster's parts, then the clusters' sums; the last of either to arrive goes on
-                int from = kw, first_slot = k_slot, step = 1, count = k.size;
-                uint32_t* counter = a.count + k_slot;
-                for (bool out = k.of == 1;;) {
-                    if (count > 1) {
-                        if (!last_of(counter, count, &sh.last)) break;
-                        join_parts<D, W>(a, sh, rsrc, first_slot, from, step, count, live, out, row_at);
-                    }
-                    if (out) break;
-                    from = w0, first_slot = partial_slot(w0, u0, all, used), step = k.step, count = k.of;
-                    counter = a.count + 2 * gridDim.x + w0;
-                    out = true;
-                }
-            }
         }
         at += g1 - g0;
         if (at < hi) lds_barrier();
@@ -862,8 +728,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 
 template <int D, int FMT>
 void launch(hipStream_t stream, const Args& a, int waves, int grid, bool join) {
-    auto* f = a.row_tiles == 0 ? (waves == 8 ? tree_attn_kernel<D, FMT, 1, 8> : tree_attn_kernel<D, FMT, 1, 4>)
-                               : waves == 8 ? tree_attn_kernel<D, FMT, 2, 8> : tree_attn_kernel<D, FMT, 2, 4>;
+    auto* f = a.row_tiles == 0 ? tree_attn_kernel<D, FMT, 1, 4> : tree_attn_kernel<D, FMT, 2, 4>;
+    if constexpr (D == 256)
+        if (waves == 8) f = tree_attn_kernel<D, FMT, 2, 8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(64 * waves), 0, stream, a);
     if (!join) return;
     const unsigned rows = (unsigned)(a.t.n * a.kv.heads * a.t.group);
@@ -900,17 +767,17 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     const int64_t groups = (cap + KV_TILE * GROUP_TILES - 1) / (KV_TILE * GROUP_TILES);  // of the longest sequence there can be
     const int64_t cus = ctx ? ctx_cus(ctx) : 1;
     auto units_of = [&](int rt) { return (int64_t)kv->heads * ((step->max_new * group + (16 << rt) - 1) >> (4 + rt)); };
-    // A chunk's rows: all of them, up to 32, while that leaves work for every CU.
-    int rt = 0;
-    while (rt < 1 && step->max_new * group > 16 << rt && units_of(rt + 1) * step->n_seq * groups >= cus) rt++;
+    // Chunks of 32 rows, where there are more than 16, read the cache half as often, but leave half as many shares: from about a
+    // share for each CU (24 x 256, 5 tokens at 16,000: 20.5 us against 24.4, at 4,000: 15.6 against 13.9; 32 x 128, 5 tokens at
+    // 16,000: 17.4 against 18.8, at 4,000: 13.0 against 11.7).
+    const int rt = step->max_new * group > 16 && units_of(1) * step->n_seq * groups >= (kv->head_dim == 256 ? cus * 3 / 4 : cus) ? 1 : 0;
     const int rows = 16 << rt;
-    // Workgroups of eight waves, or twice as many of four: those start sooner (4,099 positions of 32 x 128: 10.1 us against 11.5,
-    // of 24 x 256 13.5 against 13.8) and are out of step with one another, so that one's products run beside another's softmax
-    // (8 sequences of 8 tokens, 32 x 128: 20.6 against 27.9; 64 tokens at 8,150, 24 x 256: 43.0 against 46.0), but they leave
-    // twice the partial results (131,000 positions 61.7 against 59.6, 5 tokens at 32,700 27.8 against 24.1).
+    // Workgroups of four waves start soon, and are out of step with one another, so that one's products run beside another's
+    // softmax (24 x 256: 32 sequences of 5 tokens 33.5 us against 41.9 of eight waves, 64 tokens at 16,000 61.6 against 65.5). One
+    // long chunk alone has eight waves and half as many partial results (5 tokens at 32,700: 24.3 against 25.5, at 131,000: 59.9
+    // against 64.6; of 128 dimensions 70.0 against 62.0).
     const int64_t total = units_of(rt) * step->n_seq * groups;
-    const bool four = rt == 0 ? total <= cus : kv->head_dim < 256 || (step->max_new * group > 128 && total >= 4 * cus);
-    const int waves = four ? 4 : 8;
+    const int waves = rt && kv->head_dim == 256 && step->n_seq == 1 && step->max_new * group <= 32 && total >= 2 * cus ? 8 : 4;
     const int64_t units = units_of(rt);
     if (units * step->n_seq > 0x7fffffff / groups)
         return fail(QH_EINVAL, "tree_attn: %d sequences of up to %lld positions are too many for one call", step->n_seq, (long long)cap);
@@ -922,17 +789,14 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     a.mask = step->mask;
     a.group_inv = ((1u << 20) + group - 1) / group;
     a.scale = scale * 1.4426950408889634f;
-    const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt, waves), units * step->n_seq * groups, (int64_t)MAX_CLUSTER * MAX_CLUSTER});
-    static_assert(3 * MAX_CLUSTER * MAX_CLUSTER <= PF_SK_ITEMS_MAX);
+    const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt, waves), units * step->n_seq * groups, (int64_t)TREE_MAX_WGS});
     const size_t part = (size_t)2 * grid * rows * kv->head_dim * 4, ml = (size_t)2 * grid * rows * 8;
     if (part + ml + (TREE_MAX_SEQS + PLAN_HEAD) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
     a.row_tiles = rt;
     a.part = (float*)ctx_partials(ctx);
     a.ml_at = (int32_t)part;
     a.plan = (int32_t*)((uint8_t*)ctx_partials(ctx) + part + ml);
-    a.count = (uint32_t*)((uint8_t*)ctx_partials(ctx) + PF_SK_PART_BYTES);
-    a.fuse = rt == 0;
-    const bool join = !a.fuse && groups > 1 && grid > 1;
+    const bool join = groups > 1 && grid > 1;
     auto go = [&](auto d) {
         if (kv->fmt == QH_KV_I8) launch<decltype(d)::value, QH_KV_I8>((hipStream_t)stream, a, waves, grid, join);
         else launch<decltype(d)::value, QH_KV_E4M3>((hipStream_t)stream, a, waves, grid, join);

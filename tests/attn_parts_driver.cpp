@@ -1,6 +1,6 @@
-// How a step's partial results are shared and joined (csrc/attn_plan.h), on the CPU under sanitizers: clusters partition a
-// unit's parts and fit the joining side's arrays, shares cover all groups in order and find their owners up to the largest
-// numbers, one sequence's units get whole workgroups, and groups of twice the tiles cover the same positions.
+// How a step's work is shared (csrc/attn_plan.h), on the CPU under sanitizers: shares cover all groups in order and find their
+// owners up to the largest numbers, one sequence's units get whole workgroups, and groups of twice the tiles cover the same
+// positions.
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -19,23 +19,11 @@ using namespace qh;
     } while (0)
 
 int main() {
-    for (int parts = 1; parts <= MAX_CLUSTER * MAX_CLUSTER; parts++) {
-        int next = 0, clusters = 0;
-        for (int i = 0; i < parts; i++) {
-            const Cluster k = cluster(i, parts);
-            CHECK(k.first <= i && i < k.first + k.size && k.size >= 1 && k.size <= MAX_CLUSTER && k.of <= MAX_CLUSTER);
-            CHECK(k.first % k.step == 0 && k.first / k.step < k.of);
-            if (i == next) next += k.size, clusters++;
-            CHECK(i < next);
-            CHECK((k.of == 1) == (k.size == parts));
-        }
-        CHECK(next == parts && clusters == cluster(0, parts).of);
-    }
     std::mt19937_64 rng(11);
     auto in = [&](int64_t lo, int64_t hi) { return (int)std::uniform_int_distribution<int64_t>(lo, hi)(rng); };
     for (int trial = 0; trial < 20000; trial++) {
         const int all = trial % 3 ? in(1, 5000) : in(1, 2147483647 - 1);
-        const int used = in(1, all < 1024 ? all : 1024);
+        const int used = in(1, all < TREE_MAX_WGS ? all : TREE_MAX_WGS);
         CHECK(first_group(0, all, used) == 0 && first_group(used, all, used) == all);
         for (int k = 0; k < 20; k++) {
             const int w = in(0, used - 1), lo = first_group(w, all, used), hi = first_group(w + 1, all, used);

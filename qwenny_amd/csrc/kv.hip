@@ -18,6 +18,11 @@ using namespace qh;
 namespace {
 
 constexpr int WAVES = 4;
+
+// buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of loads past the caches
+constexpr int BUF_RSRC_WORD3 = 0x00020000;
+constexpr int CPOL_NT = 2;
+
 constexpr int BATCH = 64, BATCH_WAVES = 16;  // tokens of a workgroup that turns values over in LDS, and its waves
 
 // f over the wave's 64 lanes, or over 16 neighbouring ones: within rows of 16 by DPP, then over the rows
@@ -138,12 +143,12 @@ struct Vec<1> {
     typedef __bf16 b __attribute__((ext_vector_type(1)));
 };
 
-// One head of one token's partials, summed in their order: V values a lane, up to eight partials in flight.
+// Partials s0 .. of one head of one token added to `sum` in their order: V values a lane, up to eight partials in flight.
 template <int V>
-__device__ __forceinline__ void head_sum(const float* __restrict__ x, int splits, int64_t stride, int lane, float (&y)[V]) {
+__device__ __forceinline__ void add_partials(const float* __restrict__ x, int s0, int splits, int64_t stride, int lane,
+                                             typename Vec<V>::f& sum) {
     typedef typename Vec<V>::f vec;
-    vec sum = __builtin_nontemporal_load((const vec*)(x + lane * V));
-    for (int s0 = 1; s0 < splits; s0 += 8) {
+    for (; s0 < splits; s0 += 8) {
         vec p[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -152,9 +157,41 @@ __device__ __forceinline__ void head_sum(const float* __restrict__ x, int splits
         for (int j = 0; j < 8; j++)
             if (s0 + j < splits) sum += p[j];
     }
+}
+template <int V>
+__device__ __forceinline__ void head_sum(const float* __restrict__ x, int splits, int64_t stride, int lane, float (&y)[V]) {
+    typename Vec<V>::f sum = __builtin_nontemporal_load((const typename Vec<V>::f*)(x + lane * V));
+    add_partials<V>(x, 1, splits, stride, lane, sum);
 #pragma unroll
     for (int i = 0; i < V; i++) y[i] = sum[i];
 }
+
+// The same in two halves, so that the first P partials are in flight over other work: buffer loads, which read nothing where
+// there is none (a branch around a load would have its wait cover all loads).
+template <int V, int P>
+struct Ahead {
+    typename Vec<V>::f p[P];
+    const float* x;
+    __device__ __forceinline__ void read(const float* from, int splits, int64_t stride, int lane) {
+        x = from;
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(from + j * stride), 0, j < splits ? 64 * V * 4 : 0, BUF_RSRC_WORD3);
+            if constexpr (V == 1) p[j][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, lane * 4, 0, CPOL_NT));
+            else if constexpr (V == 2) p[j] = __builtin_bit_cast(typename Vec<V>::f, __builtin_amdgcn_raw_buffer_load_b64(rsrc, lane * 8, 0, CPOL_NT));
+            else p[j] = __builtin_bit_cast(typename Vec<V>::f, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, 0, CPOL_NT));
+        }
+    }
+    __device__ __forceinline__ void sum(int splits, int64_t stride, int lane, float (&y)[V]) {
+        auto v = p[0];
+#pragma unroll
+        for (int j = 1; j < P; j++)
+            if (j < splits) v += p[j];
+        add_partials<V>(x, P, splits, stride, lane, v);
+#pragma unroll
+        for (int i = 0; i < V; i++) y[i] = v[i];
+    }
+};
 
 // a wave for each (token, kv head, keys or values)
 template <int D, int FMT>
@@ -441,54 +478,63 @@ __device__ __forceinline__ void put(__bf16* to, const float (&y)[V], int lane) {
 }
 
 // A workgroup takes some heads (blockIdx.y's share) of one token, a wave a head at a time: queries (with their gates),
-// keys, values. The angles' sines and cosines are made once per workgroup: pos * inv_freq in turns in f64, whose fraction
-// is exact to f32 at any position.
-template <int D, int FMT>
+// keys, values. The angles' sines and cosines are made once per workgroup, while the first heads' partials are on their way:
+// pos * inv_freq in turns in f64, whose fraction is exact to f32 at any position. P: partials of a head in
+// flight at once (summed as they come instead: a token of 16 x 256, 8 partials 4.4 us against 3.4, 5 of 24 x 256, 4 partials
+// into the cache 5.6 against 4.2, 2048 of them 33.9 against 29.9).
+template <int D, int FMT, int P>
 __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
     constexpr int V = D / 64;
-    __shared__ float cs[D / 2], sn[D / 2];
-    __shared__ float rows[WAVES][D];
-    // all lines of the arguments are fetched at once, and what does not depend on the sums is read beside them: each would be
+    typedef typename Vec<V>::f vec;
+    __shared__ __align__(16) float angle[2][D];  // what a dimension and its partner are multiplied by
+    __shared__ __align__(16) float rows[WAVES][D];
+    // all lines of the arguments are fetched at once, and what does not depend on the sums is read ahead of them: each would be
     // a trip to memory of its own when first touched (2048 tokens of 24 x 256: 33.9 us against 36.8)
     const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
     static_assert(sizeof(Prep) > 128);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = a.rot / 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = a.rot / 2;
     const int64_t t = blockIdx.x;
     const int per = a.gated ? 2 : 1, heads = a.heads;
     const int64_t ld = (int64_t)(a.q_heads * per + 2 * a.kv_heads) * D, stride = a.n * ld;
     const int share = (heads + gridDim.y - 1) / gridDim.y, h1 = min(heads, (int)(blockIdx.y + 1) * share);
-    // a head's sums, with a query's those of its gate, are read while the head before is worked on
-    float next[V], next_gate[V];
+    const int slot = FMT ? a.slots[t] : 0, pos = half ? a.pos[t] : 0;
+    const int i_freq = (int)threadIdx.x < half ? threadIdx.x : threadIdx.x - half;
+    float freq = 0.0f;
+    if ((int)threadIdx.x < a.rot) freq = a.inv_freq[i_freq];
+    vec norm[2] = {};
+    if (a.q_w) norm[0] = ((const vec*)a.q_w)[lane];
+    if (a.k_w) norm[1] = ((const vec*)a.k_w)[lane];
+    // a head's partials, with a query's those of its gate, are read while the head before is worked on
+    Ahead<V, P> next, next_gate;
     auto read = [&](int h) {
         const bool is_q = h < a.q_heads;
         const float* const x = a.x + t * ld + (int64_t)(is_q ? h * per : h - a.q_heads + a.q_heads * per) * D;
-        head_sum<V>(x, a.splits, stride, lane, next);
-        if (is_q && a.gated) head_sum<V>(x + D, a.splits, stride, lane, next_gate);
+        const int splits = P == 1 && h >= h1 ? 0 : a.splits;  // (of one partial each, without a branch: 29.9 us against 34.3)
+        next.read(x, splits, stride, lane);
+        next_gate.read(x + D, is_q && a.gated ? splits : 0, stride, lane);
     };
     const int h0 = blockIdx.y * share + wave;
-    if (h0 < h1) read(h0);
-    typename Vec<V>::f norm[2] = {};
-    if (a.q_w) norm[0] = ((const typename Vec<V>::f*)a.q_w)[lane];
-    if (a.k_w) norm[1] = ((const typename Vec<V>::f*)a.k_w)[lane];
-    const int slot = FMT ? a.slots[t] : 0, pos = half ? a.pos[t] : 0;
-    asm volatile("" ::"s"(slot), "s"(pos));
-    if ((int)threadIdx.x < half) {
-        const double turns = (double)pos * (double)a.inv_freq[threadIdx.x] * 0.15915494309189535;
+    if (P == 1 || h0 < h1) read(h0);
+    if ((int)threadIdx.x < a.rot) {
+        const double turns = (double)pos * (double)freq * 0.15915494309189535;
         const float part = (float)(turns - rint(turns));
-        sincospif(2.0f * part, &sn[threadIdx.x], &cs[threadIdx.x]);
+        float sn, cs;
+        sincospif(2.0f * part, &sn, &cs);
+        angle[0][threadIdx.x] = cs, angle[1][threadIdx.x] = (int)threadIdx.x < half ? -sn : sn;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");  // (the reads stay in flight over the barrier)
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    const vec own = *(const vec*)&angle[0][lane * V], other = *(const vec*)&angle[1][lane * V];
     for (int h = h0; h < h1; h += WAVES) {
         const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
         float y[V], gate[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) y[i] = next[i], gate[i] = next_gate[i];
-        if (h + WAVES < h1) read(h + WAVES);
+        next.sum(a.splits, stride, lane, y);
+        if (is_q && a.gated) next_gate.sum(a.splits, stride, lane, gate);
+        if (P == 1 || h + WAVES < h1) read(h + WAVES);
         if (is_q ? a.q_w != nullptr : is_k && a.k_w) {
-            const auto w = is_q ? norm[0] : norm[1];
+            const vec w = is_q ? norm[0] : norm[1];
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; i++) ss += y[i] * y[i];
@@ -498,14 +544,21 @@ __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
             for (int i = 0; i < V; i++) y[i] = w[i] * (y[i] * r);
         }
         if (half && (is_q || is_k)) {
+            vec u;
 #pragma unroll
-            for (int i = 0; i < V; i++) rows[wave][lane * V + i] = y[i];
+            for (int i = 0; i < V; i++) u[i] = y[i];
+            *(vec*)&rows[wave][lane * V] = u;
             __builtin_amdgcn_wave_barrier();
+            float partner[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int d = lane * V + i;
-                if (d < half) y[i] = y[i] * cs[d] - rows[wave][d + half] * sn[d];
-                else if (d < a.rot) y[i] = y[i] * cs[d - half] + rows[wave][d - half] * sn[d - half];
+                partner[i] = rows[wave][d < half ? d + half : d < a.rot ? d - half : d];
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float turned = y[i] * own[i] + partner[i] * other[i];
+                y[i] = lane * V + i < a.rot ? turned : y[i];
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -642,7 +695,11 @@ extern "C" int qh_attn_prep(void* stream, const float* x, int splits, size_t n, 
     const unsigned shares = n >= 512 ? 1 : (heads + WAVES - 1) / WAVES;
     by_dim(D, [&](auto d) {
         constexpr int DD = decltype(d)::value;
-        auto* f = !kv ? attn_prep_kernel<DD, 0> : kv->fmt == QH_KV_I8 ? attn_prep_kernel<DD, QH_KV_I8> : attn_prep_kernel<DD, QH_KV_E4M3>;
+        auto kernel = [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            return !kv ? attn_prep_kernel<DD, 0, P> : kv->fmt == QH_KV_I8 ? attn_prep_kernel<DD, QH_KV_I8, P> : attn_prep_kernel<DD, QH_KV_E4M3, P>;
+        };
+        auto* f = splits == 1 ? kernel(std::integral_constant<int, 1>{}) : splits <= 4 ? kernel(std::integral_constant<int, 4>{}) : kernel(std::integral_constant<int, 8>{});
         hipLaunchKernelGGL(f, dim3((unsigned)n, shares), dim3(64 * WAVES), 0, (hipStream_t)stream, a);
         if (!batch) return;
         const int64_t ld = (int64_t)(rows->q_heads * (a.gated ? 2 : 1) + 2 * rows->kv_heads) * D;

@@ -25,6 +25,13 @@ constexpr int CPOL_NT = 2;
 
 constexpr int BATCH = 64, BATCH_WAVES = 16;  // tokens of a workgroup that turns values over in LDS, and its waves
 
+// A barrier for what the workgroup's waves wrote to LDS; loads and stores to memory stay in flight over it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // f over the wave's 64 lanes, or over 16 neighbouring ones: within rows of 16 by DPP, then over the rows
 template <int LANES = 64, class F>
 __device__ __forceinline__ uint32_t over_lanes(uint32_t v, F&& f) {
@@ -349,8 +356,11 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv,
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, const int32_t* __restrict__ slots, int n,
                                                                          __bf16* __restrict__ k, __bf16* __restrict__ v) {
-    constexpr int V = D / 64, EACH = BATCH / BATCH_WAVES, ROW = 17;  // words of a dimension's 64 bytes, and one
-    __shared__ uint32_t tile_codes[D * ROW];
+    constexpr int V = D / 64, EACH = BATCH / BATCH_WAVES;
+    static_assert(D * 4 <= 64 * BATCH_WAVES);
+    // where a dimension's 64 bytes lie in LDS, in words: the 64 lanes, V dimensions apart, reach different banks
+    auto row = [](int d) { return d * 17 + (d >> 6); };
+    __shared__ uint32_t tile_codes[D * 17 + V];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t0 = blockIdx.x * BATCH, which = blockIdx.y & 1, head = blockIdx.y >> 1;
     const uint32_t in_page = (1u << kv.page_shift) - 1;
     const int mine = t0 + lane < n ? slots[t0 + lane] : -1;
@@ -389,29 +399,38 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, 
             if (there >> (wave * EACH + i) & 1) put(wave * EACH + i, c[i]);
         return;
     }
-    for (uint64_t left = there; left;) {
+    // one tile after the other; the next one's values are on their way while the first's are taken out
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    uint64_t left = there, here = 0;
+    u4 next = {};
+    const int at = min((int)threadIdx.x, D * 4 - 1);
+    auto load = [&] {
         const int tile = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)left) - 1) >> 6, slot0 = tile << 6;
-        const uint64_t here = __ballot(in_cache && mine >> 6 == tile);
+        here = __ballot(in_cache && mine >> 6 == tile);
         left &= ~here;
-        const uint8_t* const block = kv.codes + kv_block<D>(kv, slot0 >> kv.page_shift, head, 1) + (size_t)(slot0 & in_page) * D;
-        for (int i = threadIdx.x; i < D * 4; i += 64 * BATCH_WAVES) {
-            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-            const u4 w = *(const u4*)(block + i * 16);
-            uint32_t* const to = tile_codes + (i >> 2) * ROW + (i & 3) * 4;
-            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+        next = *(const u4*)(kv.codes + kv_block<D>(kv, slot0 >> kv.page_shift, head, 1) + (size_t)(slot0 & in_page) * D + at * 16);
+    };
+    if (left) load();
+    while (here) {
+        if ((int)threadIdx.x < D * 4) {
+            uint32_t* const to = tile_codes + row(at >> 2) + (at & 3) * 4;
+            to[0] = next.x, to[1] = next.y, to[2] = next.z, to[3] = next.w;
         }
-        __syncthreads();
+        const uint64_t now = here;
+        here = 0;
+        if (left) load();
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int e = wave * EACH + i;
-            if (!(here >> e & 1)) continue;
+            if (!(now >> e & 1)) continue;
             const uint32_t t = __builtin_amdgcn_readlane(mine, e) & 63, byte = v_byte<D>(t, 0);
             uint8_t c[V];
 #pragma unroll
-            for (int j = 0; j < V; j++) c[j] = ((const uint8_t*)(tile_codes + (lane * V + j) * ROW))[byte];
+            for (int j = 0; j < V; j++) c[j] = ((const uint8_t*)(tile_codes + row(lane * V + j)))[byte];
             put(e, c);
         }
-        if (left) __syncthreads();
+        if (here) lds_barrier();
     }
 }
 
@@ -523,9 +542,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
         sincospif(2.0f * part, &sn, &cs);
         angle[0][threadIdx.x] = cs, angle[1][threadIdx.x] = (int)threadIdx.x < half ? -sn : sn;
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");  // (the reads stay in flight over the barrier)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    lds_barrier();
     const vec own = *(const vec*)&angle[0][lane * V], other = *(const vec*)&angle[1][lane * V];
     for (int h = h0; h < h1; h += WAVES) {
         const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;

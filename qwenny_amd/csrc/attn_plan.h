@@ -62,6 +62,12 @@ constexpr int group_owner(int at, int all, int used) {
     return w;
 }
 
+// The same in few steps, from 1 / all in 64 bits: ((at + 1) used - 1) / all, the half keeping it off whole numbers (-1 for
+// group -1)
+constexpr int owner(int at, int used, double inv_all) {
+    return at < 0 ? -1 : (int)(((double)at * used + (used - 0.5)) * inv_all);
+}
+
 // The workgroups that take part of `grid`. One sequence's units are all alike: each gets as many workgroups as any, so that no
 // workgroup has parts of two.
 constexpr int used_workgroups(int grid, int all, int n_seq, int units) {

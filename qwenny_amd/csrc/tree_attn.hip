@@ -28,7 +28,7 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int PLAN_HEAD = 4;
+constexpr int PLAN_HEAD = 6;  // of the plan in memory: groups, workgroups, whether the groups are wide, -, 1 / groups in 64 bits
 
 // buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of loads past the caches
 constexpr int BUF_RSRC_WORD3 = 0x00020000;
@@ -50,7 +50,7 @@ struct Args {
     int32_t row_tiles;     // log2 of a chunk's tiles of 16 rows
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
-    int32_t* plan;         // for join_kernel: groups, workgroups, whether the groups are wide; each sequence's first group
+    int32_t* plan;         // for join_kernel: PLAN_HEAD, each sequence's first group
 };
 
 // The compiler moves nothing across: left free it converts a whole tile's codes ahead of its products and spills.
@@ -265,7 +265,10 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     const int groups_in_all = wide ? totals.wide : totals.narrow;
     const int workgroups = __builtin_amdgcn_readfirstlane(used_workgroups(gridDim.x, groups_in_all, a.t.n_seq, totals.units));
     if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) a.plan[0] = groups_in_all, a.plan[1] = workgroups, a.plan[2] = wide;
+        if (threadIdx.x == 0) {
+            a.plan[0] = groups_in_all, a.plan[1] = workgroups, a.plan[2] = wide;
+            *(double*)(a.plan + 4) = 1.0 / groups_in_all;
+        }
         for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) a.plan[PLAN_HEAD + i] = sh.base[wide][i];
     }
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
@@ -651,12 +654,16 @@ template <int D, int W>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     constexpr int V = W / 4, SETS = 256 / V, DEEP = 4;
     __shared__ f4 sums[SETS][V];
-    const int heads = a.kv.heads * a.t.group, rows = 16 << a.row_tiles;
-    const int token = blockIdx.x / heads, h = blockIdx.x - token * heads, head = h / a.t.group;
-    const int lane = threadIdx.x & 63, set = threadIdx.x / V, d = blockIdx.y * W + threadIdx.x % V * 4;
-    const size_t at = (size_t)blockIdx.x * D + d;
+    // all lines of the arguments are fetched at once, as above
+    const auto* const line = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" ::"s"(line[0]), "s"(line[16]), "s"(line[32]));
+    const int rows = 16 << a.row_tiles, token = blockIdx.x, head = blockIdx.y;
+    const int piece = (int)(blockIdx.z * a.group_inv >> 20), in_group = blockIdx.z - piece * a.t.group;
+    const int lane = threadIdx.x & 63, set = threadIdx.x / V, d = piece * W + threadIdx.x % V * 4;
+    const size_t at = (((size_t)token * a.kv.heads + head) * a.t.group + in_group) * D + d;
     const b4 gate = load_gate(a, at);
-    const int all = a.plan[0], used = a.plan[1];
+    const int used = a.plan[1];
+    const double inv_all = *(const double*)(a.plan + 4);
     const bool wide = a.plan[2] != 0;
     // the last sequence with start <= token; up to 64 sequences all their numbers are read at once
     Seq s;
@@ -676,11 +683,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     }
     const int node = token - s.first;
     if (node < 0 || node >= s.news) return;
-    const int r = node * a.t.group + h - head * a.t.group;
+    const int r = node * a.t.group + in_group;
     const int u0 = base + (head * s.chunks + (r >> (4 + a.row_tiles))) * s.groups, u1 = u0 + s.groups;
-    const int w0 = group_owner(u0, all, used), parts = group_owner(u1 - 1, all, used) - w0 + 1;
+    const int w0 = owner(u0, used, inv_all), parts = owner(u1 - 1, used, inv_all) - w0 + 1;
     if (parts == 1) return;  // one workgroup wrote the row
-    const int first_slot = partial_slot(w0, u0, all, used), in = r & (rows - 1);
+    const int first_slot = 2 * w0 + (owner(u0 - 1, used, inv_all) == w0 ? 1 : 0), in = r & (rows - 1);  // partial_slot
     auto slot = [&](int i) { return (size_t)(i == 0 ? first_slot : 2 * (w0 + i)) * rows + in; };
     const f2* const ml = (const f2*)((const uint8_t*)a.part + a.ml_at);
     f4 y[DEEP], v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -733,9 +740,9 @@ void launch(hipStream_t stream, const Args& a, int waves, int grid, bool join) {
         if (waves == 8) f = tree_attn_kernel<D, FMT, 2, 8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(64 * waves), 0, stream, a);
     if (!join) return;
-    const unsigned rows = (unsigned)(a.t.n * a.kv.heads * a.t.group);
-    if (rows <= 512) hipLaunchKernelGGL((join_kernel<D, 64>), dim3(rows, D / 64), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((join_kernel<D, D>), dim3(rows), dim3(256), 0, stream, a);
+    const unsigned n = (unsigned)a.t.n, heads = (unsigned)a.kv.heads, group = (unsigned)a.t.group;
+    if (n * heads * group <= 512) hipLaunchKernelGGL((join_kernel<D, 64>), dim3(n, heads, group * (D / 64)), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((join_kernel<D, D>), dim3(n, heads, group), dim3(256), 0, stream, a);
 }
 
 }  // namespace

@@ -200,7 +200,8 @@ struct Ahead {
     }
 };
 
-// a wave for each (token, kv head, keys or values)
+// A wave for each (token, kv head, keys or values), for few tokens: bound by its trips to memory, the slot's and the vector's, then
+// out (9 tokens of 8 x 128: 2.4 us).
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * WAVES) void kv_write_kernel(Kv kv, const __bf16* __restrict__ k, const __bf16* __restrict__ v,
                                                               const int32_t* __restrict__ slots, int64_t vectors) {
@@ -217,6 +218,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_write_kernel(Kv kv, const __bf1
     quantise_into<D, FMT, V>(kv, slots[t], (int)(th - t * kv.heads), which, x, lane);
 }
 
+// The same back: a trip for the slot, one for codes and scale (9 tokens of 8 x 128: 2.5 us).
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * WAVES) void kv_read_kernel(Kv kv, const int32_t* __restrict__ slots, int64_t vectors,
                                                              __bf16* __restrict__ k, __bf16* __restrict__ v) {
@@ -352,7 +354,8 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv,
     }
 }
 
-// The same tokens read back: a tile's values go into LDS whole, each wave then takes its tokens' bytes out of them.
+// The same tokens read back: a tile's values go into LDS whole, each wave then takes its tokens' bytes out of them. 2048 tokens of
+// 4 x 256: 12.6 MB in 4.7 us, 2.7 TB/s, one workgroup to a CU whose trips in and out do not overlap.
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, const int32_t* __restrict__ slots, int n,
                                                                          __bf16* __restrict__ k, __bf16* __restrict__ v) {
@@ -434,7 +437,8 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, 
     }
 }
 
-// a workgroup for each (sequence, kv head, keys or values): 64 moves at a time read into LDS, then written
+// A workgroup for each (sequence, kv head, keys or values): 64 moves at a time read into LDS, then written. Bound by its trips to
+// memory: starts, slots, codes, out (a path of three, 4 x 256: 2.1 us).
 template <int D>
 __global__ __launch_bounds__(256) void kv_move_kernel(Kv kv, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
                                                       const int32_t* __restrict__ start) {
@@ -500,7 +504,7 @@ __device__ __forceinline__ void put(__bf16* to, const float (&y)[V], int lane) {
 // keys, values. The angles' sines and cosines are made once per workgroup, while the first heads' partials are on their way:
 // pos * inv_freq in turns in f64, whose fraction is exact to f32 at any position. P: partials of a head in
 // flight at once (summed as they come instead: a token of 16 x 256, 8 partials 4.4 us against 3.4, 5 of 24 x 256, 4 partials
-// into the cache 5.6 against 4.2, 2048 of them 33.9 against 29.9).
+// into the cache 5.6 against 4.2, 2048 dense ones, one partial 33.9 against 29.9, which is 5.9 TB/s).
 template <int D, int FMT, int P>
 __global__ __launch_bounds__(64 * WAVES) void attn_prep_kernel(const Prep a) {
     constexpr int V = D / 64;

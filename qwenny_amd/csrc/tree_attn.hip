@@ -247,7 +247,7 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
 // 12.8, at 16,000 18.7 against 15.3, at 131,000 54.5 against 51.9.)
 // Bound by HBM where the cache is long (131,000 positions of 24 x 256, e4m3: 269 MB in 45 us, 5.9 TB/s), by its chain of memory
 // trips where it is short (77 positions: 7.5 us), and with many rows by what goes on beside the matrix products: operands made
-// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 33.5 us).
+// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 31.2 us).
 template <int D, int FMT, int R, int W>
 __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args args) {
     constexpr int THREADS = 64 * W;
@@ -428,6 +428,9 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             const int lane = said, col = lane & 15, g = lane >> 4;
             const int t0 = (turn + wave) * KV_TILE;
             const bool more = turn + W < t_end, own = turn + wave < t_end;
+            // A wave at its softmax goes before one at its products, which the matrix units keep busy for longer than they take to
+            // issue (64 tokens at 8,150, 24 x 256: 37.5 us against 39.8; 13 at 30,000: 40.0 against 40.9).
+            __builtin_amdgcn_s_setprio(0);
             // s^T = k q^T: lane (col, g) gets row `col` of tokens 16 sub + 4 g + i
             f4 x[R][4];
 #pragma unroll
@@ -453,6 +456,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 }
                 HOLD();
             }
+            __builtin_amdgcn_s_setprio(1);
             if (!EARLY) load_values(turn);
 
             // the scores' and the values' scales, as the lanes need them
@@ -558,6 +562,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             }
             lds_barrier();
 
+            __builtin_amdgcn_s_setprio(0);
             // o^T += v^T p^T: the k index of both operands runs over tokens 16 w + 4 g + j, as the scores lie
 #pragma unroll
             for (int v = 0; v < W; v++) {

@@ -62,8 +62,8 @@ constexpr int group_owner(int at, int all, int used) {
     return w;
 }
 
-// The same in few steps, from 1 / all in 64 bits: ((at + 1) used - 1) / all, the half keeping it off whole numbers (-1 for
-// group -1)
+// group_owner in few steps, as join_kernel takes it, from 1 / all in 64 bits: ((at + 1) used - 1) / all, the half keeping it off
+// whole numbers (-1 for group -1). group_owner and partial_slot say what it has to give; the host tests hold it to them.
 constexpr int owner(int at, int used, double inv_all) {
     return at < 0 ? -1 : (int)(((double)at * used + (used - 0.5)) * inv_all);
 }

@@ -462,7 +462,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             // the scores' and the values' scales, as the lanes need them
             float(&ts)[2][KV_TILE] = sh.tile_scale[wave];
             ts[0][lane] = sk;
-            ts[1][lane] = sv;
+            ts[1][lane] = sv * __builtin_amdgcn_rcpf(ref);  // (exact: a power of two)
             float most = 0.0f;
             if (own && __any(sv > ref && sv < INFINITY)) most = wave_max(sv < INFINITY ? sv : 0.0f);
             __builtin_amdgcn_wave_barrier();
@@ -507,8 +507,9 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 const int e = min(__builtin_amdgcn_frexp_expf(most), 127);
                 grow = __builtin_ldexpf(ref, -e);
                 ref = __builtin_ldexpf(1.0f, e);
+                ts[1][lane] = sv * __builtin_amdgcn_rcpf(ref);
+                __builtin_amdgcn_wave_barrier();
             }
-            const float inv_ref = __builtin_amdgcn_rcpf(ref);  // (exact: a power of two)
 #pragma unroll
             for (int rt = 0; rt < R; rt++) {
                 const float next = fmaxf(top[rt], over(sh.largest[rt * 16 + col]));
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 h8 p[2];
 #pragma unroll
                 for (int sub = 0; sub < 4; sub++) {
-                    const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4] * inv_ref;
+                    const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4];
                     float pv[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {

@@ -355,7 +355,7 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv,
 }
 
 // The same tokens read back: a tile's values go into LDS whole, each wave then takes its tokens' bytes out of them. 2048 tokens of
-// 4 x 256: 12.6 MB in 4.7 us, 2.7 TB/s, one workgroup to a CU whose trips in and out do not overlap.
+// 4 x 256: 12.6 MB in 4.9 us, 2.6 TB/s, one workgroup to a CU whose trips in and out do not overlap.
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, const int32_t* __restrict__ slots, int n,
                                                                          __bf16* __restrict__ k, __bf16* __restrict__ v) {

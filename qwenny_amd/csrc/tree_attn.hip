@@ -245,9 +245,9 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
 // of a workgroup's part and one at its end. (Summed by the last workgroup of a row to arrive instead, without a second launch:
 // one workgroup reads them all then, and waits for stores and counters first. One token at 4,099 positions 13.7 us against
 // 12.8, at 16,000 18.7 against 15.3, at 131,000 54.5 against 51.9.)
-// Bound by HBM where the cache is long (131,000 positions of 24 x 256, e4m3: 269 MB in 45 us, 5.9 TB/s), by its chain of memory
-// trips where it is short (77 positions: 7.5 us), and with many rows by what goes on beside the matrix products: operands made
-// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 31.2 us).
+// Bound by HBM where the cache is long (131,000 positions of 24 x 256, e4m3: 272 MB in 45 us, 6.0 TB/s), by its chain of memory
+// trips where it is short (77 positions: 7.6 us), and with many rows by what goes on beside the matrix products: operands made
+// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 30.5 us).
 template <int D, int FMT, int R, int W>
 __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args args) {
     constexpr int THREADS = 64 * W;

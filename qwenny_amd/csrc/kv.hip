@@ -636,13 +636,11 @@ extern "C" int qh_kv_write(void* stream, const qh_kv* kv, const void* k_bf16, co
         if (n >= BATCH_FROM) {
             const Source ks = {(const __bf16*)k_bf16}, vs = {(const __bf16*)v_bf16};
             auto* f = kv->fmt == QH_KV_I8 ? kv_write_batch_kernel<D, QH_KV_I8, false> : kv_write_batch_kernel<D, QH_KV_E4M3, false>;
-            hipLaunchKernelGGL(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream, c,
-                               ks, vs, slots, (int)n, 0);
+            launch_kernel(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), (hipStream_t)stream, c, ks, vs, slots, (int)n, 0);
             return;
         }
         auto* f = kv->fmt == QH_KV_I8 ? kv_write_kernel<D, QH_KV_I8> : kv_write_kernel<D, QH_KV_E4M3>;
-        hipLaunchKernelGGL(f, grid, dim3(64 * WAVES), 0, (hipStream_t)stream, c, (const __bf16*)k_bf16, (const __bf16*)v_bf16,
-                           slots, vectors);
+        launch_kernel(f, grid, dim3(64 * WAVES), (hipStream_t)stream, c, (const __bf16*)k_bf16, (const __bf16*)v_bf16, slots, vectors);
     });
     return launched("kv_write");
 }
@@ -660,12 +658,11 @@ extern "C" int qh_kv_read(void* stream, const qh_kv* kv, const int32_t* slots, s
         constexpr int D = decltype(d)::value;
         if (n >= BATCH_FROM) {
             auto* f = kv->fmt == QH_KV_I8 ? kv_read_batch_kernel<D, QH_KV_I8> : kv_read_batch_kernel<D, QH_KV_E4M3>;
-            hipLaunchKernelGGL(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream, c,
-                               slots, (int)n, (__bf16*)k_bf16, (__bf16*)v_bf16);
+            launch_kernel(f, dim3((unsigned)((n + BATCH - 1) / BATCH), c.heads * 2), dim3(64 * BATCH_WAVES), (hipStream_t)stream, c, slots, (int)n, (__bf16*)k_bf16, (__bf16*)v_bf16);
             return;
         }
         auto* f = kv->fmt == QH_KV_I8 ? kv_read_kernel<D, QH_KV_I8> : kv_read_kernel<D, QH_KV_E4M3>;
-        hipLaunchKernelGGL(f, grid, dim3(64 * WAVES), 0, (hipStream_t)stream, c, slots, vectors, (__bf16*)k_bf16, (__bf16*)v_bf16);
+        launch_kernel(f, grid, dim3(64 * WAVES), (hipStream_t)stream, c, slots, vectors, (__bf16*)k_bf16, (__bf16*)v_bf16);
     });
     return launched("kv_read");
 }
@@ -679,8 +676,7 @@ extern "C" int qh_kv_move(void* stream, const qh_kv* kv, const int32_t* src, con
     if (n == 0 || n_seq == 0) return QH_OK;
     if (!src || !dst || !start) return fail(QH_EINVAL, "kv_move: null");
     by_dim(kv->head_dim, [&](auto d) {
-        hipLaunchKernelGGL((kv_move_kernel<decltype(d)::value>), dim3(n_seq, c.heads * 2), dim3(256), 0, (hipStream_t)stream, c, src,
-                           dst, (int)n, start);
+        launch_kernel(kv_move_kernel<decltype(d)::value>, dim3(n_seq, c.heads * 2), dim3(256), (hipStream_t)stream, c, src, dst, (int)n, start);
     });
     return launched("kv_move");
 }
@@ -721,13 +717,12 @@ extern "C" int qh_attn_prep(void* stream, const float* x, int splits, size_t n, 
             return !kv ? attn_prep_kernel<DD, 0, P> : kv->fmt == QH_KV_I8 ? attn_prep_kernel<DD, QH_KV_I8, P> : attn_prep_kernel<DD, QH_KV_E4M3, P>;
         };
         auto* f = splits == 1 ? kernel(std::integral_constant<int, 1>{}) : splits <= 4 ? kernel(std::integral_constant<int, 4>{}) : kernel(std::integral_constant<int, 8>{});
-        hipLaunchKernelGGL(f, dim3((unsigned)n, shares), dim3(64 * WAVES), 0, (hipStream_t)stream, a);
+        launch_kernel(f, dim3((unsigned)n, shares), dim3(64 * WAVES), (hipStream_t)stream, a);
         if (!batch) return;
         const int64_t ld = (int64_t)(rows->q_heads * (a.gated ? 2 : 1) + 2 * rows->kv_heads) * D;
         const Source vs = {nullptr, x, splits, (int64_t)n * ld, ld, (int)(ld - (int64_t)rows->kv_heads * D)};
         auto* fv = kv->fmt == QH_KV_I8 ? kv_write_batch_kernel<DD, QH_KV_I8, true> : kv_write_batch_kernel<DD, QH_KV_E4M3, true>;
-        hipLaunchKernelGGL(fv, dim3((unsigned)((n + BATCH - 1) / BATCH), rows->kv_heads), dim3(64 * BATCH_WAVES), 0, (hipStream_t)stream,
-                           a.kv, vs, vs, slots, (int)n, 1);
+        launch_kernel(fv, dim3((unsigned)((n + BATCH - 1) / BATCH), rows->kv_heads), dim3(64 * BATCH_WAVES), (hipStream_t)stream, a.kv, vs, vs, slots, (int)n, 1);
     });
     return launched("attn_prep");
 }

@@ -748,11 +748,11 @@ void launch(hipStream_t stream, const Args& a, int waves, int grid, bool join) {
     auto* f = a.row_tiles == 0 ? tree_attn_kernel<D, FMT, 1, 4> : tree_attn_kernel<D, FMT, 2, 4>;
     if constexpr (D == 256)
         if (waves == 8) f = tree_attn_kernel<D, FMT, 2, 8>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(64 * waves), 0, stream, a);
+    launch_kernel(f, dim3(grid), dim3(64 * waves), stream, a);
     if (!join) return;
     const unsigned n = (unsigned)a.t.n, heads = (unsigned)a.kv.heads, group = (unsigned)a.t.group;
-    if (n * heads * group <= 512) hipLaunchKernelGGL((join_kernel<D, 64>), dim3(n, heads, group * (D / 64)), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((join_kernel<D, D>), dim3(n, heads, group), dim3(256), 0, stream, a);
+    if (n * heads * group <= 512) launch_kernel(join_kernel<D, 64>, dim3(n, heads, group * (D / 64)), dim3(256), stream, a);
+    else launch_kernel(join_kernel<D, D>, dim3(n, heads, group), dim3(256), stream, a);
 }
 
 }  // namespace

@@ -355,8 +355,11 @@ int qh_attn_prep(void* stream, const float* x, int splits, size_t n, const qh_at
  * (int32 [n_seq][table_ld]): position p is token p % page of page table[b][p / page]. The step's tokens are in the cache
  * at len[b], len[b] + 1, .. (attn_prep or kv_write put them there). mask (u64 [n], or NULL): bit j of token i's: it sees
  * the sequence's j-th token of this step (a tree: itself and its ancestors); NULL: itself and those before it. All
- * tokens see the cached positions. A token that sees nothing gets zeros. n_seq <= 1024. A sequence whose numbers do not
- * fit (start not ascending or past n, len past the table) or that reads a page outside the cache gets NaN. */
+ * tokens see the cached positions. A token that sees nothing gets zeros, and so does one before start[0] or from
+ * start[n_seq] on, where start ascends within 0 .. n (padding). All other tokens get NaN: those of a sequence that has more
+ * than max_new, whose len is negative or past the table, that reads a page outside the cache, or whose start is below
+ * an earlier one, above its own end or past n (other sequences keep their outputs). Each of the n tokens' rows is written,
+ * unless n_seq is 0: then nothing is. n_seq <= 1024. */
 typedef struct qh_tree {
     size_t n;
     int32_t n_seq;

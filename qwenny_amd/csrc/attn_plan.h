@@ -22,11 +22,12 @@ struct TreeArrays {
 };
 
 // A sequence's part of the step: tokens first .. first + news, `old` positions before them, `total` in all; its rows (token,
-// query head of the kv head) in `chunks` of some rows each, its positions in `groups`. `bad`: its numbers do not fit, it gets
-// NaN.
+// query head of the kv head) in `chunks` of some rows each, its positions in `groups`. A sequence has work only if its numbers
+// fit; otherwise its tokens are nobody's (news = 0). `bad`: it has such tokens. `disorder`: its start lies before an
+// earlier sequence's, or its tokens are not start[b] <= start[b + 1] <= n: they are not taken, whatever they were meant to be.
 struct Seq {
     int first, news, old, total, chunks, groups;
-    bool bad;
+    bool bad, disorder;
 };
 
 // groups of `total` positions; `wide`: groups of twice the tiles, where there are enough for every workgroup
@@ -35,16 +36,33 @@ constexpr int group_count(int total, bool wide = false) {
     return (int)(((unsigned)total + size - 1) / size);
 }
 
-// (`rows`: a power of two)
-constexpr Seq sequence(const TreeArrays& a, int b, int rows, bool wide = false) {
+// (`rows`: a power of two; `before`: start_before(a, b), or 0 where the starts are in order. The firsts of all sequences then
+// ascend, and the tokens of those that have work follow one another: each token has one sequence at most, the last whose
+// first is not past it.)
+constexpr Seq sequence(const TreeArrays& a, int b, int rows, bool wide = false, int before = 0) {
     const int s0 = a.start[b], s1 = a.start[b + 1], len = a.len[b];
-    const int cap = (int)(a.table_ld << a.page_shift);
-    const int first = s0 < 0 ? 0 : s0 > a.n ? a.n : s0, last = s1 < first ? first : s1 > a.n ? a.n : s1;
-    const int most = a.max_new < cap ? a.max_new : cap, news = last - first < most ? last - first : most;
-    const int old = len < 0 ? 0 : len > cap - news ? cap - news : len, total = old + news;
+    const int cap = (int)(a.table_ld << a.page_shift), most = a.max_new < cap ? a.max_new : cap;
+    const bool disorder = s0 < before || s1 < s0 || s1 > a.n;
+    const int tokens = disorder ? 0 : s1 - s0;
+    const bool fits = tokens <= most && len >= 0 && len <= cap - tokens;
+    const int first = !disorder || (s0 > before && s0 <= a.n) ? s0 : before;
+    const int news = fits ? tokens : 0, old = fits ? len : 0, total = old + news;
     const int chunks = (news * a.group + rows - 1) >> __builtin_ctz(rows);
-    return Seq{first, news, old, total, chunks, chunks ? group_count(total, wide) : 0,
-               first != s0 || last != s1 || news != last - first || old != len};
+    return Seq{first, news, old, total, chunks, chunks ? group_count(total, wide) : 0, disorder || news != tokens, disorder};
+}
+
+// The largest of the starts before sequence b that are numbers of tokens at all (for steps whose starts are not in order).
+constexpr int start_before(const TreeArrays& a, int b) {
+    int most = 0;
+    for (int i = 0; i < b; i++)
+        if (a.start[i] > most && a.start[i] <= a.n) most = a.start[i];
+    return most;
+}
+
+// A token that no sequence has work for: outside of all sequences of a step in order (padding), or not served. `disorder`: some
+// sequence's.
+constexpr bool padding(const TreeArrays& a, int token, bool disorder) {
+    return !disorder && (token < a.start[0] || token >= a.start[a.n_seq]);
 }
 
 // `all` groups in a row (sequence by sequence, kv head by kv head, chunk by chunk) in equal parts for `used` <= all

@@ -28,7 +28,9 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int PLAN_HEAD = 6;  // of the plan in memory: groups, workgroups, whether the groups are wide, -, 1 / groups in 64 bits
+// The plan in memory, for join_kernel: -, workgroups, -, -, 1 / groups in 64 bits, -, -; then PLAN_SEQ numbers of each sequence, one
+// after the other for all of them: first group; first token | tokens << 20; chunks; groups.
+constexpr int PLAN_HEAD = 8, PLAN_SEQ = 4;
 
 // buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of loads past the caches
 constexpr int BUF_RSRC_WORD3 = 0x00020000;
@@ -50,7 +52,7 @@ struct Args {
     int32_t row_tiles;     // log2 of a chunk's tiles of 16 rows
     float* part;           // [2 * workgroups][rows of a chunk][D], then at byte ml_at f2 [2 * workgroups][rows of a chunk]:
     int32_t ml_at;         // maximum (log2) and sum
-    int32_t* plan;         // for join_kernel: PLAN_HEAD, each sequence's first group
+    int32_t* plan;         // [PLAN_HEAD + n_seq * PLAN_SEQ]
 };
 
 // The compiler moves nothing across: left free it converts a whole tile's codes ahead of its products and spills.
@@ -133,8 +135,8 @@ template <int D, int R, int W>
 struct Shared {
     int32_t base[2][TREE_MAX_SEQS];  // of each sequence: its first group (of 4, of 8 tiles),
     int32_t who[TREE_MAX_SEQS];   // first token | tokens << 20,
-    int32_t old[TREE_MAX_SEQS];   // positions before them | (its numbers do not fit) << 31
-    int32_t wave_sum[2][W];
+    int32_t old[TREE_MAX_SEQS];   // positions before them
+    int32_t wave_sum[3][W];
     float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
     uint64_t sees[16 * R];                // which of its sequence's tokens of this step a row sees
     f4 largest[16 * R][W / 4];            // each wave's largest score of the row,
@@ -145,61 +147,73 @@ struct Shared {
     h8 p[W][R][2][64];  // probabilities of each wave's tile
 };
 
-// The sequences' places in LDS, and the number of their groups: of four tiles in .x, of eight in .y. Up to 64 sequences each
-// wave makes the whole list for itself, more are shared by the workgroup's threads.
+// The sequences' places in LDS, and the number of their groups: of four tiles in .narrow, of eight in .wide. Up to 64 sequences
+// each wave makes the whole list for itself, more are shared by the workgroup's threads. Starts that are not in order are
+// found on the way; the list is then made anew, each sequence against all starts before it.
 struct Totals {
     int narrow, wide, units;  // (units: of the first sequence)
+    int rest;                 // REST_ bits
 };
+constexpr int REST_DISORDER = 1, REST_SOME = 2;  // starts are not in order; some tokens are in no sequence that has work
 template <int D, int R, int W>
 __device__ __forceinline__ Totals plan(const Args& a, Shared<D, R, W>& sh) {
     constexpr int THREADS = 64 * W;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool few = a.t.n_seq <= 64;
-    int before[2] = {0, 0}, units = 0;
-    for (int c = 0; c < a.t.n_seq; c += THREADS) {
-        const int b = c + (few ? lane : (int)threadIdx.x);
-        int v[2] = {0, 0}, run[2], sum[2];
-        Seq s = {};
-        if (b < a.t.n_seq) {
-            s = sequence(a.t, b, 16 * R);
-            units = a.kv.heads * s.chunks;
-            v[0] = units * s.groups;
-            v[1] = units * ((s.groups + 1) >> 1);
-        }
+    for (bool in_order = true;; in_order = false) {
+        int before[2] = {0, 0}, units = 0, rest = 0;
+        for (int c = 0; c < a.t.n_seq; c += THREADS) {
+            const int b = c + (few ? lane : (int)threadIdx.x);
+            int v[2] = {0, 0}, run[2], sum[2], some = 0;
+            Seq s = {};
+            if (b < a.t.n_seq) {
+                s = sequence(a.t, b, 16 * R, false, in_order ? 0 : start_before(a.t, b));
+                units = a.kv.heads * s.chunks;
+                v[0] = units * s.groups;
+                v[1] = units * ((s.groups + 1) >> 1);
+                some = s.bad || (b == 0 && s.first > 0) || (b == a.t.n_seq - 1 && s.first + s.news < a.t.n);
+            }
+            some = (__any(some) ? REST_SOME : 0) | (__any(s.disorder) ? REST_DISORDER : 0);
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            run[k] = v[k];  // inclusive over the wave
-            run[k] += dpp<0x111>(0, run[k]);
-            run[k] += dpp<0x112>(0, run[k]);
-            run[k] += dpp<0x114>(0, run[k]);
-            run[k] += dpp<0x118>(0, run[k]);
-            run[k] += dpp<0x142, 10>(0, run[k]);
-            run[k] += dpp<0x143, 12>(0, run[k]);
-            sum[k] = __builtin_amdgcn_readlane(run[k], 63);
-            run[k] += before[k] - v[k];
-        }
-        if (!few) {
-            if (lane == 0) sh.wave_sum[0][wave] = sum[0], sh.wave_sum[1][wave] = sum[1];
-            lds_barrier();
-            sum[0] = sum[1] = 0;
-            for (int w = 0; w < W; w++)
+            for (int k = 0; k < 2; k++) {
+                run[k] = v[k];  // inclusive over the wave
+                run[k] += dpp<0x111>(0, run[k]);
+                run[k] += dpp<0x112>(0, run[k]);
+                run[k] += dpp<0x114>(0, run[k]);
+                run[k] += dpp<0x118>(0, run[k]);
+                run[k] += dpp<0x142, 10>(0, run[k]);
+                run[k] += dpp<0x143, 12>(0, run[k]);
+                sum[k] = __builtin_amdgcn_readlane(run[k], 63);
+                run[k] += before[k] - v[k];
+            }
+            if (!few) {
+                if (lane == 0) sh.wave_sum[0][wave] = sum[0], sh.wave_sum[1][wave] = sum[1], sh.wave_sum[2][wave] = some;
+                lds_barrier();
+                sum[0] = sum[1] = some = 0;
+                for (int w = 0; w < W; w++) {
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    if (w < wave) run[k] += sh.wave_sum[k][w];
-                    sum[k] += sh.wave_sum[k][w];
+                    for (int k = 0; k < 2; k++) {
+                        if (w < wave) run[k] += sh.wave_sum[k][w];
+                        sum[k] += sh.wave_sum[k][w];
+                    }
+                    some |= sh.wave_sum[2][w];
                 }
-            lds_barrier();
+                lds_barrier();
+            }
+            if (b < a.t.n_seq) {
+                sh.base[0][b] = run[0];
+                sh.base[1][b] = run[1];
+                sh.who[b] = s.first | s.news << 20;
+                sh.old[b] = s.old;
+            }
+            before[0] += sum[0], before[1] += sum[1], rest |= some;
         }
-        if (b < a.t.n_seq) {
-            sh.base[0][b] = run[0];
-            sh.base[1][b] = run[1];
-            sh.who[b] = s.first | s.news << 20;
-            sh.old[b] = s.old | (s.bad ? 1 << 31 : 0);
-        }
-        before[0] += sum[0], before[1] += sum[1];
+        if (!few) lds_barrier();
+        rest = __builtin_amdgcn_readfirstlane(rest);
+        if (in_order && (rest & REST_DISORDER)) continue;
+        return Totals{__builtin_amdgcn_readfirstlane(before[0]), __builtin_amdgcn_readfirstlane(before[1]),
+                      __builtin_amdgcn_readfirstlane(units), rest};
     }
-    if (!few) lds_barrier();
-    return Totals{__builtin_amdgcn_readfirstlane(before[0]), __builtin_amdgcn_readfirstlane(before[1]), __builtin_amdgcn_readfirstlane(units)};
 }
 
 // x / y of numbers that all lanes have alike, where the quotient is below 2^20
@@ -210,16 +224,19 @@ __device__ __forceinline__ int divide(int x, int y) {
     return __builtin_amdgcn_readfirstlane(q);
 }
 
-// The sequence that group `at` lies in: the last with base <= at (empty ones share their successor's base).
-__device__ __forceinline__ int find_seq(const int32_t* base, int n_seq, int at) {
+// The sequence that a group or token `at` lies in: the last that begins at or before it, -1 for none (empty ones share their
+// successor's beginning).
+template <class F>
+__device__ __forceinline__ int find_seq(int n_seq, int at, F&& begin) {
     const int lane = threadIdx.x & 63;
     int n = 0;
     for (int c = 0; c < n_seq; c += 64) {
         const int b = c + lane;
-        n += __popcll(__ballot(b < n_seq && base[min(b, n_seq - 1)] <= at));
+        n += __popcll(__ballot(b < n_seq && begin(min(b, n_seq - 1)) <= at));
     }
     return n - 1;
 }
+constexpr int first_of(int who) { return who & 0xfffff; }
 
 __device__ __forceinline__ b4 load_gate(const Args& a, size_t at) { return a.gate ? *(const b4*)(a.gate + at) : b4{}; }
 
@@ -231,6 +248,19 @@ __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float to
         for (int u = 0; u < 4; u++) v[u] *= sigmoid((float)gate[u]);
     }
     *(b4*)(a.out + at) = __builtin_convertvector(v, b4);
+}
+
+// The outputs of tokens that no sequence has work for, the grid's workgroups in turn: zeros for padding, else NaN.
+template <int D, int R, int W>
+__device__ __forceinline__ void put_rest(const Args& a, const Shared<D, R, W>& sh, int rest) {
+    for (int token = blockIdx.x; token < a.t.n; token += gridDim.x) {
+        const int b = find_seq(a.t.n_seq, token, [&](int b) { return first_of(sh.who[b]); });
+        if (b >= 0 && token - first_of(sh.who[b]) < sh.who[b] >> 20) continue;
+        const uint32_t fill = padding(a.t, token, rest & REST_DISORDER) ? 0 : 0x7fc07fc0u;
+        const int pieces = a.kv.heads * a.t.group * (D / 8);
+        u4* const out = (u4*)a.out + (size_t)token * pieces;
+        for (int i = threadIdx.x; i < pieces; i += 64 * W) out[i] = u4{fill, fill, fill, fill};
+    }
 }
 
 // The work is a row of groups: for each sequence, kv head and chunk of 16 R rows, the cache in groups of 4 x 64 tokens. The
@@ -269,11 +299,17 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
     const int workgroups = __builtin_amdgcn_readfirstlane(used_workgroups(gridDim.x, groups_in_all, a.t.n_seq, totals.units));
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) {
-            a.plan[0] = groups_in_all, a.plan[1] = workgroups, a.plan[2] = wide;
+            a.plan[1] = workgroups;
             *(double*)(a.plan + 4) = 1.0 / groups_in_all;
         }
-        for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) a.plan[PLAN_HEAD + i] = sh.base[wide][i];
+        for (int i = threadIdx.x; i < a.t.n_seq; i += THREADS) {
+            const int who = sh.who[i], news = who >> 20;
+            int32_t* const seq = a.plan + PLAN_HEAD + i;
+            seq[0] = sh.base[wide][i], seq[a.t.n_seq] = who;
+            seq[2 * a.t.n_seq] = (news * a.t.group + ROWS - 1) / ROWS, seq[3 * a.t.n_seq] = group_count(sh.old[i] + news, wide);
+        }
     }
+    if (totals.rest) put_rest(a, sh, totals.rest);
     // consecutive parts on one XCD (workgroups b, b + 8, .. run on the same one)
     const int xcd = blockIdx.x & 7, at_xcd = blockIdx.x >> 3;
     if (at_xcd >= (workgroups >> 3) + (xcd < (workgroups & 7) ? 1 : 0)) return;
@@ -291,10 +327,10 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
         const Args& a = *(const Args*)again;
         const int page_shift = a.kv.page_shift;
         const int lane = tid & 63, col = lane & 15, g = lane >> 4, page_tiles = 1 << (page_shift - 6);
-        const int b = find_seq(sh.base[wide], a.t.n_seq, at);
-        const int who = __builtin_amdgcn_readfirstlane(sh.who[b]), was = __builtin_amdgcn_readfirstlane(sh.old[b]);
+        const int b = find_seq(a.t.n_seq, at, [&](int b) { return sh.base[wide][b]; });
+        const int who = __builtin_amdgcn_readfirstlane(sh.who[b]), old = __builtin_amdgcn_readfirstlane(sh.old[b]);
         const int past = at - __builtin_amdgcn_readfirstlane(sh.base[wide][b]);
-        const int first = who & 0xfffff, news = who >> 20, old = was & 0x7fffffff, total = old + news;
+        const int first = first_of(who), news = who >> 20, total = old + news;
         const int chunks = (news * a.t.group + ROWS - 1) / ROWS;
         const int groups = group_count(total, wide), unit = divide(past, groups), g0 = past - unit * groups;
         const int g1 = min(groups, g0 + hi - at);
@@ -396,9 +432,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 sh.q[r >> 4][q_part >> 2][0][(q_part & 3) * 16 + (r & 15)] = q[0];
                 sh.q[r >> 4][q_part >> 2][1][(q_part & 3) * 16 + (r & 15)] = q[1];
                 if (q_part == 0) {
-                    sh.factor[r] = was < 0 || top >= 0x7f80
-                                       ? NAN
-                                       : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
+                    sh.factor[r] = top >= 0x7f80 ? NAN : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
                     sh.start[r] = -0x1p-17f * sum;
                     sh.sees[r] = mask & ~0ull >> (64 - news);
                 }
@@ -674,27 +708,26 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     const b4 gate = load_gate(a, at);
     const int used = a.plan[1];
     const double inv_all = *(const double*)(a.plan + 4);
-    const bool wide = a.plan[2] != 0;
-    // the last sequence with start <= token; up to 64 sequences all their numbers are read at once
-    Seq s;
-    int base;
+    // the token's sequence; up to 64 sequences all their places are read at once
+    const int32_t* const seqs = a.plan + PLAN_HEAD;
+    int seq[PLAN_SEQ];
     if (a.t.n_seq <= 64) {
-        const int mine = min(lane, a.t.n_seq - 1);
-        const Seq one = sequence(a.t, mine, rows, wide);
-        const int first = a.plan[PLAN_HEAD + mine];
-        const int b = max(0, __popcll(__ballot(lane < a.t.n_seq && a.t.start[mine] <= token)) - 1);
-        s.first = __builtin_amdgcn_readlane(one.first, b), s.news = __builtin_amdgcn_readlane(one.news, b);
-        s.chunks = __builtin_amdgcn_readlane(one.chunks, b), s.groups = __builtin_amdgcn_readlane(one.groups, b);
-        base = __builtin_amdgcn_readlane(first, b);
+        int mine[PLAN_SEQ];
+#pragma unroll
+        for (int k = 0; k < PLAN_SEQ; k++) mine[k] = seqs[k * a.t.n_seq + min(lane, a.t.n_seq - 1)];
+        const int b = max(0, __popcll(__ballot(lane < a.t.n_seq && first_of(mine[1]) <= token)) - 1);
+#pragma unroll
+        for (int k = 0; k < PLAN_SEQ; k++) seq[k] = __builtin_amdgcn_readlane(mine[k], b);
     } else {
-        const int b = max(0, find_seq(a.t.start, a.t.n_seq, token));
-        s = sequence(a.t, b, rows, wide);
-        base = a.plan[PLAN_HEAD + b];
+        const int b = max(0, find_seq(a.t.n_seq, token, [&](int b) { return first_of(seqs[a.t.n_seq + b]); }));
+#pragma unroll
+        for (int k = 0; k < PLAN_SEQ; k++) seq[k] = seqs[k * a.t.n_seq + b];
     }
-    const int node = token - s.first;
-    if (node < 0 || node >= s.news) return;
+    const int base = seq[0], news = seq[1] >> 20, chunks = seq[2], groups = seq[3];
+    const int node = token - first_of(seq[1]);
+    if (node < 0 || node >= news) return;  // (tree_attn_kernel wrote the row)
     const int r = node * a.t.group + in_group;
-    const int u0 = base + (head * s.chunks + (r >> (4 + a.row_tiles))) * s.groups, u1 = u0 + s.groups;
+    const int u0 = base + (head * chunks + (r >> (4 + a.row_tiles))) * groups, u1 = u0 + groups;
     const int w0 = owner(u0, used, inv_all), parts = owner(u1 - 1, used, inv_all) - w0 + 1;
     if (parts == 1) return;  // one workgroup wrote the row
     const int first_slot = 2 * w0 + (owner(u0 - 1, used, inv_all) == w0 ? 1 : 0), in = r & (rows - 1);  // partial_slot
@@ -808,7 +841,7 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     a.scale = scale * 1.4426950408889634f;
     const int grid = (int)std::min({cus * wgs_per_cu(kv->head_dim, 1 << rt, waves), units * step->n_seq * groups, (int64_t)TREE_MAX_WGS});
     const size_t part = (size_t)2 * grid * rows * kv->head_dim * 4, ml = (size_t)2 * grid * rows * 8;
-    if (part + ml + (TREE_MAX_SEQS + PLAN_HEAD) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
+    if (part + ml + (TREE_MAX_SEQS * PLAN_SEQ + PLAN_HEAD) * 4 > PF_SK_PART_BYTES) return fail(QH_EINVAL, "tree_attn: scratch");
     a.row_tiles = rt;
     a.part = (float*)ctx_partials(ctx);
     a.ml_at = (int32_t)part;

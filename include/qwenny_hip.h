@@ -374,7 +374,9 @@ typedef struct qh_tree {
 /* out bf16 [n][q_heads * head_dim] = softmax(scale * q . k) v over what each token sees, with `gate` (bf16, NULL: none)
  * times sigmoid(gate): the out-projection's input. q, gate bf16 [n][q_heads][head_dim], q_heads a multiple of the cache's
  * heads (up to 64 times); kv head j serves q_heads / heads query heads in a row. Codes and queries are multiplied
- * exactly, softmax sums are f32, probabilities are rounded to f16 for their products. 16-byte aligned. It uses the
+ * exactly, softmax sums are f32. A probability times its value's scale is rounded to f16 relative to the largest such scale
+ * that the row sees: off by 2^-11 of itself, or by 2^-24 of that scale times the row's largest probability where that is more.
+ * What a row does not see takes nothing from it. 16-byte aligned. It uses the
  * context's scratch (calls on one context must not run concurrently on two streams) and gives the same bits each time.
  * Launch only. */
 int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,

@@ -138,7 +138,8 @@ struct Shared {
     int32_t old[TREE_MAX_SEQS];   // positions before them
     int32_t wave_sum[3][W];
     float factor[16 * R], start[16 * R];  // of each row: what its scores are multiplied by, and begin with
-    uint64_t sees[16 * R];                // which of its sequence's tokens of this step a row sees
+    uint64_t sees[16 * R];                // which of its sequence's tokens of this step a row sees,
+    int32_t sees_exp[16 * R];             // and their values' largest scale (scale_exp)
     f4 largest[16 * R][W / 4];            // each wave's largest score of the row,
     f4 largest_scale[W / 4];              // and largest scale of its values
     f4 sums[16 * R][W / 2];               // each wave's sum of the row's probabilities, and of their roundings
@@ -239,6 +240,10 @@ __device__ __forceinline__ int find_seq(int n_seq, int at, F&& begin) {
 constexpr int first_of(int who) { return who & 0xfffff; }
 
 __device__ __forceinline__ b4 load_gate(const Args& a, size_t at) { return a.gate ? *(const b4*)(a.gate + at) : b4{}; }
+
+// The least e >= NO_EXP for which a scale is below 2^e (to 2^126; such powers of two have exact reciprocals).
+constexpr int NO_EXP = -126;
+__device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? max(min(__builtin_amdgcn_frexp_expf(s), 126), NO_EXP) : NO_EXP; }
 
 // A row's output: four of its dimensions, divided by the sum and gated.
 __device__ __forceinline__ void put_out(const Args& a, size_t at, f4 v, float total, b4 gate) {
@@ -347,6 +352,12 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             if (pg < 0 || ((int64_t)pg << page_shift) >= a.kv.slots) places = NONE;
         };
         load_places(g0 * group_tiles);
+        // Whether rows may see different tokens here (a token alone in its step, without a mask, is seen by all rows there are): then
+        // lane l has the scale of the step's l-th token's value (0: of a page that the cache has not)
+        const bool apart = (news > 1 || a.mask) && t_end * KV_TILE > old;
+        const int fresh_at = old + min(lane, news - 1);
+        int fresh_page = 0;
+        if (apart) fresh_page = a.table[(size_t)b * a.t.table_ld + (fresh_at >> page_shift)];
 
         auto node_of = [&](int r) { return (int)((uint32_t)r * a.group_inv >> 20); };  // r / group
         // first element of a row's query, gate and output
@@ -404,6 +415,9 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 for (int i = 0; i < SL; i++) vc[v][i] = piece(tile, i * 1024);
             }
         };
+        float fresh = 0.0f;
+        if (apart && lane < news && fresh_page >= 0 && ((int64_t)fresh_page << page_shift) < a.kv.slots)
+            fresh = a.kv.scales[((((size_t)fresh_page * a.kv.heads + head) * 2 + 1) << page_shift) + (fresh_at & ((1 << page_shift) - 1))];
         load_keys(g0 * group_tiles);
         if (EARLY) load_values(g0 * group_tiles);
 
@@ -434,7 +448,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 if (q_part == 0) {
                     sh.factor[r] = top >= 0x7f80 ? NAN : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
                     sh.start[r] = -0x1p-17f * sum;
-                    sh.sees[r] = mask & ~0ull >> (64 - news);
+                    sh.sees[r] = mask & ~0ull >> (64 - news), sh.sees_exp[r] = NO_EXP;
                 }
             }
             r += PASS;
@@ -442,9 +456,36 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             load_query(r);
         }
         lds_barrier();
+        // A row's probabilities are rounded relative to the values that it sees: to the largest scale of those that all rows see, so
+        // far (`ref`), and of the step's tokens that it sees itself (sees_exp). A sibling's, however large, takes no bits from it.
+        // (Where one wave finds sees_exp from the scales' exponents, 5 tokens at 77 positions take 9.0 us; with a maximum over each
+        // row's tokens in the loop 9.2, over LDS 9.1; with one maximum for all rows, at the cost of those bits, 8.7.)
+        if (apart && wave == 0) {
+            // from the largest power of two down: which rows see a token of it
+            int mine = scale_exp(fresh < INFINITY ? fresh : 0.0f), exp[R];
+            uint64_t sees[R];
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) exp[rt] = NO_EXP, sees[rt] = sh.sees[rt * 16 + col];
+            for (;;) {
+                int most = over_lanes<16>(mine, [](int x, int y) { return max(x, y); });
+                most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
+                           max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
+                const uint64_t tokens = __ballot(mine == most);
+                bool open = false;
+#pragma unroll
+                for (int rt = 0; rt < R; rt++) {
+                    exp[rt] = exp[rt] == NO_EXP && (sees[rt] & tokens) ? most : exp[rt];
+                    open |= exp[rt] == NO_EXP;
+                }
+                if (most == NO_EXP || !__any(open)) break;
+                mine = mine == most ? NO_EXP : mine;
+            }
+#pragma unroll
+            for (int rt = 0; rt < R; rt++) sh.sees_exp[rt * 16 + col] = exp[rt];  // (read behind the loop's first barrier)
+        }
         float top[R], sum[R], rounded[R];  // rounded: the sum of the probabilities as they are multiplied
         f4 o[R][SL][CHAINS];
-        float ref = 0x1p-126f;  // the values' scales are taken relative to this power of two: probabilities fit f16
+        int ref = NO_EXP;  // values' scales are taken relative to 2^ref, or the row's own sees_exp above it: probabilities fit f16
 #pragma unroll
         for (int rt = 0; rt < R; rt++) {
             top[rt] = -INFINITY, sum[rt] = rounded[rt] = 0.0f;
@@ -495,10 +536,10 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
 
             // the scores' and the values' scales, as the lanes need them
             float(&ts)[2][KV_TILE] = sh.tile_scale[wave];
-            ts[0][lane] = sk;
-            ts[1][lane] = sv * __builtin_amdgcn_rcpf(ref);  // (exact: a power of two)
+            ts[0][lane] = sk, ts[1][lane] = sv;
+            const float shared = (!apart || t0 + lane < old) && sv < INFINITY ? sv : 0.0f;
             float most = 0.0f;
-            if (own && __any(sv > ref && sv < INFINITY)) most = wave_max(sv < INFINITY ? sv : 0.0f);
+            if (own && __any(shared > __builtin_ldexpf(1.0f, ref))) most = wave_max(shared);
             __builtin_amdgcn_wave_barrier();
             const bool whole = own && t0 + KV_TILE <= old;  // every row sees every token
 #pragma unroll
@@ -528,28 +569,22 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             HOLD();
             lds_barrier();
 
-            // the values' scales relative to ref; ref grows to the largest finite one's power of two
             const auto over = [](const f4(&v)[W / 4]) {
                 float m = fmaxf(fmaxf(v[0].x, v[0].y), fmaxf(v[0].z, v[0].w));
 #pragma unroll
                 for (int k = 1; k < W / 4; k++) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
                 return m;
             };
-            most = over(sh.largest_scale);
-            float grow = 1.0f;
-            if (__any(most > ref)) {
-                const int e = min(__builtin_amdgcn_frexp_expf(most), 127);
-                grow = __builtin_ldexpf(ref, -e);
-                ref = __builtin_ldexpf(1.0f, e);
-                ts[1][lane] = sv * __builtin_amdgcn_rcpf(ref);
-                __builtin_amdgcn_wave_barrier();
-            }
+            const int ref_was = ref;
+            ref = __builtin_amdgcn_readfirstlane(max(ref, scale_exp(over(sh.largest_scale))));
 #pragma unroll
             for (int rt = 0; rt < R; rt++) {
                 const float next = fmaxf(top[rt], over(sh.largest[rt * 16 + col]));
                 const float factor = sh.factor[rt * 16 + col];
+                const int sees_exp = sh.sees_exp[rt * 16 + col], exp = max(ref, sees_exp);
+                const float inv_ref = __builtin_ldexpf(1.0f, -exp);
+                float by = __builtin_ldexpf(1.0f, max(ref_was, sees_exp) - exp);
                 // the maximum is followed only where it has grown by more than 2^8 (the sums and f16 hold that)
-                float by = grow;
                 if (__any((next - top[rt]) * factor > 8.0f)) {
                     const float al = next > top[rt] ? __builtin_amdgcn_exp2f((top[rt] - next) * factor) : 1.0f;
                     sum[rt] *= al;
@@ -567,7 +602,7 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 h8 p[2];
 #pragma unroll
                 for (int sub = 0; sub < 4; sub++) {
-                    const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4];
+                    const f4 vs = *(const f4*)&ts[1][sub * 16 + g * 4] * inv_ref;  // (exact)
                     float pv[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -658,12 +693,13 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 for (int k = 1; k < W / 2; k++) s += sh.sums[rt * 16 + col][k];
                 sum[rt] = s.x + s.z;
                 const float back = -128.0f * (s.y + s.w);
+                const int exp = max(ref, sh.sees_exp[rt * 16 + col]);
 #pragma unroll
                 for (int i = 0; i < SL; i++) {
                     f4 v = o[rt][i][0];
                     if (CHAINS > 1) v += o[rt][i][CHAINS - 1];
                     if (FMT == QH_KV_I8) v = v * 0x1p24f + back;
-                    o[rt][i][0] = v * ref;
+                    o[rt][i][0] = v * __builtin_ldexpf(1.0f, exp);
                 }
             }
 #pragma unroll

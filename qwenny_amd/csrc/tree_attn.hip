@@ -446,9 +446,11 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 sh.q[r >> 4][q_part >> 2][0][(q_part & 3) * 16 + (r & 15)] = q[0];
                 sh.q[r >> 4][q_part >> 2][1][(q_part & 3) * 16 + (r & 15)] = q[1];
                 if (q_part == 0) {
-                    sh.factor[r] = top >= 0x7f80 ? NAN : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
+                    const uint64_t sees = mask & ~0ull >> (64 - news);
+                    // (a row that sees nothing has nothing that is not finite either)
+                    sh.factor[r] = top >= 0x7f80 && (old || sees) ? NAN : fminf(fmaxf(__builtin_ldexpf(a.scale, e + code_exp(FMT)), 1e-37f), 3e38f);
                     sh.start[r] = -0x1p-17f * sum;
-                    sh.sees[r] = mask & ~0ull >> (64 - news), sh.sees_exp[r] = NO_EXP;
+                    sh.sees[r] = sees, sh.sees_exp[r] = NO_EXP;
                 }
             }
             r += PASS;

@@ -454,6 +454,14 @@ def lora_silu(stream, xa, split, m_cols, b_f16, rank, rows, tab, tok_slot, slot_
                              _ptr(tok_slot), _ptr(slot_scale), n, _ptr(y), ldy or rows, _ptr(mid)))
 
 
+def _array(name, t, right, what):
+    """Refuses an array of another type than the kernels read, or not in one piece: it would be read as other numbers."""
+    if not right:
+        raise ValueError(f"{name}: {what} needed, not {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+
+
 class KvFmt(IntEnum):
     """Codes of the KV cache: int8, or the 8-bit float of 4 exponent and 3 mantissa bits; a f32 scale per vector."""
 
@@ -463,7 +471,8 @@ class KvFmt(IntEnum):
 
 class KvCache:
     """A layer's paged, quantised KV cache over the caller's device buffers (qh_kv): codes u8
-    [pages][heads][2][page * head_dim], scales f32 [pages][heads][2][page]. Slot s is token s % page of page s / page."""
+    [pages][heads][2][page * head_dim] (or another type of one byte), scales f32 [pages][heads][2][page]. Slot s is token
+    s % page of page s / page."""
 
     def __init__(self, fmt, heads, head_dim, page, codes, scales, pages=None):
         if pages is None:
@@ -474,6 +483,12 @@ class KvCache:
         for have, need in zip((codes, scales), KvCache.sizes(fmt, heads, head_dim, page, pages)):
             if hasattr(have, "numel") and have.numel() * have.element_size() < need:
                 raise ValueError(f"a cache buffer of {have.numel() * have.element_size()} bytes, {need} needed")
+        if hasattr(codes, "numel"):
+            _array("codes", codes, codes.element_size() == 1, "bytes")
+        if hasattr(scales, "numel"):
+            import torch
+
+            _array("scales", scales, scales.dtype is torch.float32, "float32")
 
     @staticmethod
     def sizes(fmt, heads, head_dim, page, pages):
@@ -494,8 +509,8 @@ class KvCache:
 
 
 class TreeStep:
-    """The sequences of a step (qh_tree), all device tensors: start int32 [n_seq + 1] (tokens start[b] .. start[b + 1] are
-    sequence b's), len int32 [n_seq] (cached positions before them), table int32 [n_seq][pages] (positions' pages), mask
+    """The sequences of a step (qh_tree), all contiguous device tensors: start int32 [n_seq + 1] (tokens start[b] ..
+    start[b + 1] are sequence b's), len int32 [n_seq] (cached positions before them), table int32 [n_seq][pages] (positions' pages), mask
     int64 / uint64 [n] (bit j: sees the sequence's j-th token of this step) or None (a chain); no sequence has more than
     max_new tokens."""
 
@@ -505,6 +520,12 @@ class TreeStep:
             raise ValueError("table: rows must be contiguous")
         if start.numel() != n_seq + 1 or len.numel() != n_seq or (mask is not None and mask.numel() < n):
             raise ValueError(f"{n_seq} tables, {start.numel()} starts, {len.numel()} lengths")
+        import torch
+
+        for name, t in (("start", start), ("len", len), ("table", table)):
+            _array(name, t, t.dtype is torch.int32, "int32")
+        if mask is not None:
+            _array("mask", mask, mask.dtype in (torch.int64, torch.uint64), "int64 or uint64")
         self._held = (start, len, table, mask)
         ld = table.stride(0) if n_seq > 1 else width
         if ld != width:

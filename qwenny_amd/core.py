@@ -59,8 +59,8 @@ MAX_OUT = 64
 
 
 def _ptr(t):
-    if t is None:
-        return None
+    if t is None or type(t) is int:  # (an address that is asked for data_ptr first takes 0.4 us instead of 0.1)
+        return t
     try:
         return t.data_ptr()
     except AttributeError:
@@ -70,7 +70,7 @@ def _ptr(t):
 def _ptrs(*tensors):
     """_ptr of each: a call's tensors at once, which takes half the time of one by one."""
     try:
-        return [t if t is None else t.data_ptr() for t in tensors]
+        return [t if t is None or type(t) is int else t.data_ptr() for t in tensors]
     except AttributeError:
         return [_ptr(t) for t in tensors]
 

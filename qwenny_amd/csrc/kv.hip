@@ -701,7 +701,7 @@ extern "C" int qh_attn_prep(void* stream, const float* x, int splits, size_t n, 
     if (n == 0) return QH_OK;
     if (!x || !q || (kv ? !slots : !k || !v) || (rows->gated && !gate) || (rows->rot && (!inv_freq || !pos)))
         return fail(QH_EINVAL, "attn_prep: null");
-    if (n > MAX_TOKENS || (uintptr_t)x % 16 || (uintptr_t)q % 16 || (uintptr_t)gate % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16)
+    if (n > MAX_TOKENS || ((uintptr_t)x | (uintptr_t)q_w | (uintptr_t)k_w | (uintptr_t)q | (uintptr_t)gate | (uintptr_t)k | (uintptr_t)v) % 16)
         return fail(QH_EINVAL, "attn_prep: %zu tokens (up to 2^20), buffers 16-byte aligned", n);
     a.x = x, a.splits = splits, a.n = (int64_t)n, a.q_heads = rows->q_heads, a.kv_heads = rows->kv_heads, a.rot = rows->rot;
     a.gated = rows->gated != 0, a.q_w = q_w, a.k_w = k_w, a.inv_freq = inv_freq, a.eps = eps, a.pos = pos, a.slots = slots;

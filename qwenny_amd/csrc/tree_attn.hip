@@ -343,6 +343,14 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
         const int live = min(ROWS, news * a.t.group - row0);
         const int t_end = min((total + KV_TILE - 1) / KV_TILE, g1 * group_tiles);
 
+        // Whether rows may see different tokens here (a token alone in its step, without a mask, is seen by all rows there are): then
+        // lane l has the scale of the step's l-th token's value (0: of a page that the cache has not). Its page is asked for ahead
+        // of the tiles' places, whose wait is then for both.
+        const bool apart = (news > 1 || a.mask) && t_end * KV_TILE > old;
+        const int fresh_at = old + min(lane, news - 1);
+        int fresh_page = 0;
+        if (apart) fresh_page = a.table[(size_t)b * a.t.table_ld + (fresh_at >> page_shift)];
+
         // where tiles lie, 64 at a time: lane l has the l-th's place in the cache (of its keys) in tiles
         uint32_t places = 0;
         auto load_places = [&](int t) {
@@ -352,13 +360,6 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             if (pg < 0 || ((int64_t)pg << page_shift) >= a.kv.slots) places = NONE;
         };
         load_places(g0 * group_tiles);
-        // Whether rows may see different tokens here (a token alone in its step, without a mask, is seen by all rows there are): then
-        // lane l has the scale of the step's l-th token's value (0: of a page that the cache has not)
-        const bool apart = (news > 1 || a.mask) && t_end * KV_TILE > old;
-        const int fresh_at = old + min(lane, news - 1);
-        int fresh_page = 0;
-        if (apart) fresh_page = a.table[(size_t)b * a.t.table_ld + (fresh_at >> page_shift)];
-
         auto node_of = [&](int r) { return (int)((uint32_t)r * a.group_inv >> 20); };  // r / group
         // first element of a row's query, gate and output
         auto row_at = [&](int r) {

@@ -258,7 +258,7 @@ struct Source {
 // bytes, 16.0 us for 2048 tokens of 4 x 256. Here the codes of 64 tokens are put into LDS and turned over: a thread writes four
 // tokens' codes of four dimensions, 16 threads the 64 bytes of a dimension; what does not fill four
 // tokens' places, at a run's ends, is written apart (by every thread that meets it, and with a wave for each vector: 9.4 us
-// against 6.9).
+// against 7.0).
 // `which0`: 0 for keys and values, 1 for values alone.
 template <int D, int FMT, bool PARTIALS>
 __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv, Source keys, Source values,
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_write_batch_kernel(Kv kv,
 }
 
 // The same tokens read back: a tile's values go into LDS whole, each wave then takes its tokens' bytes out of them. 2048 tokens of
-// 4 x 256: 12.6 MB in 4.9 us, 2.6 TB/s, one workgroup to a CU whose trips in and out do not overlap.
+// 4 x 256: 12.6 MB in 5.7 us (4.7 at best), 2.2 TB/s, one workgroup to a CU whose trips in and out do not overlap.
 template <int D, int FMT>
 __global__ __launch_bounds__(64 * BATCH_WAVES) void kv_read_batch_kernel(Kv kv, const int32_t* __restrict__ slots, int n,
                                                                          __bf16* __restrict__ k, __bf16* __restrict__ v) {

@@ -28,8 +28,8 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// The plan in memory, for join_kernel: -, workgroups, -, -, 1 / groups in 64 bits, -, -; then PLAN_SEQ numbers of each sequence, one
-// after the other for all of them: first group; first token | tokens << 20; chunks; groups.
+// The plan in memory, for join_kernel: -, workgroups, -, -, 1 / groups in 64 bits, -, -; then PLAN_SEQ numbers of each sequence,
+// one after the other for all of them: first group; first token | tokens << 20; chunks; groups.
 constexpr int PLAN_HEAD = 8, PLAN_SEQ = 4;
 
 // buffer resource word 3 (32-bit data format, no swizzle), and the cache policy of loads past the caches
@@ -281,8 +281,8 @@ __device__ __forceinline__ void put_rest(const Args& a, const Shared<D, R, W>& s
 // one workgroup reads them all then, and waits for stores and counters first. One token at 4,099 positions 13.7 us against
 // 12.8, at 16,000 18.7 against 15.3, at 131,000 54.5 against 51.9.)
 // Bound by HBM where the cache is long (131,000 positions of 24 x 256, e4m3: 272 MB in 45 us, 6.0 TB/s), by its chain of memory
-// trips where it is short (77 positions: 7.6 us), and with many rows by what goes on beside the matrix products: operands made
-// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 30.5 us).
+// trips where it is short (77 positions: 7.8 us), and with many rows by what goes on beside the matrix products: operands made
+// of codes, exponentials (64 tokens at 8,150: 12.8 GFLOP in 32 us).
 template <int D, int FMT, int R, int W>
 __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn_kernel(const Args args) {
     constexpr int THREADS = 64 * W;
@@ -387,6 +387,9 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
             return __builtin_amdgcn_make_buffer_rsrc(a.kv.codes + (size_t)place * (KV_TILE * D) + from, 0, there ? KV_TILE * D - from : 0,
                                                      BUF_RSRC_WORD3);
         };
+        // With chunks of 16 rows past the caches. One chunk reads its codes once (24 x 256, one token at 16,000 15.3 us against 16.1
+        // through them, 32 x 128 13.6 against 14.8); where a head has several, it depends (24 x 256, 5 tokens at 4,000 13.9 against
+        // 14.2, but at 1,000 13.4 against 12.6, 13 at 1,000 13.9 against 13.6).
         auto piece = [&](__amdgpu_buffer_rsrc_t tile, int at) {
             return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(tile, in_tile + (at & 4095), at & ~4095, R == 1 ? CPOL_NT : 0));
         };
@@ -706,22 +709,24 @@ __global__ __launch_bounds__(64 * W, W / 4 * wgs_per_cu(D, R, W)) void tree_attn
                 }
             }
 #pragma unroll
-                for (int rt = 0; rt < R; rt++) {
-                    const int r = rt * 16 + col;
-                    if (r >= live) continue;
-                    if (direct) {
+            for (int rt = 0; rt < R; rt++) {
+                const int r = rt * 16 + col;
+                if (r >= live) continue;
+                if (direct) {
 #pragma unroll
-                        for (int i = 0; i < SL; i++) put_out(a, row_at(r) + (slice + i) * 16 + g * 4, o[rt][i][0], sum[rt],
-                                AHEAD ? gate[rt][i] : load_gate(a, row_at(r) + (slice + i) * 16 + g * 4));
-                    } else {
-                        const uint32_t row = slot * ROWS + r;
-#pragma unroll
-                        for (int i = 0; i < SL; i++) *(f4*)(a.part + row * D + (slice + i) * 16 + g * 4) = o[rt][i][0];
-                        if (wave == 0 && g == 0)
-                            ((f2*)((uint8_t*)a.part + a.ml_at))[row] =
-                                f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * sh.factor[r], sum[rt]};
+                    for (int i = 0; i < SL; i++) {
+                        const size_t to = row_at(r) + (slice + i) * 16 + g * 4;
+                        put_out(a, to, o[rt][i][0], sum[rt], AHEAD ? gate[rt][i] : load_gate(a, to));
                     }
+                } else {
+                    const uint32_t row = slot * ROWS + r;
+#pragma unroll
+                    for (int i = 0; i < SL; i++) *(f4*)(a.part + row * D + (slice + i) * 16 + g * 4) = o[rt][i][0];
+                    if (wave == 0 && g == 0)
+                        ((f2*)((uint8_t*)a.part + a.ml_at))[row] =
+                            f2{top[rt] == -INFINITY ? -INFINITY : top[rt] * sh.factor[r], sum[rt]};
                 }
+            }
         }
         at += g1 - g0;
         if (at < hi) lds_barrier();
@@ -858,13 +863,17 @@ extern "C" int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_head
     auto units_of = [&](int rt) { return (int64_t)kv->heads * ((step->max_new * group + (16 << rt) - 1) >> (4 + rt)); };
     // Chunks of 32 rows, where there are more than 16, read the cache half as often, but leave half as many shares: from about a
     // share for each CU (24 x 256, 5 tokens at 16,000: 20.5 us against 24.4, at 4,000: 15.6 against 13.9; 32 x 128, 5 tokens at
-    // 16,000: 17.4 against 18.8, at 4,000: 13.0 against 11.7).
+    // 16,000: 17.4 against 18.8, at 4,000: 13.0 against 11.7). In batches of smaller heads 16 rows stay ahead longer (32 sequences of
+    // 5 tokens at up to 4,000: 32 x 128 42.4 against 40.7, 16 x 64 18.7 against 16.7), which this rule does not follow.
+    // Shares are counted from what the tables could hold, since the lengths are on the device: tables wider than the sequences
+    // need get the forms of the longest ones (24 x 256, 5 tokens at 4,000: 14.0 us, with tables of 131,072 positions 16.8).
     const int rt = step->max_new * group > 16 && units_of(1) * step->n_seq * groups >= (kv->head_dim == 256 ? cus * 3 / 4 : cus) ? 1 : 0;
     const int rows = 16 << rt;
     // Workgroups of four waves start soon, and are out of step with one another, so that one's products run beside another's
     // softmax (24 x 256: 32 sequences of 5 tokens 33.5 us against 41.9 of eight waves, 64 tokens at 16,000 61.6 against 65.5). One
     // long chunk alone has eight waves and half as many partial results (5 tokens at 32,700: 24.3 against 25.5, at 131,000: 59.9
-    // against 64.6; of 128 dimensions 70.0 against 62.0).
+    // against 64.6; of 128 dimensions 70.0 against 62.0). (31 tokens at 4,000 would gain, too: 19.9 against 22.2, of 128 dimensions
+    // 16.5 against 18.5; at 16,000 they lose: 42.5 against 40.2, 34.3 against 31.0.)
     const int64_t total = units_of(rt) * step->n_seq * groups;
     const int waves = rt && kv->head_dim == 256 && step->n_seq == 1 && step->max_new * group <= 32 && total >= 2 * cus ? 8 : 4;
     const int64_t units = units_of(rt);

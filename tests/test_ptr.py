@@ -24,4 +24,5 @@ def test_plain_addresses_are_found_as_fast_as_tensors_are():
     took = {name: min(timeit.repeat(lambda: call(a), number=20000, repeat=9))  # noqa: B023
             for name, call, a in (("tensor", _ptr, t), ("address", _ptr, 4096), ("tensors", lambda a: _ptrs(a, a, a), t),
                                   ("addresses", lambda a: _ptrs(a, a, a), 4096))}
-    assert took["address"] < 1.25 * took["tensor"] and took["addresses"] < 1.25 * took["tensors"], took
+    # (0.6 and 0.8 times; an exception for each address makes it 2.8 times. A busy machine moves them by half)
+    assert took["address"] < 1.8 * took["tensor"] and took["addresses"] < 1.8 * took["tensors"], took

@@ -382,6 +382,67 @@ typedef struct qh_tree {
 int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
                  float scale, const void* gate, void* out);
 
+/* A prompt's attention: qh_tree_attn for sequences of any number of new tokens (step->max_new: the most of one sequence;
+ * n <= 2^20). mask must be NULL: a token sees the cached positions, itself and the step's tokens of its sequence before it.
+ * Everything else as qh_tree_attn: the step's tokens are in the cache already, padding gets zeros, what does not fit NaN, rounding,
+ * alignment, scratch. Sequences of one token may stand beside chunks of thousands. Launch only. */
+int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
+                  float scale, const void* gate, void* out);
+
+/* ---- a step's pages, and what it says --------------------------------------------------------------------------- */
+
+/* The pages of a cache among a server's n_seq <= 1024 sequences, all arrays on the device and the caller's: free int32 [pages],
+ * of which the first *n_free are the numbers of free pages (a stack: its end is taken first); table int32 [n_seq][table_ld]
+ * and held int32 [n_seq], the pages of each sequence. A pool begins with all pages free, n_free = pages, held = 0 and tables of
+ * -1. */
+typedef struct qh_kv_pool {
+    int32_t page; /* tokens of a page, a power of two from 64 to 1024 */
+    int32_t n_seq;
+    size_t pages;
+    int32_t* free;
+    int32_t* n_free;
+    int32_t* table;
+    size_t table_ld;
+    int32_t* held;
+} qh_kv_pool;
+
+/* Pages back: each sequence keeps the pages of its first len[b] positions (int32 [n_seq]; 0: none, as a request that has ended;
+ * negative: all that it holds). Its table is -1 behind them. They go onto the stack in the places that qh_kv_plan would have taken
+ * them from. Launch only. */
+int qh_kv_release(void* stream, const qh_kv_pool* pool, const int32_t* len);
+
+/* The next step's arrays, as qh_attn_prep, qh_tree_attn and qh_chunk_attn take them: sequence b has len[b] cached positions and
+ * add[b] new tokens (int32 [n_seq]; 0: none in this step). It takes the pages it lacks for len[b] + add[b] positions, the
+ * sequences in turn; from the first for which there are not enough free pages on, those that need any get none. granted[b] (int32): 1,
+ * or 0 where it got none or its numbers do not fit (negative, past its table): its tokens' slots are -1 then, its table and held as they
+ * were. start int32 [n_seq + 1]: sums of add (a negative one counts as 0; no more than n). slots, pos int32 [n]: each token's slot and
+ * position, len[b] and the number of tokens before it in its sequence, or with mask (u64 [n] as qh_tree's, sequences up to 64 tokens)
+ * of those that it sees before itself (no more than 2^31 - 1). Tokens from start[n_seq] on: slot -1, position 0. No page is given back: qh_kv_release
+ * does that. Launch only. */
+int qh_kv_plan(void* stream, const qh_kv_pool* pool, const int32_t* len, const int32_t* add, const uint64_t* mask,
+               size_t n, int32_t* start, int32_t* slots, int32_t* pos, int32_t* granted);
+
+/* Drafted tokens held against the target's logits: speculative decoding's acceptance, from given random numbers. Of a
+ * sequence's tokens in the step (tokens int32 [n]) the first is what was said last, the others are drafts: a chain, or a tree
+ * by the step's mask (a token's parent is the last that it sees before itself). logits f32 [n][ld], `vocab` <= 2^22 of a row:
+ * the target's after each token. temp f32 [n_seq] (NULL: 1): p = softmax(logits / temp); 0: the likeliest token, the lowest of
+ * equals, with probability 1. u f32 [n][2] in [0, 1).
+ *  - draft NULL: each row's choice is the least token whose p and those before it add up to more than u[row][1]. From its first token a
+ *    sequence goes to the child that is its row's choice (of equal children the first), while there is one.
+ *  - draft f32 [n][draft_ld], chains only (mask NULL): row i has the probabilities that the token after token i was drawn from. It is
+ *    kept where u[i][0] draft < p; the first that is not is replaced by the choice, by u[i][1], among max(0, p - draft); where all
+ *    are kept, the last row's choice of p follows.
+ * next int32 [n_seq]: the token after the kept ones; count int32 [n_seq]: drafts kept; emit int32 [n]: from start[b] on, the kept drafts
+ * and next, -1 behind them. src, dst int32 [n] (or both NULL): the moves for qh_kv_move, with the step's start, that put the kept
+ * tokens' slots (of the step's table, of pages of `page` tokens) together, -1 where nothing moves; new_len int32 [n_seq] (or NULL):
+ * the positions then cached, len + 1 + count. A row with a NaN, an infinite largest logit or none that is finite, or whose temp is
+ * negative or not finite, ends its sequence with next = -1. A sequence without tokens, or whose numbers do not fit (qh_tree), has
+ * next = -1, count = 0, new_len = len; tokens of none get -1 everywhere. Sums are 64-bit. n_seq and max_new as qh_tree's;
+ * it uses the context's scratch (calls on one context must not run concurrently on two streams). Launch only. */
+int qh_verify(qh_ctx* ctx, void* stream, const float* logits, size_t ld, size_t vocab, const qh_tree* step, int page,
+              const int32_t* tokens, const float* draft, size_t draft_ld, const float* temp, const float* u,
+              int32_t* next, int32_t* count, int32_t* emit, int32_t* src, int32_t* dst, int32_t* new_len);
+
 /* ---- graph capture --------------------------------------------------------------------------------------------- */
 
 /* Replaces the capture and replay inside Graphs::run (src/cuda/core.rs:1151-1192); the graph cache around it (keys,

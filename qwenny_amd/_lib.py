@@ -52,6 +52,13 @@ class TreeC(ctypes.Structure):
                 ("table_ld", S), ("mask", P)]
 
 
+class KvPoolC(ctypes.Structure):
+    """qh_kv_pool (the pages of a cache among a server's sequences)"""
+
+    _fields_ = [("page", ctypes.c_int32), ("n_seq", ctypes.c_int32), ("pages", S), ("free", P), ("n_free", P), ("table", P),
+                ("table_ld", S), ("held", P)]
+
+
 # name -> (restype, argtypes); every symbol include/qwenny_hip.h declares
 SIGNATURES = {
     "qh_last_error": (ctypes.c_char_p, []),
@@ -99,6 +106,10 @@ SIGNATURES = {
     "qh_attn_prep": (I, [P, P, I, S, ctypes.POINTER(AttnRowsC), P, P, ctypes.c_float, P, P, P, P, ctypes.POINTER(KvC), P,
                          P, P]),
     "qh_tree_attn": (I, [P, P, P, I, ctypes.POINTER(KvC), ctypes.POINTER(TreeC), ctypes.c_float, P, P]),
+    "qh_chunk_attn": (I, [P, P, P, I, ctypes.POINTER(KvC), ctypes.POINTER(TreeC), ctypes.c_float, P, P]),
+    "qh_kv_release": (I, [P, ctypes.POINTER(KvPoolC), P]),
+    "qh_kv_plan": (I, [P, ctypes.POINTER(KvPoolC), P, P, P, S, P, P, P, P]),
+    "qh_verify": (I, [P, P, P, S, S, ctypes.POINTER(TreeC), I, P, P, S, P, P, P, P, P, P, P, P]),
     "qh_put_block": (I, [P, P, P, ctypes.POINTER(QuantC), P, S, P]),
 }
 

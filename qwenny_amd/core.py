@@ -13,7 +13,7 @@ from enum import IntEnum
 
 import numpy as np
 
-from ._lib import AttnRowsC, KvC, MatDesc, QuantC, TreeC, check, lib
+from ._lib import AttnRowsC, KvC, KvPoolC, MatDesc, QuantC, TreeC, check, lib
 
 P = ctypes.c_void_p
 
@@ -222,6 +222,28 @@ class Gemm:
         s = kv.head_dim ** -0.5 if scale is None else scale
         q, gate, out = _ptrs(q, gate, out)
         check(lib().qh_tree_attn(self._ctx, _stream(stream), q, q_heads, kv.c, step.c, s, gate, out))
+
+    def chunk_attn(self, stream, q, q_heads, kv, step, out, gate=None, scale=None):
+        """Attention of a prompt's tokens: tree_attn for sequences of any number of new tokens (`step`: a TreeStep without
+        mask), single tokens beside chunks of thousands."""
+        s = kv.head_dim ** -0.5 if scale is None else scale
+        q, gate, out = _ptrs(q, gate, out)
+        check(lib().qh_chunk_attn(self._ctx, _stream(stream), q, q_heads, kv.c, step.c, s, gate, out))
+
+    def verify(self, stream, logits, vocab, step, page, tokens, u, next, count, emit, temp=None, draft=None, src=None, dst=None,
+               new_len=None):
+        """Drafted tokens held against the target's logits f32 [n][>= vocab] (rows may be strided): `step` (a TreeStep; its mask a
+        tree of drafts) and tokens int32 [n], u f32 [n][2] random numbers, temp f32 [n_seq] (0: the likeliest), draft f32 [n][>= vocab] (the
+        probabilities that a chain's next tokens were drawn from) or None. Writes next, count int32 [n_seq], emit int32 [n] and, where
+        given, the moves src, dst int32 [n] for kv_move (slots of pages of `page` tokens) and new_len int32 [n_seq]."""
+        n, n_seq = step.c.n, step.c.n_seq
+        _verify_arrays(n, n_seq, vocab, logits, draft, tokens, u, temp, next, count, emit, src, dst, new_len)
+        ld = logits.stride(0) if n > 1 else max(vocab, logits.shape[1])
+        draft_ld = 0 if draft is None else draft.stride(0) if n > 1 else max(vocab, draft.shape[1])
+        logits, tokens, draft, temp, u, next, count, emit, src, dst, new_len = _ptrs(logits, tokens, draft, temp, u, next, count, emit,
+                                                                                     src, dst, new_len)
+        check(lib().qh_verify(self._ctx, _stream(stream), logits, ld, vocab, step.c, page, tokens, draft, draft_ld, temp, u, next,
+                              count, emit, src, dst, new_len))
 
     def put_block(self, stream, m, q, zeros, block, rows):
         """Write stored rows `rows` (16) of `q` as the 16-row block `block` of a matrix from Mat.marlin_rows, counting
@@ -596,6 +618,87 @@ def kv_move(stream, kv, src, dst, start, n_seq, n=None):
         _int32(src=src, dst=dst, start=start)
     src, dst, start = _ptrs(src, dst, start)
     check(lib().qh_kv_move(_stream(stream), kv.c, src, dst, n, start, n_seq))
+
+
+_FLOAT32 = None  # torch.float32, likewise
+
+
+def _sized(name, t, n, dtype):
+    """Refuses an array of a call that is missing, of another type, not in one piece or too short."""
+    if t is None or t.dtype is not dtype or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} needed"
+                         + ("" if t is None else f", not {t.dtype} of {t.numel()}"))
+
+
+def _verify_arrays(n, n_seq, vocab, logits, draft, tokens, u, temp, next, count, emit, src, dst, new_len):
+    global _INT32, _FLOAT32
+    if _FLOAT32 is None or _INT32 is None:
+        import torch
+
+        _INT32, _FLOAT32 = torch.int32, torch.float32
+    for name, t in (("logits", logits), ("draft", draft)):
+        if t is None and name == "draft":
+            continue
+        if t.dtype is not _FLOAT32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < n or t.shape[1] < vocab:
+            raise ValueError(f"{name}: float32 [{n}][{vocab}] with contiguous rows needed, not {t.dtype} {list(t.shape)}")
+    for name, t in (("tokens", tokens), ("emit", emit), ("src", src), ("dst", dst)):
+        if t is not None or name in ("tokens", "emit"):
+            _sized(name, t, n, _INT32)
+    for name, t in (("next", next), ("count", count), ("new_len", new_len)):
+        if t is not None or name != "new_len":
+            _sized(name, t, n_seq, _INT32)
+    _sized("u", u, 2 * n, _FLOAT32)
+    if temp is not None:
+        _sized("temp", temp, n_seq, _FLOAT32)
+
+
+class KvPool:
+    """The pages of a cache among a server's sequences (qh_kv_pool), int32 device tensors: free [pages], of which the first n_free [1] are
+    the numbers of free pages, table [n_seq][width] and held [n_seq], the pages of each sequence."""
+
+    def __init__(self, page, free, n_free, table, held):
+        import torch
+
+        global _INT32
+        _INT32 = torch.int32
+        n_seq, width = table.shape
+        for name, t, n in (("free", free, 1), ("n_free", n_free, 1), ("table", table, 1), ("held", held, n_seq)):
+            _sized(name, t, n, _INT32)
+        self.page, self.pages, self.free, self.n_free, self.table, self.held = page, free.numel(), free, n_free, table, held
+        self.c = KvPoolC(page, n_seq, free.numel(), _ptr(free), _ptr(n_free), _ptr(table), width, _ptr(held))
+
+    @classmethod
+    def new(cls, page, pages, n_seq, width, device="cuda:0"):
+        """A pool of `pages` free pages for n_seq sequences of up to `width` pages each; the lowest page is taken first."""
+        import torch
+
+        i32 = {"dtype": torch.int32, "device": device}
+        return cls(page, torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32), torch.full((n_seq, width), -1, **i32),
+                   torch.zeros(n_seq, **i32))
+
+
+def kv_release(stream, pool, len):
+    """Pages back to the pool: each sequence keeps those of its first len (int32 [n_seq]) positions."""
+    _sized("len", len, pool.c.n_seq, _INT32)
+    check(lib().qh_kv_release(_stream(stream), pool.c, _ptr(len)))
+
+
+def kv_plan(stream, pool, len, add, n, start, slots, pos, granted, mask=None):
+    """The next step's arrays from the requests' lengths: sequence b has len[b] cached positions and add[b] new tokens. Takes the
+    pages that it lacks, and writes start int32 [n_seq + 1], slots and pos int32 [n] (with mask, a tree's positions), and
+    granted int32 [n_seq] (0: no pages, its tokens' slots are -1)."""
+    n_seq = pool.c.n_seq
+    for name, t, k in (("len", len, n_seq), ("add", add, n_seq), ("start", start, n_seq + 1), ("slots", slots, n), ("pos", pos, n),
+                       ("granted", granted, n_seq)):
+        if t.dtype is not _INT32 or t.numel() < k or not t.is_contiguous():
+            _sized(name, t, k, _INT32)
+    if mask is not None:
+        import torch
+
+        if mask.dtype not in (torch.int64, torch.uint64) or mask.numel() < n or not mask.is_contiguous():
+            raise ValueError(f"mask: a contiguous int64 or uint64 tensor of {n} needed, not {mask.dtype} of {mask.numel()}")
+    len, add, mask, start, slots, pos, granted = _ptrs(len, add, mask, start, slots, pos, granted)
+    check(lib().qh_kv_plan(_stream(stream), pool.c, len, add, mask, n, start, slots, pos, granted))
 
 
 def pack_dense_bf16(w_bf16, order):

@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "gemm.h"
 #include "internal.h"
@@ -28,7 +29,15 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 8, THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+// The compiler moves nothing across: left free it fetches a whole tile's operands ahead of its products and spills.
+#define HOLD() __builtin_amdgcn_sched_barrier(0)
+#define LIKELY(x) __builtin_expect(x, 1)  // a branch that is taken makes a wave wait for its instructions, with none beside it
+#define UNLIKELY(x) __builtin_expect(x, 0)
+#define INLINE __attribute__((always_inline))  // (left out of line, a lambda's captures would be in memory)
+
+constexpr int BUF_RSRC_WORD3 = 0x00020000;  // buffer resource word 3: 32-bit data format, no swizzle
+
+constexpr int WAVES = 4, THREADS = 64 * WAVES, SETS = 2, ROWS = 32 * SETS * WAVES;  // a wave has sets of 32 rows
 
 struct Args {
     const __bf16* q;     // [n][heads][D]
@@ -55,6 +64,39 @@ __device__ __forceinline__ h4 operands(uint32_t a) {
     return h4{p[0].x, p[0].y, p[1].x, p[1].y};
 }
 
+// The matrix instructions are written out, so that outputs stay in accumulation registers and scores in vector registers: of a
+// function's builtins the compiler puts all into one kind, and moves the other's values back and forth around every product. It
+// does not know them, so what has to be waited for stands here: a register that a vector instruction wrote is read two steps later
+// (OPERANDS_READY), a product is read when it is through (PRODUCTS_READY: 8 passes and 4 steps; 20 are left). A product added to the one
+// before it in the same registers needs no wait.
+#define OPERANDS_READY() asm volatile("s_nop 3")
+#define PRODUCTS_READY() asm volatile("s_nop 15\n\ts_nop 3")
+__device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void product(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b)); }
+__device__ __forceinline__ float kept(float o) {
+    float v;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(o));
+    return v;
+}
+__device__ __forceinline__ float keep(float v) {
+    float o;
+    asm volatile("v_accvgpr_write_b32 %0, %1" : "=a"(o) : "v"(v));
+    return o;
+}
+
+// f(0), f(1), .. f(N - 1), the numbers known to the compiler
+template <class F, int... I>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each(std::make_integer_sequence<int, N>{}, f);
+}
+template <int R>
+using Set = std::integral_constant<int, R>;
+
 // over the two lanes that hold one row (l, l ^ 32)
 __device__ __forceinline__ float both_max(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -68,8 +110,9 @@ __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
 
-// The least e >= NO_EXP for which a scale is below 2^e (to 2^126; such powers of two have exact reciprocals).
-constexpr int NO_EXP = -126;
+// The least e >= NO_EXP for which a scale is below 2^e (to 2^126; such powers of two have exact reciprocals, that a probability
+// may be multiplied by).
+constexpr int NO_EXP = -100;
 __device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? max(min(__builtin_amdgcn_frexp_expf(s), 126), NO_EXP) : NO_EXP; }
 
 // The sequences' places: first unit (of 256 rows of a kv head), first token and tokens.
@@ -150,15 +193,28 @@ __device__ __forceinline__ void put_rest(const Args& a, const Plan& plan, int re
 // What a workgroup holds of a tile of 64 tokens, as operands: keys [D / 8][64 tokens] of 8 dimensions; values [4][2][D] of the 8
 // tokens 16 s + 4 h .. + 3, 16 s + 8 + 4 h .. + 3, which the product of keys and queries leaves in one lane (its half h).
 template <int D>
-struct Shared {
+struct Tile {
     h8 k[D / 8][KV_TILE];
     h8 v[4][2][D];
-    float scale[2][KV_TILE];
+    float key_scale[KV_TILE];    // with all that a score is multiplied by
+    float value_scale[KV_TILE];
+    _Float16 factor[KV_TILE];    // what the values were multiplied by
+};
+template <int D>
+struct Shared {
+    Tile<D> tile[2];
+    int32_t top_exp[WAVES];
     Plan plan;
 };
 
+// A lane's row's softmax: the reference m that scores are taken against (in powers of two), and the sums of 2^(score - m). A score
+// may come to m + 15, since f16 holds that; m is set 7 below a largest score, so that probabilities keep f16's full bits down to 2^-21
+// of the largest and are dropped below 2^-32.
+constexpr float ROOM = 15.0f, BELOW = 7.0f;
+constexpr int VALUE_EXP = 7;  // values are taken relative to 2^-7 of the largest scale, for the same reason
+
 template <int D, int FMT>
-__global__ __launch_bounds__(THREADS, 2) void chunk_attn_kernel(const Args a) {
+__global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(const Args a) {
     __shared__ Shared<D> sh;
     int rest;
     const int units = make_plan(a, sh.plan, &rest);
@@ -176,154 +232,426 @@ __global__ __launch_bounds__(THREADS, 2) void chunk_attn_kernel(const Args a) {
     const int all_see = old + row0 / group + 1;   // positions that all its rows see
     const int t_end = (old + last / group + 1 + KV_TILE - 1) / KV_TILE;
 
-    const int row = min(row0 + wave * 32 + col, last), node = row / group;
-    const int sees = old + node + 1;
-    const size_t at = ((size_t)(first + node) * a.kv.heads * group + head * group + (row - node * group)) * D;
+    // the lane's row of a set, and its first query and output
+    auto row_of = [&](int r) INLINE { return row0 + wave * (32 * SETS) + r * 32 + col; };
+    auto row_at = [&](int r) INLINE {
+        const int row = min(row_of(r), last), node = row / group;
+        return ((size_t)(first + node) * a.kv.heads * group + head * group + (row - node * group)) * D;
+    };
+    int sees[SETS];
+#pragma unroll
+    for (int r = 0; r < SETS; r++) sees[r] = old + min(row_of(r), last) / group + 1;
 
-    // the lane's queries: dimensions 16 i + 8 half .. + 7, scaled by a power of two into f16's range (the factor goes to the scores)
-    h8 q[D / 16];
-    float factor;
-    {
-        b8 raw[D / 16];
-        uint32_t top = 0;  // bf16 with the sign taken off compares as a whole number; from 0x7f80 on it is not finite
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-            raw[i] = *(const b8*)(a.q + at + i * 16 + half * 8);
-            const u4 bits = __builtin_bit_cast(u4, raw[i]);
-#pragma unroll
-            for (int k = 0; k < 4; k++) top = max(top, max(bits[k] & 0x7fffu, bits[k] >> 16 & 0x7fffu));
-        }
-        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        top = max(both[0], both[1]);
-        const int e = top < 0x7f80 ? __builtin_amdgcn_frexp_expf(__uint_as_float(top << 16)) - 15 : 0;
-#pragma unroll
-        for (int i = 0; i < D / 16; i++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) q[i][k] = (_Float16)__builtin_ldexpf((float)raw[i][k], -e);
-        factor = top >= 0x7f80 ? NAN : fminf(fmaxf(__builtin_ldexpf(a.scale, e), 1e-37f), 3e38f);
-    }
-
-    f16 o[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; i++)
-#pragma unroll
-        for (int k = 0; k < 16; k++) o[i][k] = 0.0f;
-    float top = -INFINITY, sum = 0.0f;
-    int exp = NO_EXP;  // values' scales are taken relative to 2^exp, the largest that the row sees: probabilities fit f16
+    // where tiles lie, 64 at a time: lane l has the l-th's place in the cache (of its keys) in tiles
+    constexpr uint32_t NONE = ~0u;
     const int page_tiles = 1 << (a.kv.page_shift - 6);
+    uint32_t places = 0;
+    auto load_places = [&](int t) INLINE {
+        const int mine = min(t + lane, t_end - 1);
+        const int page = a.table[(size_t)b * a.t.table_ld + (mine >> (a.kv.page_shift - 6))];
+        places = (uint32_t)((page * a.kv.heads + head) * 2 * page_tiles + (mine & (page_tiles - 1)));
+        if (page < 0 || ((int64_t)page << a.kv.page_shift) >= a.kv.slots) places = NONE;
+    };
+    load_places(0);
 
-    for (int t = 0; t < t_end; t++) {
-        const int page = a.table[(size_t)b * a.t.table_ld + (t >> (a.kv.page_shift - 6))];
-        const bool none = page < 0 || ((int64_t)page << a.kv.page_shift) >= a.kv.slots;
-        const size_t place = none ? 0 : ((size_t)page * a.kv.heads + head) * 2 * page_tiles + (t & (page_tiles - 1));
-        const int there = none ? 0 : min(old + news - t * KV_TILE, KV_TILE);  // tokens of the tile that were written
+    // a thread's pieces of a tile: 16 dimensions of a token's key, 16 tokens of a dimension of the values
+    constexpr int PIECES = KV_TILE * D / 16 / THREADS;
+    const int l16 = lane & 15, c4 = lane >> 4, g4 = (c4 & 1) * 2 + (c4 >> 1);
+    u4 raw[PIECES];
+    float ks, vs;
+    bool none;
+    uint32_t place;
+    // (buffer loads: an address is a lane's 32 bits beside what the wave has alike)
+    auto rsrc = [&](const void* p, int bytes) INLINE { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, BUF_RSRC_WORD3); };
+    auto piece = [&](__amdgpu_buffer_rsrc_t codes, int at, int i) INLINE {
+        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(codes, at, (wave + i * WAVES) * 1024, 0));
+    };
+    auto load_keys = [&](int t) INLINE {
+        if (UNLIKELY((t & 63) == 0 && t)) load_places(t);
+        const uint32_t p = __builtin_amdgcn_readlane(places, t & 63);
+        none = p == NONE;
+        place = none ? 0 : p;
+        const auto sc = rsrc(a.kv.scales + (size_t)place * KV_TILE, (page_tiles + 1) * KV_TILE * 4);
+        ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sc, lane * 4, 0, 0));
+        vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sc, lane * 4, page_tiles * KV_TILE * 4, 0));
+        const auto codes = rsrc(a.kv.codes + (size_t)place * (KV_TILE * D), KV_TILE * D);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16 * 64 + c4 * 16, i);
+    };
+    auto load_values = [&]() INLINE {
+        const auto codes = rsrc(a.kv.codes + ((size_t)place + page_tiles) * (KV_TILE * D), KV_TILE * D);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16 * 64 + g4 * 16, i);
+    };
+    auto put_keys = [&](Tile<D>& to, int i) INLINE {
+        const int u = wave + i * WAVES, token = u / (D / 64) * 16 + l16, chunk = u % (D / 64) * 8 + c4 * 2;
+        const h4 k0 = operands<FMT>(raw[i].x), k1 = operands<FMT>(raw[i].y), k2 = operands<FMT>(raw[i].z), k3 = operands<FMT>(raw[i].w);
+        to.k[chunk][token] = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
+        to.k[chunk + 1][token] = __builtin_shufflevector(k2, k3, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    h4 factor[4];  // of the thread's tokens
+    auto load_factors = [&](const Tile<D>& to) INLINE {
+#pragma unroll
+        for (int s = 0; s < 4; s++) factor[s] = *(const h4*)&to.factor[s * 16 + g4 * 4];
+    };
+    auto put_values = [&](Tile<D>& to, int i, int there) INLINE {
+        const int dim = (wave + i * WAVES) * 16 + l16;
+        if (FMT == QH_KV_E4M3 && UNLIKELY(there < KV_TILE)) {  // what was not written may be NaN codes, which no probability takes away
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const int keep = max(there - (s * 16 + g4 * 4), 0);
+                raw[i][s] = keep < 4 ? raw[i][s] & ((1u << 8 * keep) - 1) : raw[i][s];
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) ((h4*)&to.v[s][g4 & 1][dim])[g4 >> 1] = operands<FMT>(raw[i][s]) * factor[s];
+    };
+
+    // the lane's queries: dimensions 16 i + 8 half .. + 7, scaled by a power of two into f16's range. One power for the workgroup, that goes
+    // into the keys' scales; in a wave with rows 2^16 and more below the largest, or not finite, each row its own, with a factor for
+    // what it then differs by.
+    // Where queries reach 2^55, the rest of the power is left to the differences of scores (`late`): the scores themselves might be
+    // infinite. All tiles are then taken apart.
+    h8 q[SETS][D / 16];
+    float key_factor, row_factor[SETS], late;
+    bool wide = false;
+    {
+        constexpr int LOW = -1000;
+        uint32_t top[SETS];  // bf16 with the sign taken off compares as a whole number; from 0x7f80 on it is not finite
+        int e[SETS], most = LOW;
+#pragma unroll
+        for (int r = 0; r < SETS; r++) {
+            top[r] = 0;
+            const size_t at = row_at(r);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const u4 bits = *(const u4*)(a.q + at + i * 16 + half * 8);
+#pragma unroll
+                for (int k = 0; k < 4; k++) top[r] = max(top[r], max(bits[k] & 0x7fffu, bits[k] >> 16 & 0x7fffu));
+            }
+            const auto both = __builtin_amdgcn_permlane32_swap(top[r], top[r], false, false);
+            top[r] = max(both[0], both[1]);
+            e[r] = top[r] && top[r] < 0x7f80 ? __builtin_amdgcn_frexp_expf(__uint_as_float(top[r] << 16)) - 15 : LOW;
+            most = max(most, e[r]);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) most = max(most, __shfl_xor(most, d));
+        if (lane == 0) sh.top_exp[wave] = most;
         __syncthreads();
-        for (int p = tid; p < KV_TILE * D / 16; p += THREADS) {
-            const int u = p >> 6, l = p & 63, c = l >> 4;
-            const uint8_t* const codes = a.kv.codes + place * (KV_TILE * D) + u * 1024 + (l & 15) * 64;
-            const u4 k = *(const u4*)(codes + c * 16);
-            const int token = u / (D / 64) * 16 + (l & 15), chunk = u % (D / 64) * 8 + c * 2;
-            const h4 k0 = operands<FMT>(k.x), k1 = operands<FMT>(k.y), k2 = operands<FMT>(k.z), k3 = operands<FMT>(k.w);
-            sh.k[chunk][token] = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
-            sh.k[chunk + 1][token] = __builtin_shufflevector(k2, k3, 0, 1, 2, 3, 4, 5, 6, 7);
-            const int g = (c & 1) * 2 + (c >> 1);
-            u4 v = *(const u4*)(codes + (size_t)page_tiles * (KV_TILE * D) + g * 16);
-            if (FMT == QH_KV_E4M3 && there < KV_TILE) {  // what was not written may be NaN codes, which no probability takes away
+        for (int w = 0; w < WAVES; w++) most = max(most, sh.top_exp[w]);
+        most = __builtin_amdgcn_readfirstlane(most == LOW ? 0 : most);
 #pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const int keep = max(there - (s * 16 + g * 4), 0);
-                    v[s] = keep < 4 ? v[s] & ((1u << 8 * keep) - 1) : v[s];
-                }
+        for (int r = 0; r < SETS; r++) wide |= __any(top[r] >= 0x7f80 || (top[r] && e[r] < most - 16));
+#pragma unroll
+        for (int r = 0; r < SETS; r++) {
+            row_factor[r] = !wide ? 1.0f : top[r] >= 0x7f80 ? NAN : __builtin_ldexpf(1.0f, e[r] == LOW ? 0 : e[r] - most);
+            const int by = wide && e[r] != LOW ? e[r] : most;
+            const size_t at = row_at(r);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const b8 in = *(const b8*)(a.q + at + i * 16 + half * 8);
+#pragma unroll
+                for (int k = 0; k < 8; k++) q[r][i][k] = (_Float16)__builtin_ldexpf((float)in[k], -by);
+                if (i % 4 == 3) HOLD();
             }
-#pragma unroll
-            for (int s = 0; s < 4; s++) ((h4*)&sh.v[s][g & 1][u * 16 + (l & 15)])[g >> 1] = operands<FMT>(v[s]);
         }
-        if (tid < 2 * KV_TILE) {
-            const int which = tid >> 6;
-            sh.scale[which][lane] = none ? NAN : a.kv.scales[(place + which * page_tiles) * KV_TILE + lane];
-        }
-        __syncthreads();
-        const bool whole = (t + 1) * KV_TILE <= all_see;
-#pragma unroll 1
-        for (int tb = 0; tb < 2; tb++) {
-            // s^T = k q^T: the lane gets its row's scores of tokens 8 (i / 4) + 4 half + i % 4
-            f16 x;
-#pragma unroll
-            for (int k = 0; k < 16; k++) x[k] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(sh.k[2 * i + half][tb * 32 + col], q[i], x, 0, 0, 0);
-            const int t0 = t * KV_TILE + tb * 32 + half * 4;
-            float mx = -INFINITY, largest = 0.0f;
-            f4 vs[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f4 ks = *(const f4*)&sh.scale[0][tb * 32 + j * 8 + half * 4];
-                vs[j] = *(const f4*)&sh.scale[1][tb * 32 + j * 8 + half * 4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const bool seen = whole || t0 + 8 * j + i < sees;
-                    const float s = seen ? x[4 * j + i] * ks[i] : -INFINITY;
-                    x[4 * j + i] = s;
-                    mx = fmaxf(mx, s);
-                    largest = fmaxf(largest, seen && vs[j][i] < INFINITY ? vs[j][i] : 0.0f);
-                }
-            }
-            mx = both_max(mx), largest = both_max(largest);
-            const int exp_was = exp;
-            exp = max(exp, scale_exp(largest));
-            float by = __builtin_ldexpf(1.0f, exp_was - exp);
-            const float next = fmaxf(top, mx);
-            // the maximum is followed only where it has grown by more than 2^8 (the sums and f16 hold that)
-            if (__any((next - top) * factor > 8.0f)) {
-                const float al = next > top ? __builtin_amdgcn_exp2f((top - next) * factor) : 1.0f;
-                sum *= al;
-                top = next;
-                by *= al;
-            }
-            if (__any(by != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) o[i] *= by;
-            }
-            const float off = top == -INFINITY ? 0.0f : top, inv = __builtin_ldexpf(1.0f, -exp);
-            h8 p[2];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float pv[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float s = x[4 * j + i], pr = __builtin_amdgcn_exp2f((s - off) * factor);
-                    pv[i] = s == -INFINITY ? 0.0f : pr * (vs[j][i] * inv);
-                    sum += pr;
-                }
-                const h2 p0 = __builtin_convertvector((f2{pv[0], pv[1]}), h2), p1 = __builtin_convertvector((f2{pv[2], pv[3]}), h2);
-                const int k = (j & 1) * 4;
-                p[j >> 1][k] = p0.x, p[j >> 1][k + 1] = p0.y, p[j >> 1][k + 2] = p1.x, p[j >> 1][k + 3] = p1.y;
-            }
-            // o^T += v^T p^T: the lane has its row's dimensions 32 i + 8 (k / 4) + 4 half + k % 4
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int i = 0; i < D / 32; i++)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(sh.v[tb * 2 + s][half][i * 32 + col], p[s], o[i], 0, 0, 0);
-        }
+        key_factor = fmaxf(__builtin_ldexpf(a.scale, min(most, 40)), 1e-37f);
+        late = __builtin_ldexpf(1.0f, max(most - 40, 0));
     }
 
-    if (row0 + wave * 32 + col > last) return;
-    sum = both_sum(sum);
-    const float total = __builtin_ldexpf(__builtin_amdgcn_rcpf(sum), exp);
+    // Values are multiplied by their scales as they become operands, relative to 2^ref, the largest scale so far: for tiles that all rows
+    // see whole. In other tiles (`apart`) the scales go to the probabilities, relative to the largest that the row itself sees.
+    int ref = NO_EXP;
+    bool apart = false, apart_next = false;
+    int ref_next = NO_EXP;
+    // what is said of a tile before its values become operands
+    auto put_scales = [&](Tile<D>& to, int t) INLINE {
+        if (none) ks = vs = NAN;
+        const bool whole = (t + 1) * KV_TILE <= all_see;
+        apart_next = apart_next || !whole || late > 1.0f || __any(!(vs < INFINITY));  // (and so for good: units then only grow)
+        if (UNLIKELY(!apart_next && __any(vs > __builtin_ldexpf(1.0f, ref_next)))) {
+            float most = vs;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const size_t d = at + i * 32 + j * 8 + half * 4;
-            f4 v = f4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]} * total;
-            if (a.gate) {
-                const b4 g = *(const b4*)(a.gate + d);
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] *= sigmoid((float)g[k]);
-            }
-            *(b4*)(a.out + d) = __builtin_convertvector(v, b4);
+            for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+            ref_next = __builtin_amdgcn_readfirstlane(max(ref_next, scale_exp(most)));
         }
+        // (Each wave writes them all: one that did it alone would be late for the others.) A value that is not finite goes by its token's
+        // score: what sees it is NaN, and nothing else.
+        to.key_scale[lane] = vs < INFINITY ? ks * key_factor : NAN;
+        to.value_scale[lane] = vs < INFINITY ? vs : 0.0f;
+        to.factor[lane] = apart_next ? (_Float16)1.0f : (_Float16)__builtin_ldexpf(vs, VALUE_EXP - ref_next);
+    };
+    auto written = [&](int t) INLINE { return none ? 0 : min(old + news - t * KV_TILE, KV_TILE); };  // tokens of the tile
+
+    f16 o[SETS][D / 32];
+    float m[SETS], sum[SETS];
+    int unit[SETS];  // o is in units of 2^unit
+    each<SETS>([&](auto set) INLINE {
+        constexpr int r = decltype(set)::value;
+        m[r] = -INFINITY, sum[r] = 0.0f, unit[r] = NO_EXP;
+        each<D / 32>([&](auto i) INLINE { each<16>([&](auto k) INLINE { o[r][i][k.value] = keep(0.0f); }); });
+    });
+    auto scale_out = [&](auto set, float by) INLINE {
+        constexpr int r = decltype(set)::value;
+        HOLD();
+        PRODUCTS_READY();
+        each<D / 32>([&](auto i) INLINE {
+            HOLD();
+            each<16>([&](auto k) INLINE { o[r][i][k.value] = keep(kept(o[r][i][k.value]) * by); });
+        });
+        HOLD();
+        OPERANDS_READY();
+    };
+
+    f16 x[SETS];    // scores of 32 tokens: the lane has its rows' of tokens 8 (i / 4) + 4 half + i % 4
+    h8 p[SETS][2];  // their probabilities, as operands
+    float mx[SETS];
+    int to[SETS];  // the units that the values then have
+    // A set's scores relative to m (as yet none: as they are), in 16 steps that may go on beside products.
+    f4 sc[2];
+    auto load_scales = [&](const Tile<D>& tile, int tb, auto at) INLINE {
+        constexpr int j = decltype(at)::value;
+        sc[j & 1] = *(const f4*)&tile.key_scale[tb * 32 + j * 8 + half * 4];
+    };
+    auto relative = [&](const Tile<D>& tile, int tb, auto set, auto at) INLINE {
+        constexpr int r = decltype(set)::value, k = decltype(at)::value;
+        if constexpr (k % 4 == 0 && k < 12) load_scales(tile, tb, Set<k / 4 + 1>{});
+        const float s = __builtin_fmaf(x[r][k], sc[k / 4 & 1][k & 3], m[r] == -INFINITY ? -0.0f : -m[r]);
+        x[r][k] = s;
+        mx[r] = k == 0 ? s : fmaxf(mx[r], s);
+    };
+    // then, in tiles taken apart, what a row does not see is left out; the units that the values have
+    auto mask = [&](const Tile<D>& tile, int t, int tb, auto set) INLINE {
+        constexpr int r = decltype(set)::value;
+        to[r] = ref - VALUE_EXP;
+        if (LIKELY(!apart)) return;
+        const int t0 = t * KV_TILE + tb * 32 + half * 4, behind = (t + 1) * KV_TILE <= all_see ? 0x7fffffff : sees[r];
+        float largest = 0.0f;
+        mx[r] = -INFINITY;
+        each<4>([&](auto at) INLINE {
+            constexpr int j = decltype(at)::value;
+            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half * 4];
+            HOLD();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool seen = t0 + 8 * j + i < behind;
+                x[r][4 * j + i] = seen ? x[r][4 * j + i] : -INFINITY;
+                mx[r] = fmaxf(mx[r], x[r][4 * j + i]);
+                largest = fmaxf(largest, seen ? sv[i] : 0.0f);
+            }
+        });
+        to[r] = max(max(ref, unit[r]), scale_exp(both_max(largest)));
+    };
+    // whether m has to follow, or the units change
+    auto moved = [&](auto set) INLINE {
+        constexpr int r = decltype(set)::value;
+        return __any(mx[r] * late > ROOM || m[r] == -INFINITY || unit[r] != to[r]);
+    };
+    // m follows the scores where some are above ROOM, by whole numbers: the power of two by which the sums are multiplied
+    auto follow = [&](auto set) INLINE {
+        constexpr int r = decltype(set)::value;
+        const float most = both_max(mx[r]);
+        const bool none = m[r] == -INFINITY;
+        const float up = most * late > ROOM || (none && most > -INFINITY) 
+                             ? (fabsf(most * late) < 0x1p30f ? floorf(most * late - BELOW) / late : most) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; k++) x[r][k] -= up;
+        m[r] = none ? (most > -INFINITY ? up : m[r]) : m[r] + up;
+        const float by = none ? 1.0f : __builtin_amdgcn_exp2f(-up * late);
+        sum[r] *= by;
+        const float units = __builtin_ldexpf(by, unit[r] - to[r]);
+        unit[r] = to[r];
+        return units;
+    };
+    // In tiles taken apart the sum is of the probabilities by themselves, and their values' scales go into the exponents.
+    auto settle = [&](const Tile<D>& tile, int tb, auto set) INLINE {
+        constexpr int r = decltype(set)::value;
+        if (LIKELY(!apart)) return;
+        each<4>([&](auto at) INLINE {
+            constexpr int j = decltype(at)::value;
+            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half * 4];
+            HOLD();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float s = x[r][4 * j + i] * late;
+                sum[r] += __builtin_amdgcn_exp2f(s);
+                x[r][4 * j + i] = s + (__builtin_amdgcn_logf(sv[i]) - (float)unit[r]);  // (log2; an unseen token's score is -inf)
+            }
+        });
+    };
+    // The probabilities of a set's scores, in 16 steps beside products. (Sums are of the probabilities as they are multiplied.)
+    h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
+    float even;
+    auto soft = [&](auto set, auto at) INLINE {
+        constexpr int r = decltype(set)::value, k = decltype(at)::value;
+        const float pr = __builtin_amdgcn_exp2f(x[r][k]);
+        if constexpr (k % 2 == 0) {
+            even = pr;
+        } else {
+            const h2 pp = __builtin_convertvector((f2{even, pr}), h2);
+            sum[r] = __builtin_amdgcn_fdot2(pp, ones, sum[r], false);
+            p[r][k >> 3][(k & 7) - 1] = pp.x, p[r][k >> 3][k & 7] = pp.y;
+        }
+    };
+
+    constexpr int DEEP = 4;  // operands under way
+    // s^T = k q^T of 32 tokens, with `beside(i)` beside the products of 16 dimensions
+    auto scores = [&](const Tile<D>& tile, int tb, auto&& beside) INLINE {
+        h8 f[DEEP];
+        auto key = [&](int i) INLINE { return tile.k[2 * i + half][tb * 32 + col]; };
+#pragma unroll
+        for (int k = 0; k < DEEP - 1; k++) f[k] = key(k);
+        each<D / 16>([&](auto at) INLINE {
+            constexpr int i = decltype(at)::value;
+            HOLD();
+            if constexpr (i + DEEP - 1 < D / 16) f[(i + DEEP - 1) % DEEP] = key(i + DEEP - 1);
+#pragma unroll
+            for (int r = 0; r < SETS; r++) {
+                if constexpr (i == 0) product_first(x[r], f[0], q[r][0]);
+                else product(x[r], f[i % DEEP], q[r][i]);
+            }
+            beside(at);
+        });
+        HOLD();
+    };
+    // o^T += v^T p^T of a set: the lane has its row's dimensions 32 i + 8 (k / 4) + 4 half + k % 4
+    constexpr int PRODUCTS = D / 32 * 2;  // of 32 dimensions, then of 16 tokens
+    auto outputs = [&](const Tile<D>& tile, int tb, auto set, auto&& beside) INLINE {
+        constexpr int r = decltype(set)::value;
+        h8 f[DEEP];
+        auto value = [&](int n) INLINE { return tile.v[tb * 2 + n / (D / 32)][half][n % (D / 32) * 32 + col]; };
+#pragma unroll
+        for (int k = 0; k < DEEP - 1; k++) f[k] = value(k);
+        HOLD();
+        OPERANDS_READY();
+        each<PRODUCTS>([&](auto at) INLINE {
+            constexpr int n = decltype(at)::value;
+            HOLD();
+            if constexpr (n + DEEP - 1 < PRODUCTS) f[(n + DEEP - 1) % DEEP] = value(n + DEEP - 1);
+            product_kept(o[r][n % (D / 32)], f[n % DEEP], p[r][n / (D / 32)]);
+            beside(at);
+        });
+        HOLD();
+    };
+    // 16 steps spread over a set's products
+    auto spread = [&](auto at, auto&& step) INLINE {
+        constexpr int n = decltype(at)::value, from = 16 * n / PRODUCTS, to = 16 * (n + 1) / PRODUCTS;
+        each<to - from>([&](auto k) INLINE { step(std::integral_constant<int, from + decltype(k)::value>{}); });
+    };
+    const auto nothing = [](auto) INLINE {};
+
+    load_keys(0);
+    put_scales(sh.tile[0], 0);
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) put_keys(sh.tile[0], i);
+    load_values();
+    __syncthreads();
+    load_factors(sh.tile[0]);
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) put_values(sh.tile[0], i, written(0));
+    apart = apart_next, ref = ref_next;
+    __syncthreads();
+    // The second set's products with the values stand behind the next block's scores: the first set's softmax then has them beside it,
+    // and the second set's the first set's products. To begin with, probabilities of nothing.
+#pragma unroll
+    for (int k = 0; k < 8; k++) p[1][0][k] = p[1][1][k] = (_Float16)0.0f;
+    auto widen = [&]() INLINE {
+        if (UNLIKELY(wide)) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) x[0][k] *= row_factor[0], x[1][k] *= row_factor[1];
+        }
+    };
+    auto first_set = [&](const Tile<D>& tile, int t, int tb) INLINE {
+        PRODUCTS_READY();
+        widen();
+        load_scales(tile, tb, Set<0>{});
+        each<16>([&](auto k) INLINE { relative(tile, tb, Set<0>{}, k); });
+        mask(tile, t, tb, Set<0>{});
+    };
+    scores(sh.tile[0], 0, nothing);
+    first_set(sh.tile[0], 0, 0);
+    (void)follow(Set<0>{});
+    settle(sh.tile[0], 0, Set<0>{});
+    int t = 0;
+    do {  // (there is a tile at least; a loop that might not run would have its outputs in registers of their own)
+        const Tile<D>& tile = sh.tile[t & 1];
+        Tile<D>& next = sh.tile[(t + 1) & 1];
+        const bool more = t + 1 < t_end;
+        each<2>([&](auto block) INLINE {
+            constexpr int tb = decltype(block)::value;
+            const Tile<D>& before = tb ? tile : sh.tile[(max(t, 1) - 1) & 1];
+            if (LIKELY(more)) {
+                if constexpr (tb == 0) load_keys(t + 1);
+                else load_values();
+            }
+            ones = apart ? h2{(_Float16)0.0f, (_Float16)0.0f} : h2{(_Float16)1.0f, (_Float16)1.0f};
+            load_scales(tile, tb, Set<0>{});
+            outputs(before, tb ^ 1, Set<1>{}, [&](auto at) INLINE {
+                spread(at, [&](auto k) INLINE {
+                    soft(Set<0>{}, k);
+                    relative(tile, tb, Set<1>{}, k);
+                });
+            });
+            mask(tile, t, tb, Set<1>{});
+            if (UNLIKELY(moved(Set<1>{}))) scale_out(Set<1>{}, follow(Set<1>{}));
+            settle(tile, tb, Set<1>{});
+            outputs(tile, tb, Set<0>{}, [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<1>{}, k); }); });
+            if (tb == 0 || LIKELY(more)) {
+                const Tile<D>& coming = tb == 0 ? tile : next;
+                // the next tile's operands beside the scores, late enough for its codes to be there
+                scores(coming, tb ^ 1, [&](auto at) INLINE {
+                    constexpr int i = decltype(at)::value - D / 32;
+                    if constexpr (i == -1) {
+                        if constexpr (tb == 0) {
+                            if (LIKELY(more)) put_scales(next, t + 1);
+                        } else {
+                            load_factors(next);
+                        }
+                    }
+                    if constexpr (i >= 0 && i % 2 == 0 && i / 2 < PIECES) {
+                        if constexpr (tb == 0) {
+                            if (LIKELY(more)) put_keys(next, i / 2);
+                        } else {
+                            put_values(next, i / 2, written(t + 1));
+                        }
+                    }
+                });
+                if constexpr (tb == 1) apart = apart_next, ref = ref_next;
+                first_set(coming, t + tb, tb ^ 1);
+                if (UNLIKELY(moved(Set<0>{}))) scale_out(Set<0>{}, follow(Set<0>{}));
+                settle(coming, tb ^ 1, Set<0>{});
+            }
+            __syncthreads();
+        });
+    } while (++t < t_end);
+    outputs(sh.tile[(t_end - 1) & 1], 1, Set<1>{}, nothing);
+    PRODUCTS_READY();
+
+    auto put = [&](auto set, auto gated) INLINE {
+        constexpr int r = decltype(set)::value;
+        if (row_of(r) > last) return;
+        const float total = __builtin_ldexpf(__builtin_amdgcn_rcpf(both_sum(sum[r])), unit[r]);
+        const size_t at = row_at(r) + half * 4;
+        each<D / 32>([&](auto dims) INLINE {
+            constexpr int i = decltype(dims)::value;
+            HOLD();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const size_t d = at + i * 32 + j * 8;
+                f4 v = f4{kept(o[r][i][4 * j]), kept(o[r][i][4 * j + 1]), kept(o[r][i][4 * j + 2]), kept(o[r][i][4 * j + 3])} * total;
+                if constexpr (decltype(gated)::value) {
+                    const b4 g = *(const b4*)(a.gate + d);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[k] *= sigmoid((float)g[k]);
+                }
+                *(b4*)(a.out + d) = __builtin_convertvector(v, b4);
+            }
+        });
+    };
+    each<SETS>([&](auto set) INLINE {
+        if (a.gate) put(set, std::true_type{});
+        else put(set, std::false_type{});
+    });
 }
 
 }  // namespace
@@ -349,6 +677,8 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
         return fail(QH_EINVAL, "chunk_attn: q, gate and out must be 16-byte aligned");
     if (step->table_ld < 1 || step->table_ld > ((size_t)1 << 30) / kv->page)
         return fail(QH_EINVAL, "chunk_attn: tables of %zu pages of %d tokens (1 to 2^30 positions)", step->table_ld, kv->page);
+    if ((uint64_t)a.kv.slots / KV_TILE * 2 * kv->heads >= 0xffffffffu)  // (a tile's place is a 32-bit number)
+        return fail(QH_EINVAL, "chunk_attn: a cache of %zu pages of %d tokens of %d heads is too large", kv->pages, kv->page, kv->heads);
     const int group = q_heads / kv->heads;
     const uint64_t units = ((uint64_t)step->n * group / ROWS + step->n_seq) * kv->heads;  // as many as there can be
     if (units > 0x7fffffffu) return fail(QH_EINVAL, "chunk_attn: %zu tokens of %d heads are too many for one call", step->n, q_heads);

@@ -47,6 +47,17 @@ struct Args {
     TreeArrays t;
     const int32_t* table;  // [n_seq][table_ld]
     float scale;           // softmax scale * log2(e)
+    int32_t parts;         // workgroups that the work may be shared among in equal parts; 0: each has a unit
+    float* part;           // [2 parts][256 rows x D], as the lanes hold them, and of each row (maximum, sum, unit):
+    f4* part_rows;         // [2 parts][256]
+    struct Cut* cuts;      // [parts]
+};
+
+// Where a part begins within a unit, for join_kernel.
+struct Cut {
+    int32_t first_tile, tiles;  // the unit's, in the row of all (tiles 0: the part begins with a unit)
+    int32_t all, used;          // the tiles and parts in all
+    int32_t first, head, row0, last;
 };
 
 // Four codes as exact f16 operands: an int8 code c = q + 128 becomes 1024 + c by its bits, then q; e4m3 by its conversion.
@@ -74,6 +85,7 @@ __device__ __forceinline__ h4 operands(uint32_t a) {
 __device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void product(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void nothing_kept(f16& o, h8 zero) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(o) : "v"(zero)); }
 __device__ __forceinline__ float kept(float o) {
     float v;
     asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(o));
@@ -122,6 +134,13 @@ struct Plan {
 };
 constexpr int REST_DISORDER = 1, REST_SOME = 2;  // starts are not in order; some tokens are in no sequence that has work
 
+constexpr int MAX_UNITS = 2048;  // units of a call that may be shared in equal parts
+
+// A unit: 256 rows of a sequence's kv head, and the tiles that they see.
+struct Unit {
+    int b, first, old, head, row0, last, tiles;
+};
+
 // Fills the plan and returns the units in all. Starts that are not in order are found on the way; the plan is then made anew, each
 // sequence against all starts before it.
 __device__ __forceinline__ int make_plan(const Args& a, Plan& plan, int* rest_out) {
@@ -168,13 +187,61 @@ __device__ __forceinline__ int make_plan(const Args& a, Plan& plan, int* rest_ou
 }
 
 // The last sequence that begins at or before `at`, -1 for none (empty ones share their successor's beginning).
-__device__ __forceinline__ int find_seq(const int32_t* begin, int n_seq, int at) {
-    int lo = -1, hi = n_seq;
+__device__ __forceinline__ int find(const int32_t* begin, int n, int at) {
+    int lo = -1, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         (begin[mid] <= at ? lo : hi) = mid;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    return lo;
+}
+__device__ __forceinline__ int find_seq(const int32_t* begin, int n_seq, int at) {
+    return __builtin_amdgcn_readfirstlane(find(begin, n_seq, at));
+}
+
+// The u-th unit: a sequence's longest first, the heads in turn; or head by head, so that neighbours read the same cache.
+__device__ __forceinline__ Unit unit_at(const Args& a, const Plan& plan, int u, bool by_head) {
+    Unit v;
+    v.b = find(plan.base, a.t.n_seq, u);
+    v.first = plan.first[v.b];
+    v.old = a.t.len[v.b];
+    const int past = u - plan.base[v.b], rows = plan.news[v.b] * a.t.group, chunks = (rows + ROWS - 1) / ROWS;
+    v.head = by_head ? past / chunks : past % a.kv.heads;
+    v.row0 = (chunks - 1 - (by_head ? past % chunks : past / a.kv.heads)) * ROWS;
+    v.last = min(v.row0 + ROWS, rows) - 1;
+    v.tiles = (v.old + v.last / a.t.group + 1 + KV_TILE - 1) / KV_TILE;
+    return v;
+}
+
+// The tiles before each unit (in head order), and in all; the most of a unit.
+__device__ __forceinline__ int count_tiles(const Args& a, const Plan& plan, int units, int32_t* before, int32_t* sums, int* most_out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int all = 0, most = 0;
+#pragma unroll 1
+    for (int c = 0; c < units; c += THREADS) {
+        const int u = c + threadIdx.x;
+        const int tiles = u < units ? unit_at(a, plan, u, true).tiles : 0;
+        int run = tiles, top = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int left = __shfl_up(run, d);
+            run += lane >= d ? left : 0;
+            top = max(top, __shfl_xor(top, d));
+        }
+        if (lane == 63) sums[wave] = run, sums[WAVES + wave] = top;
+        __syncthreads();
+        int at = all + run - tiles;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            at += w < wave ? sums[w] : 0;
+            all += sums[w];
+            most = max(most, sums[WAVES + w]);
+        }
+        if (u < units) before[u] = at;
+        __syncthreads();
+    }
+    *most_out = __builtin_amdgcn_readfirstlane(most);
+    return __builtin_amdgcn_readfirstlane(all);
 }
 
 // The outputs of tokens that no sequence has work for, the grid's workgroups in turn: zeros for padding, else NaN.
@@ -205,7 +272,17 @@ struct Shared {
     Tile<D> tile[2];
     int32_t top_exp[WAVES];
     Plan plan;
+    int32_t tiles_before[MAX_UNITS];
 };
+
+// The rounds that unshared units take against equal parts, in tiles: equal parts cost the partial results' way through memory and a
+// second launch, about as much as JOIN_TILES.
+constexpr int JOIN_TILES = 12, PART_TILES = 4;  // (and no part is below PART_TILES)
+__device__ __forceinline__ bool share(int units, int all, int most, int parts) {
+    const int even = (all + parts - 1) / parts;
+    return (units <= parts ? most : max(most, even + most / 2)) > even + JOIN_TILES;
+}
+
 
 // A lane's row's softmax: the reference m that scores are taken against (in powers of two), and the sums of 2^(score - m). A score
 // may come to m + 15, since f16 holds that; m is set 7 below a largest score, so that probabilities keep f16's full bits down to 2^-21
@@ -219,18 +296,47 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     int rest;
     const int units = make_plan(a, sh.plan, &rest);
     if (rest) put_rest<D>(a, sh.plan, rest);
-    if ((int)blockIdx.x >= units) return;
-
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
-    const int b = find_seq(sh.plan.base, a.t.n_seq, blockIdx.x);
-    const int first = __builtin_amdgcn_readfirstlane(sh.plan.first[b]), news = __builtin_amdgcn_readfirstlane(sh.plan.news[b]);
-    const int old = a.t.len[b], group = a.t.group, rows = news * group, chunks = (rows + ROWS - 1) / ROWS;
-    // the longest first
-    const int past = blockIdx.x - __builtin_amdgcn_readfirstlane(sh.plan.base[b]);
-    const int head = past % a.kv.heads, row0 = (chunks - 1 - past / a.kv.heads) * ROWS;
-    const int last = min(row0 + ROWS, rows) - 1;  // the last row of the workgroup
-    const int all_see = old + row0 / group + 1;   // positions that all its rows see
-    const int t_end = (old + last / group + 1 + KV_TILE - 1) / KV_TILE;
+    // A unit each; or all tiles of all units in a row, in equal parts, consecutive ones on one XCD (workgroups b, b + 8, .. run on the same
+    // one), whose L2 then serves those that read the same head's cache.
+    int at = 0, hi = 1, all = 0, used = 0, part = 0;
+    bool shared = false;
+    if (a.parts) {
+        int most;
+        all = count_tiles(a, sh.plan, units, sh.tiles_before, sh.plan.sums[0], &most);
+        shared = all > 0 && share(units, all, most, a.parts);
+        used = shared ? min(a.parts, max(all / PART_TILES, 1)) : 0;
+        part = blockIdx.x;
+        if (part < used) {
+            const int xcd = part & 7, at_xcd = part >> 3;
+            part = xcd * (used >> 3) + min(xcd, used & 7) + at_xcd;
+        }
+        if (part < a.parts && part >= used && tid == 0) a.cuts[part] = Cut{};
+    }
+    if (shared) {
+        if (part >= used) return;
+        at = __builtin_amdgcn_readfirstlane(first_group(part, all, used));
+        hi = __builtin_amdgcn_readfirstlane(first_group(part + 1, all, used));
+        if (at >= hi) {
+            if (tid == 0) a.cuts[part] = Cut{};
+            return;
+        }
+    } else if ((int)blockIdx.x >= units) {
+        return;
+    }
+  do {
+    const int u = shared ? find_seq(sh.tiles_before, units, at) : (int)blockIdx.x;
+    const int unit_begin = shared ? __builtin_amdgcn_readfirstlane(sh.tiles_before[u]) : 0;
+    const Unit v = unit_at(a, sh.plan, u, shared);
+    const int b = __builtin_amdgcn_readfirstlane(v.b), first = __builtin_amdgcn_readfirstlane(v.first);
+    const int news = __builtin_amdgcn_readfirstlane(sh.plan.news[v.b]), old = __builtin_amdgcn_readfirstlane(v.old), group = a.t.group;
+    const int head = __builtin_amdgcn_readfirstlane(v.head), row0 = __builtin_amdgcn_readfirstlane(v.row0);
+    const int last = __builtin_amdgcn_readfirstlane(v.last), tiles = __builtin_amdgcn_readfirstlane(v.tiles);  // the last row
+    const int all_see = old + row0 / group + 1;  // positions that all its rows see
+    const int t_begin = shared ? at - unit_begin : 0, t_end = shared ? min(tiles, t_begin + hi - at) : tiles;
+    if (shared && at == first_group(part, all, used) && tid == 0)
+        a.cuts[part] = t_begin ? Cut{unit_begin, tiles, all, used, first, head, row0, last} : Cut{};
+    if (shared) __syncthreads();  // (the unit before is through with LDS)
 
     // the lane's row of a set, and its first query and output
     auto row_of = [&](int r) INLINE { return row0 + wave * (32 * SETS) + r * 32 + col; };
@@ -252,7 +358,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         places = (uint32_t)((page * a.kv.heads + head) * 2 * page_tiles + (mine & (page_tiles - 1)));
         if (page < 0 || ((int64_t)page << a.kv.page_shift) >= a.kv.slots) places = NONE;
     };
-    load_places(0);
+    load_places(t_begin);
 
     // a thread's pieces of a tile: 16 dimensions of a token's key, 16 tokens of a dimension of the values
     constexpr int PIECES = KV_TILE * D / 16 / THREADS;
@@ -267,8 +373,8 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(codes, at, (wave + i * WAVES) * 1024, 0));
     };
     auto load_keys = [&](int t) INLINE {
-        if (UNLIKELY((t & 63) == 0 && t)) load_places(t);
-        const uint32_t p = __builtin_amdgcn_readlane(places, t & 63);
+        if (UNLIKELY(((t - t_begin) & 63) == 0 && t > t_begin)) load_places(t);
+        const uint32_t p = __builtin_amdgcn_readlane(places, (t - t_begin) & 63);
         none = p == NONE;
         place = none ? 0 : p;
         const auto sc = rsrc(a.kv.scales + (size_t)place * KV_TILE, (page_tiles + 1) * KV_TILE * 4);
@@ -319,16 +425,22 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         constexpr int LOW = -1000;
         uint32_t top[SETS];  // bf16 with the sign taken off compares as a whole number; from 0x7f80 on it is not finite
         int e[SETS], most = LOW;
+        u4 raw_q[SETS][D / 16];
 #pragma unroll
         for (int r = 0; r < SETS; r++) {
-            top[r] = 0;
-            const size_t at = row_at(r);
+            const __bf16* const from = a.q + row_at(r) + half * 8;
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const u4 bits = *(const u4*)(a.q + at + i * 16 + half * 8);
+            for (int i = 0; i < D / 16; i++) raw_q[r][i] = *(const u4*)(from + i * 16);
+        }
+        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-                for (int k = 0; k < 4; k++) top[r] = max(top[r], max(bits[k] & 0x7fffu, bits[k] >> 16 & 0x7fffu));
-            }
+        for (int r = 0; r < SETS; r++) {
+            us2 largest = {0, 0};
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(us2, raw_q[r][i][k] & 0x7fff7fffu));
+            top[r] = max(largest.x, largest.y);
             const auto both = __builtin_amdgcn_permlane32_swap(top[r], top[r], false, false);
             top[r] = max(both[0], both[1]);
             e[r] = top[r] && top[r] < 0x7f80 ? __builtin_amdgcn_frexp_expf(__uint_as_float(top[r] << 16)) - 15 : LOW;
@@ -338,23 +450,27 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         for (int d = 1; d < 32; d <<= 1) most = max(most, __shfl_xor(most, d));
         if (lane == 0) sh.top_exp[wave] = most;
         __syncthreads();
+#pragma unroll
         for (int w = 0; w < WAVES; w++) most = max(most, sh.top_exp[w]);
         most = __builtin_amdgcn_readfirstlane(most == LOW ? 0 : most);
 #pragma unroll
         for (int r = 0; r < SETS; r++) wide |= __any(top[r] >= 0x7f80 || (top[r] && e[r] < most - 16));
-#pragma unroll
-        for (int r = 0; r < SETS; r++) {
+        each<SETS>([&](auto set) INLINE {
+            constexpr int r = decltype(set)::value;
             row_factor[r] = !wide ? 1.0f : top[r] >= 0x7f80 ? NAN : __builtin_ldexpf(1.0f, e[r] == LOW ? 0 : e[r] - most);
             const int by = wide && e[r] != LOW ? e[r] : most;
-            const size_t at = row_at(r);
+            each<D / 16>([&](auto at) INLINE {
+                constexpr int i = decltype(at)::value;
+                HOLD();
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const b8 in = *(const b8*)(a.q + at + i * 16 + half * 8);
-#pragma unroll
-                for (int k = 0; k < 8; k++) q[r][i][k] = (_Float16)__builtin_ldexpf((float)in[k], -by);
-                if (i % 4 == 3) HOLD();
-            }
-        }
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t two = raw_q[r][i][k];
+                    const h2 h = __builtin_convertvector((f2{__builtin_ldexpf(__uint_as_float(two << 16), -by),
+                                                             __builtin_ldexpf(__uint_as_float(two & 0xffff0000u), -by)}), h2);
+                    q[r][i][2 * k] = h.x, q[r][i][2 * k + 1] = h.y;
+                }
+            });
+        });
         key_factor = fmaxf(__builtin_ldexpf(a.scale, min(most, 40)), 1e-37f);
         late = __builtin_ldexpf(1.0f, max(most - 40, 0));
     }
@@ -389,10 +505,11 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     each<SETS>([&](auto set) INLINE {
         constexpr int r = decltype(set)::value;
         m[r] = -INFINITY, sum[r] = 0.0f, unit[r] = NO_EXP;
-        each<D / 32>([&](auto i) INLINE { each<16>([&](auto k) INLINE { o[r][i][k.value] = keep(0.0f); }); });
+        each<D / 32>([&](auto i) INLINE { nothing_kept(o[r][i], h8{}); });
     });
     auto scale_out = [&](auto set, float by) INLINE {
         constexpr int r = decltype(set)::value;
+        if (!__any(by != 1.0f)) return;
         HOLD();
         PRODUCTS_READY();
         each<D / 32>([&](auto i) INLINE {
@@ -459,7 +576,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         m[r] = none ? (most > -INFINITY ? up : m[r]) : m[r] + up;
         const float by = none ? 1.0f : __builtin_amdgcn_exp2f(-up * late);
         sum[r] *= by;
-        const float units = __builtin_ldexpf(by, unit[r] - to[r]);
+        const float units = none ? 1.0f : __builtin_ldexpf(by, unit[r] - to[r]);  // (none: there are no outputs yet)
         unit[r] = to[r];
         return units;
     };
@@ -540,15 +657,15 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     };
     const auto nothing = [](auto) INLINE {};
 
-    load_keys(0);
-    put_scales(sh.tile[0], 0);
+    load_keys(t_begin);
+    put_scales(sh.tile[t_begin & 1], t_begin);
 #pragma unroll
-    for (int i = 0; i < PIECES; i++) put_keys(sh.tile[0], i);
+    for (int i = 0; i < PIECES; i++) put_keys(sh.tile[t_begin & 1], i);
     load_values();
     __syncthreads();
-    load_factors(sh.tile[0]);
+    load_factors(sh.tile[t_begin & 1]);
 #pragma unroll
-    for (int i = 0; i < PIECES; i++) put_values(sh.tile[0], i, written(0));
+    for (int i = 0; i < PIECES; i++) put_values(sh.tile[t_begin & 1], i, written(t_begin));
     apart = apart_next, ref = ref_next;
     __syncthreads();
     // The second set's products with the values stand behind the next block's scores: the first set's softmax then has them beside it,
@@ -568,18 +685,18 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         each<16>([&](auto k) INLINE { relative(tile, tb, Set<0>{}, k); });
         mask(tile, t, tb, Set<0>{});
     };
-    scores(sh.tile[0], 0, nothing);
-    first_set(sh.tile[0], 0, 0);
+    scores(sh.tile[t_begin & 1], 0, nothing);
+    first_set(sh.tile[t_begin & 1], t_begin, 0);
     (void)follow(Set<0>{});
-    settle(sh.tile[0], 0, Set<0>{});
-    int t = 0;
+    settle(sh.tile[t_begin & 1], 0, Set<0>{});
+    int t = t_begin;
     do {  // (there is a tile at least; a loop that might not run would have its outputs in registers of their own)
         const Tile<D>& tile = sh.tile[t & 1];
         Tile<D>& next = sh.tile[(t + 1) & 1];
         const bool more = t + 1 < t_end;
         each<2>([&](auto block) INLINE {
             constexpr int tb = decltype(block)::value;
-            const Tile<D>& before = tb ? tile : sh.tile[(max(t, 1) - 1) & 1];
+            const Tile<D>& before = tb ? tile : sh.tile[(max(t, t_begin + 1) - 1) & 1];
             if (LIKELY(more)) {
                 if constexpr (tb == 0) load_keys(t + 1);
                 else load_values();
@@ -628,30 +745,100 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     PRODUCTS_READY();
 
     auto put = [&](auto set, auto gated) INLINE {
-        constexpr int r = decltype(set)::value;
-        if (row_of(r) > last) return;
+        constexpr int r = decltype(set)::value, N = D / 8;
         const float total = __builtin_ldexpf(__builtin_amdgcn_rcpf(both_sum(sum[r])), unit[r]);
         const size_t at = row_at(r) + half * 4;
-        each<D / 32>([&](auto dims) INLINE {
-            constexpr int i = decltype(dims)::value;
+        b4 g[N];  // (all at once: each is a trip to memory)
+        if constexpr (decltype(gated)::value)
+            each<N>([&](auto k) INLINE { g[k.value] = *(const b4*)(a.gate + at + k.value * 8); });
+        const bool there = row_of(r) <= last;
+        each<N>([&](auto piece) INLINE {
+            constexpr int k = decltype(piece)::value, i = k / 4, j = k % 4;
             HOLD();
+            f4 v = f4{kept(o[r][i][4 * j]), kept(o[r][i][4 * j + 1]), kept(o[r][i][4 * j + 2]), kept(o[r][i][4 * j + 3])} * total;
+            if constexpr (decltype(gated)::value) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const size_t d = at + i * 32 + j * 8;
-                f4 v = f4{kept(o[r][i][4 * j]), kept(o[r][i][4 * j + 1]), kept(o[r][i][4 * j + 2]), kept(o[r][i][4 * j + 3])} * total;
-                if constexpr (decltype(gated)::value) {
-                    const b4 g = *(const b4*)(a.gate + d);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] *= sigmoid((float)g[k]);
-                }
-                *(b4*)(a.out + d) = __builtin_convertvector(v, b4);
+                for (int n = 0; n < 4; n++) v[n] *= sigmoid((float)g[k][n]);
             }
+            if (there) *(b4*)(a.out + at + k * 8) = __builtin_convertvector(v, b4);
         });
     };
-    each<SETS>([&](auto set) INLINE {
-        if (a.gate) put(set, std::true_type{});
-        else put(set, std::false_type{});
-    });
+    if (t_begin == 0 && t_end == tiles) {
+        each<SETS>([&](auto set) INLINE {
+            if (a.gate) put(set, std::true_type{});
+            else put(set, std::false_type{});
+        });
+    } else {
+        const size_t slot = partial_slot(part, unit_begin, all, used);
+        f4* const rows = a.part_rows + slot * ROWS + wave * (32 * SETS) + col;
+        f4* const to = (f4*)a.part + slot * (ROWS * D / 4) + (size_t)wave * SETS * (D * 8) + lane;
+        each<SETS>([&](auto set) INLINE {
+            constexpr int r = decltype(set)::value;
+            const float total = both_sum(sum[r]);
+            if (half == 0) rows[r * 32] = f4{m[r], total, (float)unit[r], 0.0f};
+            each<D / 32>([&](auto dims) INLINE {
+                constexpr int i = decltype(dims)::value;
+                HOLD();
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    to[((r * (D / 32) + i) * 4 + j) * 64] = f4{kept(o[r][i][4 * j]), kept(o[r][i][4 * j + 1]), kept(o[r][i][4 * j + 2]), kept(o[r][i][4 * j + 3])};
+            });
+        });
+    }
+    at += t_end - t_begin;
+  } while (shared && at < hi);
+}
+
+// The partial results of a unit that several parts have: a workgroup for each 32 rows of it. The maxima's powers of two between the
+// parts and their units are joined; bound by the partial results' bytes.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+    const int part = blockIdx.x, set = blockIdx.y;
+    if (part == 0) return;
+    const Cut cut = a.cuts[part];
+    // the first part that begins within the unit joins it
+    if (cut.tiles == 0 || first_group(part - 1, cut.all, cut.used) > cut.first_tile) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    const int row = cut.row0 + set * 32 + col;
+    const int end = group_owner(cut.first_tile + cut.tiles - 1, cut.all, cut.used);
+    auto slot = [&](int w) { return (size_t)partial_slot(w, cut.first_tile, cut.all, cut.used); };
+    auto row_state = [&](int w) { return a.part_rows[slot(w) * ROWS + set * 32 + col]; };
+    float m = -INFINITY, units = NO_EXP, sum = 0.0f;
+    for (int w = part - 1; w <= end; w++) {
+        const f4 s = row_state(w);
+        m = fmaxf(m, s.x), units = fmaxf(units, s.z);
+    }
+    constexpr int PER_WAVE = D / 32 * 4 / 4;  // pieces of 8 dimensions that a wave has
+    f4 o[PER_WAVE];
+#pragma unroll
+    for (int k = 0; k < PER_WAVE; k++) o[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = part - 1; w <= end; w++) {
+        const f4 s = row_state(w);
+        const float by = s.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.x - m);
+        const float scale = __builtin_ldexpf(by, (int)(s.z - units));
+        sum += s.x == -INFINITY ? s.y : s.y * by;  // (a row that sees nothing of a part adds nothing, or that it is not finite)
+        const f4* const from = (const f4*)a.part + slot(w) * (ROWS * D / 4) + (size_t)(set / SETS) * SETS * (D * 8) + (set % SETS) * (D * 8) + lane;
+#pragma unroll
+        for (int k = 0; k < PER_WAVE; k++) {
+            const f4 v = from[(wave * PER_WAVE + k) * 64];
+            o[k] += s.x == -INFINITY ? f4{0.0f, 0.0f, 0.0f, 0.0f} : v * scale;
+        }
+    }
+    if (row > cut.last) return;
+    const float total = __builtin_ldexpf(__builtin_amdgcn_rcpf(sum), (int)units);
+    const int group = a.t.group, node = row / group;
+    const size_t at = ((size_t)(cut.first + node) * a.kv.heads * group + cut.head * group + (row - node * group)) * D + half * 4;
+#pragma unroll
+    for (int k = 0; k < PER_WAVE; k++) {
+        const size_t d = at + (wave * PER_WAVE + k) * 8;
+        f4 v = o[k] * total;
+        if (a.gate) {
+            const b4 g = *(const b4*)(a.gate + d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] *= sigmoid((float)g[i]);
+        }
+        *(b4*)(a.out + d) = __builtin_convertvector(v, b4);
+    }
 }
 
 }  // namespace
@@ -688,9 +875,21 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
                      group};
     a.table = step->table;
     a.scale = scale * 1.4426950408889634f;
+    // Work is shared in equal parts where units alone might leave compute units without: not where a table names few tiles, nor with many
+    // units. (Which it is to be the device decides, from the lengths.)
+    const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * (kv->head_dim == 64 ? 2 : 1);
+    const size_t slot = (size_t)ROWS * kv->head_dim * 4 + ROWS * sizeof(f4);
+    if (most > JOIN_TILES && units <= MAX_UNITS && units * most <= 0x7fffffff) {
+        a.parts = (int32_t)std::min<uint64_t>({wgs, TREE_MAX_WGS, (PF_SK_PART_BYTES - TREE_MAX_WGS * sizeof(Cut)) / (2 * slot)});
+        a.part = (float*)ctx_partials(ctx);
+        a.part_rows = (f4*)((uint8_t*)a.part + (size_t)2 * a.parts * ROWS * kv->head_dim * 4);
+        a.cuts = (Cut*)(a.part_rows + (size_t)2 * a.parts * ROWS);
+    }
     auto go = [&](auto d, auto fmt) {
         constexpr int D = decltype(d)::value;
-        launch_kernel(chunk_attn_kernel<D, decltype(fmt)::value>, dim3((unsigned)units), dim3(THREADS), (hipStream_t)stream, a);
+        launch_kernel(chunk_attn_kernel<D, decltype(fmt)::value>, dim3((unsigned)std::max<uint64_t>(units, a.parts)), dim3(THREADS),
+                      (hipStream_t)stream, a);
+        if (a.parts) launch_kernel(join_kernel<D>, dim3((unsigned)a.parts, ROWS / 32), dim3(256), (hipStream_t)stream, a);
     };
     auto of = [&](auto d) {
         if (kv->fmt == QH_KV_I8) go(d, std::integral_constant<int, QH_KV_I8>{});

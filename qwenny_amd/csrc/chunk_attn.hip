@@ -82,9 +82,9 @@ __device__ __forceinline__ h4 operands(uint32_t a) {
 // before it in the same registers needs no wait.
 #define OPERANDS_READY() asm volatile("s_nop 3")
 #define PRODUCTS_READY() asm volatile("s_nop 15\n\ts_nop 3")
-__device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b)); }
-__device__ __forceinline__ void product(f16& x, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b)); }
-__device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void product(f16& x, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void nothing_kept(f16& o, h8 zero) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(o) : "v"(zero)); }
 __device__ __forceinline__ float kept(float o) {
     float v;
@@ -533,9 +533,8 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     auto relative = [&](const Tile<D>& tile, int tb, auto set, auto at) INLINE {
         constexpr int r = decltype(set)::value, k = decltype(at)::value;
         if constexpr (k % 4 == 0 && k < 12) load_scales(tile, tb, Set<k / 4 + 1>{});
-        const float s = __builtin_fmaf(x[r][k], sc[k / 4 & 1][k & 3], m[r] == -INFINITY ? -0.0f : -m[r]);
-        x[r][k] = s;
-        mx[r] = k == 0 ? s : fmaxf(mx[r], s);
+        x[r][k] = __builtin_fmaf(x[r][k], sc[k / 4 & 1][k & 3], m[r] == -INFINITY ? -0.0f : -m[r]);
+        if constexpr (k % 2 == 1) mx[r] = fmaxf(fmaxf(k == 1 ? -INFINITY : mx[r], x[r][k - 1]), x[r][k]);
     };
     // then, in tiles taken apart, what a row does not see is left out; the units that the values have
     auto mask = [&](const Tile<D>& tile, int t, int tb, auto set) INLINE {
@@ -622,6 +621,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
             constexpr int i = decltype(at)::value;
             HOLD();
             if constexpr (i + DEEP - 1 < D / 16) f[(i + DEEP - 1) % DEEP] = key(i + DEEP - 1);
+            if constexpr (D == 64) asm volatile("s_nop 1");  // (a query may come from an accumulation register, right here)
 #pragma unroll
             for (int r = 0; r < SETS; r++) {
                 if constexpr (i == 0) product_first(x[r], f[0], q[r][0]);

@@ -80,11 +80,25 @@ __device__ __forceinline__ h4 operands(uint32_t a) {
 // does not know them, so what has to be waited for stands here: a register that a vector instruction wrote is read two steps later
 // (OPERANDS_READY), a product is read when it is through (PRODUCTS_READY: 8 passes and 4 steps; 20 are left). A product added to the one
 // before it in the same registers needs no wait.
-#define OPERANDS_READY() asm volatile("s_nop 3")
+#define OPERANDS_READY() asm volatile("s_nop 1")
 #define PRODUCTS_READY() asm volatile("s_nop 15\n\ts_nop 3")
-__device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b)); }
-__device__ __forceinline__ void product(f16& x, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b)); }
-__device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b)); }
+// (WAIT: where the compiler may fetch an operand from elsewhere right before. It does with D = 64, whose kernel has half the registers; a
+// test looks at what was built.)
+template <bool WAIT>
+__device__ __forceinline__ void product_first(f16& x, h8 a, h8 b) {
+    if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(x) : "v"(a), "v"(b));
+}
+template <bool WAIT>
+__device__ __forceinline__ void product(f16& x, h8 a, h8 b) {
+    if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(x) : "v"(a), "v"(b));
+}
+template <bool WAIT>
+__device__ __forceinline__ void product_kept(f16& o, h8 a, h8 b) {
+    if constexpr (WAIT) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(o) : "v"(a), "v"(b));
+}
 __device__ __forceinline__ void nothing_kept(f16& o, h8 zero) { asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(o) : "v"(zero)); }
 __device__ __forceinline__ float kept(float o) {
     float v;
@@ -271,6 +285,8 @@ template <int D>
 struct Shared {
     Tile<D> tile[2];
     int32_t top_exp[WAVES];
+    int32_t sees[ROWS];        // positions that a row sees
+    float row_factor[ROWS];
     Plan plan;
     int32_t tiles_before[MAX_UNITS];
 };
@@ -296,7 +312,15 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     int rest;
     const int units = make_plan(a, sh.plan, &rest);
     if (rest) put_rest<D>(a, sh.plan, rest);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (The lane is said anew in each block: what follows from it would otherwise be kept in registers over the blocks, and they run out.)
+    int lane = tid & 63;
+    auto col = [&]() INLINE { return lane & 31; };
+    auto half = [&]() INLINE { return lane >> 5; };
+    auto l16 = [&]() INLINE { return lane & 15; };
+    auto c4 = [&]() INLINE { return lane >> 4; };
+    auto g4 = [&]() INLINE { return (lane >> 4 & 1) * 2 + (lane >> 5); };
+    auto my_row = [&]() INLINE { return wave * (32 * SETS) + (lane & 31); };
     // A unit each; or all tiles of all units in a row, in equal parts, consecutive ones on one XCD (workgroups b, b + 8, .. run on the same
     // one), whose L2 then serves those that read the same head's cache.
     int at = 0, hi = 1, all = 0, used = 0, part = 0;
@@ -339,14 +363,14 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     if (shared) __syncthreads();  // (the unit before is through with LDS)
 
     // the lane's row of a set, and its first query and output
-    auto row_of = [&](int r) INLINE { return row0 + wave * (32 * SETS) + r * 32 + col; };
+    auto row_of = [&](int r) INLINE { return row0 + wave * (32 * SETS) + r * 32 + col(); };
     auto row_at = [&](int r) INLINE {
         const int row = min(row_of(r), last), node = row / group;
         return ((size_t)(first + node) * a.kv.heads * group + head * group + (row - node * group)) * D;
     };
-    int sees[SETS];
+    // (what only some tiles and waves need lies in LDS: registers run out)
 #pragma unroll
-    for (int r = 0; r < SETS; r++) sees[r] = old + min(row_of(r), last) / group + 1;
+    for (int r = 0; r < SETS; r++) sh.sees[my_row() + r * 32] = old + min(row_of(r), last) / group + 1;
 
     // where tiles lie, 64 at a time: lane l has the l-th's place in the cache (of its keys) in tiles
     constexpr uint32_t NONE = ~0u;
@@ -362,7 +386,6 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
 
     // a thread's pieces of a tile: 16 dimensions of a token's key, 16 tokens of a dimension of the values
     constexpr int PIECES = KV_TILE * D / 16 / THREADS;
-    const int l16 = lane & 15, c4 = lane >> 4, g4 = (c4 & 1) * 2 + (c4 >> 1);
     u4 raw[PIECES];
     float ks, vs;
     bool none;
@@ -382,15 +405,15 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sc, lane * 4, page_tiles * KV_TILE * 4, 0));
         const auto codes = rsrc(a.kv.codes + (size_t)place * (KV_TILE * D), KV_TILE * D);
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16 * 64 + c4 * 16, i);
+        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16() * 64 + c4() * 16, i);
     };
     auto load_values = [&]() INLINE {
         const auto codes = rsrc(a.kv.codes + ((size_t)place + page_tiles) * (KV_TILE * D), KV_TILE * D);
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16 * 64 + g4 * 16, i);
+        for (int i = 0; i < PIECES; i++) raw[i] = piece(codes, l16() * 64 + g4() * 16, i);
     };
     auto put_keys = [&](Tile<D>& to, int i) INLINE {
-        const int u = wave + i * WAVES, token = u / (D / 64) * 16 + l16, chunk = u % (D / 64) * 8 + c4 * 2;
+        const int u = wave + i * WAVES, token = u / (D / 64) * 16 + l16(), chunk = u % (D / 64) * 8 + c4() * 2;
         const h4 k0 = operands<FMT>(raw[i].x), k1 = operands<FMT>(raw[i].y), k2 = operands<FMT>(raw[i].z), k3 = operands<FMT>(raw[i].w);
         to.k[chunk][token] = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
         to.k[chunk + 1][token] = __builtin_shufflevector(k2, k3, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -398,19 +421,19 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     h4 factor[4];  // of the thread's tokens
     auto load_factors = [&](const Tile<D>& to) INLINE {
 #pragma unroll
-        for (int s = 0; s < 4; s++) factor[s] = *(const h4*)&to.factor[s * 16 + g4 * 4];
+        for (int s = 0; s < 4; s++) factor[s] = *(const h4*)&to.factor[s * 16 + g4() * 4];
     };
     auto put_values = [&](Tile<D>& to, int i, int there) INLINE {
-        const int dim = (wave + i * WAVES) * 16 + l16;
+        const int dim = (wave + i * WAVES) * 16 + l16();
         if (FMT == QH_KV_E4M3 && UNLIKELY(there < KV_TILE)) {  // what was not written may be NaN codes, which no probability takes away
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const int keep = max(there - (s * 16 + g4 * 4), 0);
+                const int keep = max(there - (s * 16 + g4() * 4), 0);
                 raw[i][s] = keep < 4 ? raw[i][s] & ((1u << 8 * keep) - 1) : raw[i][s];
             }
         }
 #pragma unroll
-        for (int s = 0; s < 4; s++) ((h4*)&to.v[s][g4 & 1][dim])[g4 >> 1] = operands<FMT>(raw[i][s]) * factor[s];
+        for (int s = 0; s < 4; s++) ((h4*)&to.v[s][g4() & 1][dim])[g4() >> 1] = operands<FMT>(raw[i][s]) * factor[s];
     };
 
     // the lane's queries: dimensions 16 i + 8 half .. + 7, scaled by a power of two into f16's range. One power for the workgroup, that goes
@@ -419,7 +442,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     // Where queries reach 2^55, the rest of the power is left to the differences of scores (`late`): the scores themselves might be
     // infinite. All tiles are then taken apart.
     h8 q[SETS][D / 16];
-    float key_factor, row_factor[SETS], late;
+    float key_factor, late;
     bool wide = false;
     {
         constexpr int LOW = -1000;
@@ -428,7 +451,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         u4 raw_q[SETS][D / 16];
 #pragma unroll
         for (int r = 0; r < SETS; r++) {
-            const __bf16* const from = a.q + row_at(r) + half * 8;
+            const __bf16* const from = a.q + row_at(r) + half() * 8;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) raw_q[r][i] = *(const u4*)(from + i * 16);
         }
@@ -457,7 +480,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         for (int r = 0; r < SETS; r++) wide |= __any(top[r] >= 0x7f80 || (top[r] && e[r] < most - 16));
         each<SETS>([&](auto set) INLINE {
             constexpr int r = decltype(set)::value;
-            row_factor[r] = !wide ? 1.0f : top[r] >= 0x7f80 ? NAN : __builtin_ldexpf(1.0f, e[r] == LOW ? 0 : e[r] - most);
+            sh.row_factor[my_row() + r * 32] = top[r] >= 0x7f80 ? NAN : __builtin_ldexpf(1.0f, e[r] == LOW ? 0 : e[r] - most);
             const int by = wide && e[r] != LOW ? e[r] : most;
             each<D / 16>([&](auto at) INLINE {
                 constexpr int i = decltype(at)::value;
@@ -471,8 +494,9 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
                 }
             });
         });
-        key_factor = fmaxf(__builtin_ldexpf(a.scale, min(most, 40)), 1e-37f);
-        late = __builtin_ldexpf(1.0f, max(most - 40, 0));
+        auto alike = [&](float v) INLINE { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); };
+        key_factor = alike(fmaxf(__builtin_ldexpf(a.scale, min(most, 40)), 1e-37f));
+        late = alike(__builtin_ldexpf(1.0f, max(most - 40, 0)));
     }
 
     // Values are multiplied by their scales as they become operands, relative to 2^ref, the largest scale so far: for tiles that all rows
@@ -525,28 +549,25 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     float mx[SETS];
     int to[SETS];  // the units that the values then have
     // A set's scores relative to m (as yet none: as they are), in 16 steps that may go on beside products.
-    f4 sc[2];
-    auto load_scales = [&](const Tile<D>& tile, int tb, auto at) INLINE {
-        constexpr int j = decltype(at)::value;
-        sc[j & 1] = *(const f4*)&tile.key_scale[tb * 32 + j * 8 + half * 4];
-    };
+    f4 sc[2];  // the block's keys' scales, four tokens' and the next ones'; behind the first set's last, its first again
+    auto load_scale = [&](const Tile<D>& tile, int tb, int j) INLINE { sc[j & 1] = *(const f4*)&tile.key_scale[tb * 32 + j * 8 + half() * 4]; };
     auto relative = [&](const Tile<D>& tile, int tb, auto set, auto at) INLINE {
         constexpr int r = decltype(set)::value, k = decltype(at)::value;
-        if constexpr (k % 4 == 0 && k < 12) load_scales(tile, tb, Set<k / 4 + 1>{});
         x[r][k] = __builtin_fmaf(x[r][k], sc[k / 4 & 1][k & 3], m[r] == -INFINITY ? -0.0f : -m[r]);
         if constexpr (k % 2 == 1) mx[r] = fmaxf(fmaxf(k == 1 ? -INFINITY : mx[r], x[r][k - 1]), x[r][k]);
+        if constexpr (k % 4 == 3 && (r == 0 || k < 8)) load_scale(tile, tb, (k / 4 + 2) % 4);
     };
     // then, in tiles taken apart, what a row does not see is left out; the units that the values have
     auto mask = [&](const Tile<D>& tile, int t, int tb, auto set) INLINE {
         constexpr int r = decltype(set)::value;
         to[r] = ref - VALUE_EXP;
         if (LIKELY(!apart)) return;
-        const int t0 = t * KV_TILE + tb * 32 + half * 4, behind = (t + 1) * KV_TILE <= all_see ? 0x7fffffff : sees[r];
+        const int t0 = t * KV_TILE + tb * 32 + half() * 4, behind = (t + 1) * KV_TILE <= all_see ? 0x7fffffff : sh.sees[my_row() + r * 32];
         float largest = 0.0f;
         mx[r] = -INFINITY;
         each<4>([&](auto at) INLINE {
             constexpr int j = decltype(at)::value;
-            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half * 4];
+            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half() * 4];
             HOLD();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -585,7 +606,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         if (LIKELY(!apart)) return;
         each<4>([&](auto at) INLINE {
             constexpr int j = decltype(at)::value;
-            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half * 4];
+            const f4 sv = *(const f4*)&tile.value_scale[tb * 32 + j * 8 + half() * 4];
             HOLD();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -610,22 +631,25 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         }
     };
 
-    constexpr int DEEP = 4;  // operands under way
+    // Operands are asked for DEEP - 1 products ahead of theirs, over the borders of what follows one another: `ahead(k)` has the k-th of what comes
+    // after.
+    constexpr int DEEP = 4;
+    static_assert(D / 16 % DEEP == 0);
+    h8 f[DEEP];
+    auto key = [&](const Tile<D>& tile, int tb, int i) INLINE { return tile.k[2 * i + half()][tb * 32 + col()]; };
+    auto value = [&](const Tile<D>& tile, int tb, int n) INLINE { return tile.v[tb * 2 + n / (D / 32)][half()][n % (D / 32) * 32 + col()]; };
     // s^T = k q^T of 32 tokens, with `beside(i)` beside the products of 16 dimensions
-    auto scores = [&](const Tile<D>& tile, int tb, auto&& beside) INLINE {
-        h8 f[DEEP];
-        auto key = [&](int i) INLINE { return tile.k[2 * i + half][tb * 32 + col]; };
-#pragma unroll
-        for (int k = 0; k < DEEP - 1; k++) f[k] = key(k);
+    auto scores = [&](const Tile<D>& tile, int tb, auto&& beside, auto&& ahead) INLINE {
         each<D / 16>([&](auto at) INLINE {
-            constexpr int i = decltype(at)::value;
+            constexpr int i = decltype(at)::value, to = (i + DEEP - 1) % DEEP;
             HOLD();
-            if constexpr (i + DEEP - 1 < D / 16) f[(i + DEEP - 1) % DEEP] = key(i + DEEP - 1);
-            if constexpr (D == 64) asm volatile("s_nop 1");  // (a query may come from an accumulation register, right here)
+            if constexpr (i + DEEP - 1 < D / 16) f[to] = key(tile, tb, i + DEEP - 1);
+            else f[to] = ahead(i + DEEP - 1 - D / 16);
+            if constexpr (i >= D / 16 - 2) load_scale(tile, tb, i - D / 16 + 2);
 #pragma unroll
             for (int r = 0; r < SETS; r++) {
-                if constexpr (i == 0) product_first(x[r], f[0], q[r][0]);
-                else product(x[r], f[i % DEEP], q[r][i]);
+                if constexpr (i == 0) product_first<D == 64>(x[r], f[0], q[r][0]);
+                else product<D == 64>(x[r], f[i % DEEP], q[r][i]);
             }
             beside(at);
         });
@@ -633,19 +657,16 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     };
     // o^T += v^T p^T of a set: the lane has its row's dimensions 32 i + 8 (k / 4) + 4 half + k % 4
     constexpr int PRODUCTS = D / 32 * 2;  // of 32 dimensions, then of 16 tokens
-    auto outputs = [&](const Tile<D>& tile, int tb, auto set, auto&& beside) INLINE {
+    auto outputs = [&](const Tile<D>& tile, int tb, auto set, auto&& beside, auto&& ahead) INLINE {
         constexpr int r = decltype(set)::value;
-        h8 f[DEEP];
-        auto value = [&](int n) INLINE { return tile.v[tb * 2 + n / (D / 32)][half][n % (D / 32) * 32 + col]; };
-#pragma unroll
-        for (int k = 0; k < DEEP - 1; k++) f[k] = value(k);
         HOLD();
         OPERANDS_READY();
         each<PRODUCTS>([&](auto at) INLINE {
-            constexpr int n = decltype(at)::value;
+            constexpr int n = decltype(at)::value, to = (n + DEEP - 1) % DEEP;
             HOLD();
-            if constexpr (n + DEEP - 1 < PRODUCTS) f[(n + DEEP - 1) % DEEP] = value(n + DEEP - 1);
-            product_kept(o[r][n % (D / 32)], f[n % DEEP], p[r][n / (D / 32)]);
+            if constexpr (n + DEEP - 1 < PRODUCTS) f[to] = value(tile, tb, n + DEEP - 1);
+            else f[to] = ahead(n + DEEP - 1 - PRODUCTS);
+            product_kept<D == 64>(o[r][n % (D / 32)], f[n % DEEP], p[r][n / (D / 32)]);
             beside(at);
         });
         HOLD();
@@ -675,17 +696,18 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     auto widen = [&]() INLINE {
         if (UNLIKELY(wide)) {
 #pragma unroll
-            for (int k = 0; k < 16; k++) x[0][k] *= row_factor[0], x[1][k] *= row_factor[1];
+            for (int k = 0; k < 16; k++) x[0][k] *= sh.row_factor[my_row()], x[1][k] *= sh.row_factor[my_row() + 32];
         }
     };
     auto first_set = [&](const Tile<D>& tile, int t, int tb) INLINE {
         PRODUCTS_READY();
         widen();
-        load_scales(tile, tb, Set<0>{});
         each<16>([&](auto k) INLINE { relative(tile, tb, Set<0>{}, k); });
         mask(tile, t, tb, Set<0>{});
     };
-    scores(sh.tile[t_begin & 1], 0, nothing);
+#pragma unroll
+    for (int k = 0; k < DEEP - 1; k++) f[k] = key(sh.tile[t_begin & 1], 0, k);
+    scores(sh.tile[t_begin & 1], 0, nothing, [&](int k) INLINE { return value(sh.tile[t_begin & 1], 1, k); });
     first_set(sh.tile[t_begin & 1], t_begin, 0);
     (void)follow(Set<0>{});
     settle(sh.tile[t_begin & 1], 0, Set<0>{});
@@ -696,25 +718,27 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         const bool more = t + 1 < t_end;
         each<2>([&](auto block) INLINE {
             constexpr int tb = decltype(block)::value;
+            asm volatile("" : "+v"(lane));
             const Tile<D>& before = tb ? tile : sh.tile[(max(t, t_begin + 1) - 1) & 1];
             if (LIKELY(more)) {
                 if constexpr (tb == 0) load_keys(t + 1);
                 else load_values();
             }
             ones = apart ? h2{(_Float16)0.0f, (_Float16)0.0f} : h2{(_Float16)1.0f, (_Float16)1.0f};
-            load_scales(tile, tb, Set<0>{});
             outputs(before, tb ^ 1, Set<1>{}, [&](auto at) INLINE {
                 spread(at, [&](auto k) INLINE {
                     soft(Set<0>{}, k);
                     relative(tile, tb, Set<1>{}, k);
                 });
-            });
+            }, [&](int k) INLINE { return value(tile, tb, k); });
             mask(tile, t, tb, Set<1>{});
             if (UNLIKELY(moved(Set<1>{}))) scale_out(Set<1>{}, follow(Set<1>{}));
             settle(tile, tb, Set<1>{});
-            outputs(tile, tb, Set<0>{}, [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<1>{}, k); }); });
+            // (behind the last tile's last block there are no scores: what is asked for then is the tile's again, and not used)
+            const Tile<D>& coming = tb == 0 ? tile : next;
+            outputs(tile, tb, Set<0>{}, [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<1>{}, k); }); },
+                    [&](int k) INLINE { return key(coming, tb ^ 1, k); });
             if (tb == 0 || LIKELY(more)) {
-                const Tile<D>& coming = tb == 0 ? tile : next;
                 // the next tile's operands beside the scores, late enough for its codes to be there
                 scores(coming, tb ^ 1, [&](auto at) INLINE {
                     constexpr int i = decltype(at)::value - D / 32;
@@ -732,7 +756,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
                             put_values(next, i / 2, written(t + 1));
                         }
                     }
-                });
+                }, [&](int k) INLINE { return value(tile, tb, k); });
                 if constexpr (tb == 1) apart = apart_next, ref = ref_next;
                 first_set(coming, t + tb, tb ^ 1);
                 if (UNLIKELY(moved(Set<0>{}))) scale_out(Set<0>{}, follow(Set<0>{}));
@@ -741,13 +765,15 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
             __syncthreads();
         });
     } while (++t < t_end);
-    outputs(sh.tile[(t_end - 1) & 1], 1, Set<1>{}, nothing);
+#pragma unroll
+    for (int k = 0; k < DEEP - 1; k++) f[k] = value(sh.tile[(t_end - 1) & 1], 1, k);
+    outputs(sh.tile[(t_end - 1) & 1], 1, Set<1>{}, nothing, [&](int) INLINE { return f[0]; });
     PRODUCTS_READY();
 
     auto put = [&](auto set, auto gated) INLINE {
         constexpr int r = decltype(set)::value, N = D / 8;
         const float total = __builtin_ldexpf(__builtin_amdgcn_rcpf(both_sum(sum[r])), unit[r]);
-        const size_t at = row_at(r) + half * 4;
+        const size_t at = row_at(r) + half() * 4;
         b4 g[N];  // (all at once: each is a trip to memory)
         if constexpr (decltype(gated)::value)
             each<N>([&](auto k) INLINE { g[k.value] = *(const b4*)(a.gate + at + k.value * 8); });
@@ -770,12 +796,12 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         });
     } else {
         const size_t slot = partial_slot(part, unit_begin, all, used);
-        f4* const rows = a.part_rows + slot * ROWS + wave * (32 * SETS) + col;
+        f4* const rows = a.part_rows + slot * ROWS + wave * (32 * SETS) + col();
         f4* const to = (f4*)a.part + slot * (ROWS * D / 4) + (size_t)wave * SETS * (D * 8) + lane;
         each<SETS>([&](auto set) INLINE {
             constexpr int r = decltype(set)::value;
             const float total = both_sum(sum[r]);
-            if (half == 0) rows[r * 32] = f4{m[r], total, (float)unit[r], 0.0f};
+            if (half() == 0) rows[r * 32] = f4{m[r], total, (float)unit[r], 0.0f};
             each<D / 32>([&](auto dims) INLINE {
                 constexpr int i = decltype(dims)::value;
                 HOLD();

@@ -37,7 +37,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int BUF_RSRC_WORD3 = 0x00020000;  // buffer resource word 3: 32-bit data format, no swizzle
 
-constexpr int WAVES = 4, THREADS = 64 * WAVES, SETS = 2, ROWS = 32 * SETS * WAVES;  // a wave has sets of 32 rows
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
+constexpr int rows_of(int sets) { return 32 * sets * WAVES; }  // of a workgroup whose waves have so many sets of 32 rows
 
 struct Args {
     const __bf16* q;     // [n][heads][D]
@@ -157,6 +158,7 @@ struct Unit {
 
 // Fills the plan and returns the units in all. Starts that are not in order are found on the way; the plan is then made anew, each
 // sequence against all starts before it.
+template <int ROWS>
 __device__ __forceinline__ int make_plan(const Args& a, Plan& plan, int* rest_out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (bool in_order = true;; in_order = false) {
@@ -214,6 +216,7 @@ __device__ __forceinline__ int find_seq(const int32_t* begin, int n_seq, int at)
 }
 
 // The u-th unit: a sequence's longest first, the heads in turn; or head by head, so that neighbours read the same cache.
+template <int ROWS>
 __device__ __forceinline__ Unit unit_at(const Args& a, const Plan& plan, int u, bool by_head) {
     Unit v;
     v.b = find(plan.base, a.t.n_seq, u);
@@ -228,13 +231,14 @@ __device__ __forceinline__ Unit unit_at(const Args& a, const Plan& plan, int u, 
 }
 
 // The tiles before each unit (in head order), and in all; the most of a unit.
+template <int ROWS>
 __device__ __forceinline__ int count_tiles(const Args& a, const Plan& plan, int units, int32_t* before, int32_t* sums, int* most_out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int all = 0, most = 0;
 #pragma unroll 1
     for (int c = 0; c < units; c += THREADS) {
         const int u = c + threadIdx.x;
-        const int tiles = u < units ? unit_at(a, plan, u, true).tiles : 0;
+        const int tiles = u < units ? unit_at<ROWS>(a, plan, u, true).tiles : 0;
         int run = tiles, top = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -281,7 +285,7 @@ struct Tile {
     float value_scale[KV_TILE];
     _Float16 factor[KV_TILE];    // what the values were multiplied by
 };
-template <int D>
+template <int D, int ROWS>
 struct Shared {
     Tile<D> tile[2];
     int32_t top_exp[WAVES];
@@ -293,7 +297,8 @@ struct Shared {
 
 // The rounds that unshared units take against equal parts, in tiles: equal parts cost the partial results' way through memory and a
 // second launch, about as much as JOIN_TILES.
-constexpr int JOIN_TILES = 12, PART_TILES = 4;  // (and no part is below PART_TILES)
+constexpr int SHORT_TILES = 80;
+constexpr int JOIN_TILES = 25, PART_TILES = 4;  // (and no part is below PART_TILES)
 __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
     const int even = (all + parts - 1) / parts;
     return (units <= parts ? most : max(most, even + most / 2)) > even + JOIN_TILES;
@@ -306,11 +311,13 @@ __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
 constexpr float ROOM = 15.0f, BELOW = 7.0f;
 constexpr int VALUE_EXP = 7;  // values are taken relative to 2^-7 of the largest scale, for the same reason
 
-template <int D, int FMT>
+template <int D, int FMT, int SETS>
 __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(const Args a) {
-    __shared__ Shared<D> sh;
+    constexpr int ROWS = rows_of(SETS);
+    constexpr bool WAIT = D == 64;
+    __shared__ Shared<D, ROWS> sh;
     int rest;
-    const int units = make_plan(a, sh.plan, &rest);
+    const int units = make_plan<ROWS>(a, sh.plan, &rest);
     if (rest) put_rest<D>(a, sh.plan, rest);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // (The lane is said anew in each block: what follows from it would otherwise be kept in registers over the blocks, and they run out.)
@@ -325,9 +332,9 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     // one), whose L2 then serves those that read the same head's cache.
     int at = 0, hi = 1, all = 0, used = 0, part = 0;
     bool shared = false;
-    if (a.parts) {
+    if (SETS == 2 && a.parts) {
         int most;
-        all = count_tiles(a, sh.plan, units, sh.tiles_before, sh.plan.sums[0], &most);
+        all = count_tiles<ROWS>(a, sh.plan, units, sh.tiles_before, sh.plan.sums[0], &most);
         shared = all > 0 && share(units, all, most, a.parts);
         used = shared ? min(a.parts, max(all / PART_TILES, 1)) : 0;
         part = blockIdx.x;
@@ -351,7 +358,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
   do {
     const int u = shared ? find_seq(sh.tiles_before, units, at) : (int)blockIdx.x;
     const int unit_begin = shared ? __builtin_amdgcn_readfirstlane(sh.tiles_before[u]) : 0;
-    const Unit v = unit_at(a, sh.plan, u, shared);
+    const Unit v = unit_at<ROWS>(a, sh.plan, u, shared);
     const int b = __builtin_amdgcn_readfirstlane(v.b), first = __builtin_amdgcn_readfirstlane(v.first);
     const int news = __builtin_amdgcn_readfirstlane(sh.plan.news[v.b]), old = __builtin_amdgcn_readfirstlane(v.old), group = a.t.group;
     const int head = __builtin_amdgcn_readfirstlane(v.head), row0 = __builtin_amdgcn_readfirstlane(v.row0);
@@ -545,7 +552,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     };
 
     f16 x[SETS];    // scores of 32 tokens: the lane has its rows' of tokens 8 (i / 4) + 4 half + i % 4
-    h8 p[SETS][2];  // their probabilities, as operands
+    h8 p[2][2];     // their probabilities, as operands: of each set; or with one set, of a block and of the one before
     float mx[SETS];
     int to[SETS];  // the units that the values then have
     // A set's scores relative to m (as yet none: as they are), in 16 steps that may go on beside products.
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         constexpr int r = decltype(set)::value, k = decltype(at)::value;
         x[r][k] = __builtin_fmaf(x[r][k], sc[k / 4 & 1][k & 3], m[r] == -INFINITY ? -0.0f : -m[r]);
         if constexpr (k % 2 == 1) mx[r] = fmaxf(fmaxf(k == 1 ? -INFINITY : mx[r], x[r][k - 1]), x[r][k]);
-        if constexpr (k % 4 == 3 && (r == 0 || k < 8)) load_scale(tile, tb, (k / 4 + 2) % 4);
+        if constexpr (k % 4 == 3 && (r + 1 < SETS || k < 8)) load_scale(tile, tb, (k / 4 + 2) % 4);
     };
     // then, in tiles taken apart, what a row does not see is left out; the units that the values have
     auto mask = [&](const Tile<D>& tile, int t, int tb, auto set) INLINE {
@@ -619,15 +626,15 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     // The probabilities of a set's scores, in 16 steps beside products. (Sums are of the probabilities as they are multiplied.)
     h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
     float even;
-    auto soft = [&](auto set, auto at) INLINE {
-        constexpr int r = decltype(set)::value, k = decltype(at)::value;
+    auto soft = [&](auto set, auto at, auto to) INLINE {
+        constexpr int r = decltype(set)::value, k = decltype(at)::value, q = decltype(to)::value;
         const float pr = __builtin_amdgcn_exp2f(x[r][k]);
         if constexpr (k % 2 == 0) {
             even = pr;
         } else {
             const h2 pp = __builtin_convertvector((f2{even, pr}), h2);
             sum[r] = __builtin_amdgcn_fdot2(pp, ones, sum[r], false);
-            p[r][k >> 3][(k & 7) - 1] = pp.x, p[r][k >> 3][k & 7] = pp.y;
+            p[q][k >> 3][(k & 7) - 1] = pp.x, p[q][k >> 3][k & 7] = pp.y;
         }
     };
 
@@ -648,8 +655,8 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
             if constexpr (i >= D / 16 - 2) load_scale(tile, tb, i - D / 16 + 2);
 #pragma unroll
             for (int r = 0; r < SETS; r++) {
-                if constexpr (i == 0) product_first<D == 64>(x[r], f[0], q[r][0]);
-                else product<D == 64>(x[r], f[i % DEEP], q[r][i]);
+                if constexpr (i == 0) product_first<WAIT>(x[r], f[0], q[r][0]);
+                else product<WAIT>(x[r], f[i % DEEP], q[r][i]);
             }
             beside(at);
         });
@@ -657,8 +664,8 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     };
     // o^T += v^T p^T of a set: the lane has its row's dimensions 32 i + 8 (k / 4) + 4 half + k % 4
     constexpr int PRODUCTS = D / 32 * 2;  // of 32 dimensions, then of 16 tokens
-    auto outputs = [&](const Tile<D>& tile, int tb, auto set, auto&& beside, auto&& ahead) INLINE {
-        constexpr int r = decltype(set)::value;
+    auto outputs = [&](const Tile<D>& tile, int tb, auto set, auto from, auto&& beside, auto&& ahead) INLINE {
+        constexpr int r = decltype(set)::value, q = decltype(from)::value;
         HOLD();
         OPERANDS_READY();
         each<PRODUCTS>([&](auto at) INLINE {
@@ -666,7 +673,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
             HOLD();
             if constexpr (n + DEEP - 1 < PRODUCTS) f[to] = value(tile, tb, n + DEEP - 1);
             else f[to] = ahead(n + DEEP - 1 - PRODUCTS);
-            product_kept<D == 64>(o[r][n % (D / 32)], f[n % DEEP], p[r][n / (D / 32)]);
+            product_kept<WAIT>(o[r][n % (D / 32)], f[n % DEEP], p[q][n / (D / 32)]);
             beside(at);
         });
         HOLD();
@@ -690,13 +697,16 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     apart = apart_next, ref = ref_next;
     __syncthreads();
     // The second set's products with the values stand behind the next block's scores: the first set's softmax then has them beside it,
-    // and the second set's the first set's products. To begin with, probabilities of nothing.
+    // and the second set's the first set's products. One set alone stands behind as a whole, its softmax beside the block before's products.
+    // To begin with, probabilities of nothing.
 #pragma unroll
     for (int k = 0; k < 8; k++) p[1][0][k] = p[1][1][k] = (_Float16)0.0f;
     auto widen = [&]() INLINE {
         if (UNLIKELY(wide)) {
 #pragma unroll
-            for (int k = 0; k < 16; k++) x[0][k] *= sh.row_factor[my_row()], x[1][k] *= sh.row_factor[my_row() + 32];
+            for (int r = 0; r < SETS; r++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) x[r][k] *= sh.row_factor[my_row() + r * 32];
         }
     };
     auto first_set = [&](const Tile<D>& tile, int t, int tb) INLINE {
@@ -725,19 +735,25 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
                 else load_values();
             }
             ones = apart ? h2{(_Float16)0.0f, (_Float16)0.0f} : h2{(_Float16)1.0f, (_Float16)1.0f};
-            outputs(before, tb ^ 1, Set<1>{}, [&](auto at) INLINE {
-                spread(at, [&](auto k) INLINE {
-                    soft(Set<0>{}, k);
-                    relative(tile, tb, Set<1>{}, k);
-                });
-            }, [&](int k) INLINE { return value(tile, tb, k); });
-            mask(tile, t, tb, Set<1>{});
-            if (UNLIKELY(moved(Set<1>{}))) scale_out(Set<1>{}, follow(Set<1>{}));
-            settle(tile, tb, Set<1>{});
             // (behind the last tile's last block there are no scores: what is asked for then is the tile's again, and not used)
             const Tile<D>& coming = tb == 0 ? tile : next;
-            outputs(tile, tb, Set<0>{}, [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<1>{}, k); }); },
-                    [&](int k) INLINE { return key(coming, tb ^ 1, k); });
+            auto coming_key = [&](int k) INLINE { return key(coming, tb ^ 1, k); };
+            if constexpr (SETS == 1) {
+                outputs(before, tb ^ 1, Set<0>{}, Set<(tb ^ 1)>{},
+                        [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<0>{}, k, Set<tb>{}); }); }, coming_key);
+            } else {
+                outputs(before, tb ^ 1, Set<1>{}, Set<1>{}, [&](auto at) INLINE {
+                    spread(at, [&](auto k) INLINE {
+                        soft(Set<0>{}, k, Set<0>{});
+                        relative(tile, tb, Set<1>{}, k);
+                    });
+                }, [&](int k) INLINE { return value(tile, tb, k); });
+                mask(tile, t, tb, Set<1>{});
+                if (UNLIKELY(moved(Set<1>{}))) scale_out(Set<1>{}, follow(Set<1>{}));
+                settle(tile, tb, Set<1>{});
+                outputs(tile, tb, Set<0>{}, Set<0>{},
+                        [&](auto at) INLINE { spread(at, [&](auto k) INLINE { soft(Set<1>{}, k, Set<1>{}); }); }, coming_key);
+            }
             if (tb == 0 || LIKELY(more)) {
                 // the next tile's operands beside the scores, late enough for its codes to be there
                 scores(coming, tb ^ 1, [&](auto at) INLINE {
@@ -759,7 +775,14 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
                 }, [&](int k) INLINE { return value(tile, tb, k); });
                 if constexpr (tb == 1) apart = apart_next, ref = ref_next;
                 first_set(coming, t + tb, tb ^ 1);
-                if (UNLIKELY(moved(Set<0>{}))) scale_out(Set<0>{}, follow(Set<0>{}));
+                if (UNLIKELY(moved(Set<0>{}))) {
+                    const float by = follow(Set<0>{});
+                    scale_out(Set<0>{}, by);
+                    if constexpr (SETS == 1) {  // what stands behind, too
+#pragma unroll
+                        for (int k = 0; k < 16; k++) p[tb][k >> 3][k & 7] = (_Float16)((float)p[tb][k >> 3][k & 7] * by);
+                    }
+                }
                 settle(coming, tb ^ 1, Set<0>{});
             }
             __syncthreads();
@@ -767,7 +790,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     } while (++t < t_end);
 #pragma unroll
     for (int k = 0; k < DEEP - 1; k++) f[k] = value(sh.tile[(t_end - 1) & 1], 1, k);
-    outputs(sh.tile[(t_end - 1) & 1], 1, Set<1>{}, nothing, [&](int) INLINE { return f[0]; });
+    outputs(sh.tile[(t_end - 1) & 1], 1, Set<SETS - 1>{}, Set<1>{}, nothing, [&](int) INLINE { return f[0]; });
     PRODUCTS_READY();
 
     auto put = [&](auto set, auto gated) INLINE {
@@ -819,6 +842,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
 // parts and their units are joined; bound by the partial results' bytes.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
+    constexpr int SETS = 2, ROWS = rows_of(SETS);
     const int part = blockIdx.x, set = blockIdx.y;
     if (part == 0) return;
     const Cut cut = a.cuts[part];
@@ -893,29 +917,32 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
     if ((uint64_t)a.kv.slots / KV_TILE * 2 * kv->heads >= 0xffffffffu)  // (a tile's place is a 32-bit number)
         return fail(QH_EINVAL, "chunk_attn: a cache of %zu pages of %d tokens of %d heads is too large", kv->pages, kv->page, kv->heads);
     const int group = q_heads / kv->heads;
-    const uint64_t units = ((uint64_t)step->n * group / ROWS + step->n_seq) * kv->heads;  // as many as there can be
-    if (units > 0x7fffffffu) return fail(QH_EINVAL, "chunk_attn: %zu tokens of %d heads are too many for one call", step->n, q_heads);
+    auto units_of = [&](int sets) { return ((uint64_t)step->n * group / rows_of(sets) + step->n_seq) * kv->heads; };  // as many as there can be
+    if (units_of(1) > 0x7fffffffu) return fail(QH_EINVAL, "chunk_attn: %zu tokens of %d heads are too many for one call", step->n, q_heads);
     if (!ctx) return fail(QH_EINVAL, "chunk_attn: null context");
     a.q = (const __bf16*)q, a.gate = (const __bf16*)gate, a.out = (__bf16*)out;
     a.t = TreeArrays{step->start, step->len, (int64_t)step->table_ld, a.kv.page_shift, (int)step->n, step->n_seq, step->max_new,
                      group};
     a.table = step->table;
     a.scale = scale * 1.4426950408889634f;
+    const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * (kv->head_dim == 64 ? 2 : 1);
+    // Units of 128 rows where there are less than two of 256 for each workgroup that runs at once, and none is long
+    const int sets = most <= SHORT_TILES && units_of(2) < 2 * wgs ? 1 : 2;
+    const uint64_t units = units_of(sets);
     // Work is shared in equal parts where units alone might leave compute units without: not where a table names few tiles, nor with many
     // units. (Which it is to be the device decides, from the lengths.)
-    const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * (kv->head_dim == 64 ? 2 : 1);
-    const size_t slot = (size_t)ROWS * kv->head_dim * 4 + ROWS * sizeof(f4);
-    if (most > JOIN_TILES && units <= MAX_UNITS && units * most <= 0x7fffffff) {
+    const size_t rows = rows_of(2), slot = rows * kv->head_dim * 4 + rows * sizeof(f4);
+    if (sets == 2 && most > JOIN_TILES && units <= MAX_UNITS && units * most <= 0x7fffffff) {
         a.parts = (int32_t)std::min<uint64_t>({wgs, TREE_MAX_WGS, (PF_SK_PART_BYTES - TREE_MAX_WGS * sizeof(Cut)) / (2 * slot)});
         a.part = (float*)ctx_partials(ctx);
-        a.part_rows = (f4*)((uint8_t*)a.part + (size_t)2 * a.parts * ROWS * kv->head_dim * 4);
-        a.cuts = (Cut*)(a.part_rows + (size_t)2 * a.parts * ROWS);
+        a.part_rows = (f4*)((uint8_t*)a.part + 2 * a.parts * rows * kv->head_dim * 4);
+        a.cuts = (Cut*)(a.part_rows + 2 * a.parts * rows);
     }
     auto go = [&](auto d, auto fmt) {
-        constexpr int D = decltype(d)::value;
-        launch_kernel(chunk_attn_kernel<D, decltype(fmt)::value>, dim3((unsigned)std::max<uint64_t>(units, a.parts)), dim3(THREADS),
-                      (hipStream_t)stream, a);
-        if (a.parts) launch_kernel(join_kernel<D>, dim3((unsigned)a.parts, ROWS / 32), dim3(256), (hipStream_t)stream, a);
+        constexpr int D = decltype(d)::value, FMT = decltype(fmt)::value;
+        launch_kernel(sets == 1 ? chunk_attn_kernel<D, FMT, 1> : chunk_attn_kernel<D, FMT, 2>, dim3((unsigned)std::max<uint64_t>(units, a.parts)),
+                      dim3(THREADS), (hipStream_t)stream, a);
+        if (a.parts) launch_kernel(join_kernel<D>, dim3((unsigned)a.parts, (unsigned)rows / 32), dim3(256), (hipStream_t)stream, a);
     };
     auto of = [&](auto d) {
         if (kv->fmt == QH_KV_I8) go(d, std::integral_constant<int, QH_KV_I8>{});

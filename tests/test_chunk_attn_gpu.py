@@ -41,10 +41,11 @@ class Chunk(Step):
                 ds = np.where(late, 0, np.abs(q[mine, head]) @ np.abs(k).T * scale * (self.d + 8) * 2.0**-24).max(-1, keepdims=True)
                 ds += np.where(late, 0, top - s).max(-1, keepdims=True) * 2.0**-22
                 seen = a + np.arange(m)[:, None] + 1
-                # a probability times its value's scale is rounded to f16: 2^-11 of it, or half of f16's smallest step relative to the
-                # largest scale that the row sees (the reference is at most twice that)
+                # a probability is rounded to f16, and so are a value's scale and the value: 2^-11 of it each (where a row does not see all of
+                # a tile, only the probability times the scale is); or half of f16's smallest step relative to the largest scale that
+                # the row sees (the reference is at most twice that)
                 small = seen * 2.0**-25 * 2 * np.where(late, 0, vs).max(-1, keepdims=True) * TOP[self.kv.fmt] / l
-                tol[mine, head] = (2.0**-11 + 4 * ds + (seen + 64) * 2.0**-23) * (p @ np.abs(v) / l) + small
+                tol[mine, head] = (3 * 2.0**-11 + 4 * ds + (seen + 64) * 2.0**-23) * (p @ np.abs(v) / l) + small
         if self.gate is not None:
             sig = 1 / (1 + np.exp(-_f64(self.gate)))
             out, tol = out * sig, tol * sig + np.abs(out * sig) * 2.0**-20
@@ -57,39 +58,55 @@ class Chunk(Step):
         assert (off[rows] <= 0).all(), off[rows].max()
 
 
+class Wide(Chunk):
+    """The same with tables of far more positions than the sequences have: units of twice the rows, shared in parts where that is
+    worth it."""
+
+    def step(self, max_new=None):
+        if self.table.shape[1] * self.kv.page < 90 * 64:
+            more = -(-90 * 64 // self.kv.page) - self.table.shape[1]
+            self.table = np.concatenate((self.table, np.full((len(self.seqs), more), -7, np.int32)), 1)
+        return super().step(max_new)
+
+
+FORMS = pytest.mark.parametrize("form", [Chunk, Wide])
 SHORT = [[(0, 1)], [(0, 2)], [(0, 31)], [(0, 32)], [(0, 33)], [(0, 64)], [(0, 65)], [(1, 64)], [(63, 1)], [(63, 2)], [(64, 130)], [(100, 257)],
          [(1000, 43)], [(511, 86)]]
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", list(KvFmt))
 @pytest.mark.parametrize("seqs", SHORT, ids=str)
-def test_short_lengths(gemm, fmt, seqs):
+def test_short_lengths(gemm, form, fmt, seqs):
     print(f"chunk {fmt!r} {seqs}", flush=True)
-    Chunk(seqs, fmt, 6, 1, 256, 64, gate=True).check(gemm)
+    form(seqs, fmt, 6, 1, 256, 64, gate=True).check(gemm)
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", list(KvFmt))
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("h,j,page", [(1, 1, 64), (4, 4, 128), (16, 4, 256), (7, 1, 1024), (17, 1, 64), (64, 1, 64)])
-def test_head_layouts(gemm, fmt, d, h, j, page):
+def test_head_layouts(gemm, form, fmt, d, h, j, page):
     print(f"chunk {fmt!r} {h}/{j}x{d} page {page}", flush=True)
-    Chunk([(300, 70), (0, 3)], fmt, h, j, d, page, seed=h).check(gemm)
+    form([(300, 70), (0, 3)], fmt, h, j, d, page, seed=h).check(gemm)
 
 
 RAGGED = [(50, 100), (0, 0), (4, 1), (0, 200), (129, 64), (3, 0), (700, 31), (2000, 1), (63, 65)]
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", list(KvFmt))
 @pytest.mark.parametrize("d,h,j", [(256, 24, 4), (128, 8, 8), (64, 4, 1)])
-def test_ragged_batches(gemm, fmt, d, h, j):
+def test_ragged_batches(gemm, form, fmt, d, h, j):
     print(f"chunks {fmt!r} {h}/{j}x{d}", flush=True)
-    Chunk(RAGGED, fmt, h, j, d, 128).check(gemm)
+    form(RAGGED, fmt, h, j, d, 128).check(gemm)
 
 
-def test_many_sequences(gemm):
+@FORMS
+def test_many_sequences(gemm, form):
     """As many sequences as a step takes: the plan's last places."""
     print("1024 sequences", flush=True)
-    Chunk([(b % 70, b % 3 if b % 100 else 80) for b in range(1024)], KvFmt.I8, 2, 1, 64, 64).check(gemm)
+    form([(b % 70, b % 3 if b % 100 else 80) for b in range(1024)], KvFmt.I8, 2, 1, 64, 64).check(gemm)
 
 
 @pytest.mark.parametrize("fmt,seqs,h,j,d", [(KvFmt.I8, [(20001, 66)], 6, 1, 256), (KvFmt.E4M3, [(9000, 90)], 12, 2, 128),
@@ -101,11 +118,12 @@ def test_long_caches(gemm, fmt, seqs, h, j, d):
     assert torch.equal(s.run(gemm), s.run(gemm))
 
 
+@FORMS
 @pytest.mark.parametrize("scale", [1.0, 1e-4, 30.0])
 @pytest.mark.parametrize("fmt", list(KvFmt))
-def test_scales(gemm, fmt, scale):
+def test_scales(gemm, form, fmt, scale):
     """A flat softmax, and one so peaked that all but one probability vanish."""
-    Chunk([(700, 70)], fmt, 4, 2, 128, 64).check(gemm, scale=scale)
+    form([(700, 70)], fmt, 4, 2, 128, 64).check(gemm, scale=scale)
 
 
 def test_max_new_above_what_is_there(gemm):
@@ -113,12 +131,13 @@ def test_max_new_above_what_is_there(gemm):
     s.check(gemm, step=s.step(5000))
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", list(KvFmt))
 @pytest.mark.parametrize("d", [64, 256])
 @pytest.mark.parametrize("rising", [True, False])
-def test_values_of_very_different_size(gemm, fmt, d, rising):
+def test_values_of_very_different_size(gemm, form, fmt, d, rising):
     """Over 2^100 from the first position to the last and back: what a row sees later is taken relative to a larger scale."""
-    s = Chunk([(500, 200), (0, 70)], fmt, 4, 2, d, 64, gate=True)
+    s = form([(500, 200), (0, 70)], fmt, 4, 2, d, 64, gate=True)
     for slots in s.slots:
         at = np.arange(len(slots)) / len(slots)
         size = 2.0 ** (100 * (at if rising else 1 - at) - 60)
@@ -128,13 +147,14 @@ def test_values_of_very_different_size(gemm, fmt, d, rising):
     s.check(gemm)
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", list(KvFmt))
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3e38])
 @pytest.mark.parametrize("which", [0, 1])
-def test_what_a_row_does_not_see(gemm, fmt, bad, which):
+def test_what_a_row_does_not_see(gemm, form, fmt, bad, which):
     """A later token's key or value that is not finite, or huge, and what lies behind the sequence's end, take nothing from a row
     before it; rows from it on have it."""
-    s = Chunk([(100, 90), (0, 70)], fmt, 4, 2, 128, 64)
+    s = form([(100, 90), (0, 70)], fmt, 4, 2, 128, 64)
     out, tol = s.want()
     at = 140  # a token of the first sequence: its 40th new one
     for head in range(2):  # the last entry is what follows the sequence
@@ -153,8 +173,9 @@ def test_what_a_row_does_not_see(gemm, fmt, bad, which):
         s.check_rows(got, np.r_[0:160])
 
 
-def test_queries_that_are_not_finite(gemm):
-    s = Chunk([(100, 90)], KvFmt.I8, 4, 2, 128, 64)
+@FORMS
+def test_queries_that_are_not_finite(gemm, form):
+    s = form([(100, 90)], KvFmt.I8, 4, 2, 128, 64)
     s.q[3, 1, 7] = float("nan")
     s.q[70, 2, 100] = float("inf")
     s.q[5, 0] = 0.0
@@ -168,8 +189,9 @@ def test_queries_that_are_not_finite(gemm):
     assert (off <= 0).all(), off.max()
 
 
-def test_pages_outside_the_cache(gemm):
-    s = Chunk([(100, 90), (200, 70)], KvFmt.E4M3, 4, 2, 128, 64)
+@FORMS
+def test_pages_outside_the_cache(gemm, form):
+    s = form([(100, 90), (200, 70)], KvFmt.E4M3, 4, 2, 128, 64)
     out, tol = s.want()
     for page in (-1, s.kv.pages, 2**31 - 1):
         s.table[0, 2] = page  # positions 128 to 191: tokens from the 28th on
@@ -186,10 +208,11 @@ STARTS = [([0, 70, 73, 173], 100, "==="), ([0, 70, 70, 170], 200, "=N"), ([0, 70
           ([0, 70, 73, 173], 60, "n=n"), ([0, 99, 73, 173], 100, None), ([-HUGE - 1, HUGE, -1, HUGE], 100, "nnn")]
 
 
+@FORMS
 @pytest.mark.parametrize("start,max_new,kinds", STARTS, ids=str)
-def test_starts(gemm, start, max_new, kinds):
+def test_starts(gemm, form, start, max_new, kinds):
     print(f"starts {start} up to {max_new}", flush=True)
-    s = Chunk([(100, 70), (300, 3), (40, 100)], KvFmt.I8, 4, 2, 128, 64, gate=True)
+    s = form([(100, 70), (300, 3), (40, 100)], KvFmt.I8, 4, 2, 128, 64, gate=True)
     out, tol = s.want()
     s.start = np.array(start, np.int64).astype(np.int32)
     got = s.run(gemm, step=s.step(max_new))
@@ -209,9 +232,10 @@ def test_starts(gemm, start, max_new, kinds):
             assert (np.abs(_f64(got)[rows] - out[rows]) <= tol[rows]).all()
 
 
+@FORMS
 @pytest.mark.parametrize("old", [-1, -HUGE, HUGE, None])
-def test_lengths_past_the_table(gemm, old):
-    s = Chunk([(300, 70), (900, 66), (64, 0), (700, 80)], KvFmt.I8, 6, 1, 64, 64)
+def test_lengths_past_the_table(gemm, form, old):
+    s = form([(300, 70), (900, 66), (64, 0), (700, 80)], KvFmt.I8, 6, 1, 64, 64)
     out, tol = s.want()
     s.len[1] = s.table.shape[1] * 64 - 65 if old is None else old
     s.len[2] = old or 0
@@ -233,9 +257,10 @@ def test_padding_and_strides_of_tables(gemm):
     s.check_rows(got[:n], np.r_[0:n])
 
 
-def test_agrees_with_tree_attn(gemm):
+@FORMS
+def test_agrees_with_tree_attn(gemm, form):
     """Chains of up to 64 tokens by either operator, each within its bound."""
-    s = Chunk([(100, 64), (2000, 1), (0, 30)], KvFmt.I8, 24, 4, 256, 256, gate=True)
+    s = form([(100, 64), (2000, 1), (0, 30)], KvFmt.I8, 24, 4, 256, 256, gate=True)
     a, b = s.run(gemm), Step.run(s, gemm)
     out, tol = s.want()
     for got in (a, b):
@@ -263,10 +288,12 @@ class FarChunk(Chunk):
             self.kv, self.slots = whole, slots
 
 
+@FORMS
 @pytest.mark.parametrize("seqs", [[(100, 70)], [(3000, 130), (0, 66), (50, 1)]], ids=str)
-def test_graphs(gemm, seqs):
+def test_graphs(gemm, form, seqs):
     """A captured call follows the lengths and tables from replay to replay; two graphs share the context's scratch."""
-    s = Chunk(seqs, KvFmt.I8, 6, 2, 128, 64, gate=True)
+    s = form(seqs, KvFmt.I8, 6, 2, 128, 64, gate=True)
+    s.step()  # (the form's tables)
     lens = _dev(s.len)
     step = TreeStep(s.n, _dev(s.start), lens, _dev(s.table), max(m for _, m in seqs))
     out = [torch.zeros((s.n, s.h, s.d), dtype=torch.bfloat16, device="cuda") for _ in range(2)]

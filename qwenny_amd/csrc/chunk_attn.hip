@@ -56,8 +56,8 @@ struct Args {
 
 // Where a part begins within a unit, for join_kernel.
 struct Cut {
-    int32_t first_tile, tiles;  // the unit's, in the row of all (tiles 0: the part begins with a unit)
-    int32_t all, used;          // the tiles and parts in all
+    int32_t begin, end;  // the unit's, in the row of all (end 0: the part begins with a unit, or another before it joins this one)
+    int32_t all, used;   // the row's length, and its parts
     int32_t first, head, row0, last;
 };
 
@@ -230,7 +230,12 @@ __device__ __forceinline__ Unit unit_at(const Args& a, const Plan& plan, int u, 
     return v;
 }
 
-// The tiles before each unit (in head order), and in all; the most of a unit.
+// What a unit takes beside its tiles, in tiles: queries in, outputs out, the first tile's way (24 x 256 in units of 128 rows: 14 us and
+// 3.1 a tile).
+constexpr int UNIT_TILES = 6;
+__device__ __forceinline__ int length(const Unit& v) { return v.tiles + UNIT_TILES; }
+
+// The lengths before each unit (in head order), and in all; the most of a unit.
 template <int ROWS>
 __device__ __forceinline__ int count_tiles(const Args& a, const Plan& plan, int units, int32_t* before, int32_t* sums, int* most_out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -238,7 +243,7 @@ __device__ __forceinline__ int count_tiles(const Args& a, const Plan& plan, int 
 #pragma unroll 1
     for (int c = 0; c < units; c += THREADS) {
         const int u = c + threadIdx.x;
-        const int tiles = u < units ? unit_at<ROWS>(a, plan, u, true).tiles : 0;
+        const int tiles = u < units ? length(unit_at<ROWS>(a, plan, u, true)) : 0;
         int run = tiles, top = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -311,10 +316,13 @@ __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
 constexpr float ROOM = 15.0f, BELOW = 7.0f;
 constexpr int VALUE_EXP = 7;  // values are taken relative to 2^-7 of the largest scale, for the same reason
 
+// Waves of a SIMD: what the registers (and LDS) leave room for.
+constexpr int waves_of(int d) { return d == 64 ? 2 : 1; }
+
 template <int D, int FMT, int SETS>
-__global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(const Args a) {
+__global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const Args a) {
     constexpr int ROWS = rows_of(SETS);
-    constexpr bool WAIT = D == 64;
+    constexpr bool WAIT = waves_of(D) > 1;
     __shared__ Shared<D, ROWS> sh;
     int rest;
     const int units = make_plan<ROWS>(a, sh.plan, &rest);
@@ -332,7 +340,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     // one), whose L2 then serves those that read the same head's cache.
     int at = 0, hi = 1, all = 0, used = 0, part = 0;
     bool shared = false;
-    if (SETS == 2 && a.parts) {
+    if (a.parts) {
         int most;
         all = count_tiles<ROWS>(a, sh.plan, units, sh.tiles_before, sh.plan.sums[0], &most);
         shared = all > 0 && share(units, all, most, a.parts);
@@ -344,10 +352,17 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
         }
         if (part < a.parts && part >= used && tid == 0) a.cuts[part] = Cut{};
     }
+    // where a part begins: not within what a unit takes beside its tiles, but with the unit
+    auto begin_of = [&](int w) INLINE {
+        const int begin = first_group(w, all, used);
+        if (begin >= all) return all;
+        const int unit = sh.tiles_before[find_seq(sh.tiles_before, units, begin)];
+        return __builtin_amdgcn_readfirstlane(begin - unit <= UNIT_TILES ? unit : begin);  // (a tile at least before it)
+    };
     if (shared) {
         if (part >= used) return;
-        at = __builtin_amdgcn_readfirstlane(first_group(part, all, used));
-        hi = __builtin_amdgcn_readfirstlane(first_group(part + 1, all, used));
+        at = begin_of(part);
+        hi = begin_of(part + 1);
         if (at >= hi) {
             if (tid == 0) a.cuts[part] = Cut{};
             return;
@@ -364,9 +379,12 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
     const int head = __builtin_amdgcn_readfirstlane(v.head), row0 = __builtin_amdgcn_readfirstlane(v.row0);
     const int last = __builtin_amdgcn_readfirstlane(v.last), tiles = __builtin_amdgcn_readfirstlane(v.tiles);  // the last row
     const int all_see = old + row0 / group + 1;  // positions that all its rows see
-    const int t_begin = shared ? at - unit_begin : 0, t_end = shared ? min(tiles, t_begin + hi - at) : tiles;
-    if (shared && at == first_group(part, all, used) && tid == 0)
-        a.cuts[part] = t_begin ? Cut{unit_begin, tiles, all, used, first, head, row0, last} : Cut{};
+    const int t_begin = shared ? max(at - unit_begin - UNIT_TILES, 0) : 0;
+    const int t_end = shared ? min(tiles, hi - unit_begin - UNIT_TILES) : tiles;
+    if (shared && at == begin_of(part)) {  // the first part that begins within a unit has it joined
+        const bool joins = t_begin && begin_of(part - 1) <= unit_begin;
+        if (tid == 0) a.cuts[part] = joins ? Cut{unit_begin, unit_begin + length(v), all, used, first, head, row0, last} : Cut{};
+    }
     if (shared) __syncthreads();  // (the unit before is through with LDS)
 
     // the lane's row of a set, and its first query and output
@@ -834,44 +852,54 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void chunk_attn_kernel(co
             });
         });
     }
-    at += t_end - t_begin;
+    at = unit_begin + UNIT_TILES + t_end;
   } while (shared && at < hi);
 }
 
-// The partial results of a unit that several parts have: a workgroup for each 32 rows of it. The maxima's powers of two between the
-// parts and their units are joined; bound by the partial results' bytes.
-template <int D>
+// The partial results of a unit that several parts have: a workgroup for 32 rows of it and 64 dimensions. The maxima's powers of two and
+// the units of the parts are joined; four parts' results are under way at once. Bound by their bytes.
+template <int D, int SETS>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
-    constexpr int SETS = 2, ROWS = rows_of(SETS);
+    constexpr int ROWS = rows_of(SETS), AHEAD = 4, PIECES = 2;  // pieces of 8 dimensions that a wave has
     const int part = blockIdx.x, set = blockIdx.y;
     if (part == 0) return;
     const Cut cut = a.cuts[part];
-    // the first part that begins within the unit joins it
-    if (cut.tiles == 0 || first_group(part - 1, cut.all, cut.used) > cut.first_tile) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    if (cut.end == 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5, piece = (blockIdx.z * 4 + wave) * PIECES;
     const int row = cut.row0 + set * 32 + col;
-    const int end = group_owner(cut.first_tile + cut.tiles - 1, cut.all, cut.used);
-    auto slot = [&](int w) { return (size_t)partial_slot(w, cut.first_tile, cut.all, cut.used); };
+    const int end = group_owner(cut.end - 1, cut.all, cut.used);
+    auto slot = [&](int w) { return (size_t)partial_slot(w, cut.begin, cut.all, cut.used); };
     auto row_state = [&](int w) { return a.part_rows[slot(w) * ROWS + set * 32 + col]; };
     float m = -INFINITY, units = NO_EXP, sum = 0.0f;
-    for (int w = part - 1; w <= end; w++) {
-        const f4 s = row_state(w);
-        m = fmaxf(m, s.x), units = fmaxf(units, s.z);
+    for (int w0 = part - 1; w0 <= end; w0 += AHEAD) {
+        f4 s[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) s[k] = row_state(min(w0 + k, end));
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) m = fmaxf(m, s[k].x), units = fmaxf(units, s[k].z);
     }
-    constexpr int PER_WAVE = D / 32 * 4 / 4;  // pieces of 8 dimensions that a wave has
-    f4 o[PER_WAVE];
+    f4 o[PIECES];
 #pragma unroll
-    for (int k = 0; k < PER_WAVE; k++) o[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = part - 1; w <= end; w++) {
-        const f4 s = row_state(w);
-        const float by = s.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.x - m);
-        const float scale = __builtin_ldexpf(by, (int)(s.z - units));
-        sum += s.x == -INFINITY ? s.y : s.y * by;  // (a row that sees nothing of a part adds nothing, or that it is not finite)
-        const f4* const from = (const f4*)a.part + slot(w) * (ROWS * D / 4) + (size_t)(set / SETS) * SETS * (D * 8) + (set % SETS) * (D * 8) + lane;
+    for (int i = 0; i < PIECES; i++) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w0 = part - 1; w0 <= end; w0 += AHEAD) {
+        f4 s[AHEAD], v[AHEAD][PIECES];
 #pragma unroll
-        for (int k = 0; k < PER_WAVE; k++) {
-            const f4 v = from[(wave * PER_WAVE + k) * 64];
-            o[k] += s.x == -INFINITY ? f4{0.0f, 0.0f, 0.0f, 0.0f} : v * scale;
+        for (int k = 0; k < AHEAD; k++) {
+            const int w = min(w0 + k, end);
+            s[k] = row_state(w);
+            const f4* const from = (const f4*)a.part + slot(w) * (ROWS * D / 4) + (size_t)set * (D * 8) + lane;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) v[k][i] = from[(piece + i) * 64];
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            if (w0 + k > end) break;
+            const bool none = s[k].x == -INFINITY;  // (a row that sees nothing of a part adds nothing, or that it is not finite)
+            const float by = none ? 0.0f : __builtin_amdgcn_exp2f(s[k].x - m);
+            sum += none ? s[k].y : s[k].y * by;
+            const float scale = __builtin_ldexpf(by, (int)(s[k].z - units));
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) o[i] += none ? f4{0.0f, 0.0f, 0.0f, 0.0f} : v[k][i] * scale;
         }
     }
     if (row > cut.last) return;
@@ -879,13 +907,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     const int group = a.t.group, node = row / group;
     const size_t at = ((size_t)(cut.first + node) * a.kv.heads * group + cut.head * group + (row - node * group)) * D + half * 4;
 #pragma unroll
-    for (int k = 0; k < PER_WAVE; k++) {
-        const size_t d = at + (wave * PER_WAVE + k) * 8;
-        f4 v = o[k] * total;
+    for (int i = 0; i < PIECES; i++) {
+        const size_t d = at + (piece + i) * 8;
+        f4 v = o[i] * total;
         if (a.gate) {
             const b4 g = *(const b4*)(a.gate + d);
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] *= sigmoid((float)g[i]);
+            for (int n = 0; n < 4; n++) v[n] *= sigmoid((float)g[n]);
         }
         *(b4*)(a.out + d) = __builtin_convertvector(v, b4);
     }
@@ -925,14 +953,15 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
                      group};
     a.table = step->table;
     a.scale = scale * 1.4426950408889634f;
-    const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * (kv->head_dim == 64 ? 2 : 1);
+    const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * waves_of(kv->head_dim);
     // Units of 128 rows where there are less than two of 256 for each workgroup that runs at once, and none is long
     const int sets = most <= SHORT_TILES && units_of(2) < 2 * wgs ? 1 : 2;
     const uint64_t units = units_of(sets);
     // Work is shared in equal parts where units alone might leave compute units without: not where a table names few tiles, nor with many
     // units. (Which it is to be the device decides, from the lengths.)
-    const size_t rows = rows_of(2), slot = rows * kv->head_dim * 4 + rows * sizeof(f4);
-    if (sets == 2 && most > JOIN_TILES && units <= MAX_UNITS && units * most <= 0x7fffffff) {
+    const uint64_t longest = most + UNIT_TILES;
+    const size_t rows = rows_of(sets), slot = rows * kv->head_dim * 4 + rows * sizeof(f4);
+    if (most > JOIN_TILES && units <= MAX_UNITS && units * longest <= 0x7fffffff) {
         a.parts = (int32_t)std::min<uint64_t>({wgs, TREE_MAX_WGS, (PF_SK_PART_BYTES - TREE_MAX_WGS * sizeof(Cut)) / (2 * slot)});
         a.part = (float*)ctx_partials(ctx);
         a.part_rows = (f4*)((uint8_t*)a.part + 2 * a.parts * rows * kv->head_dim * 4);
@@ -942,7 +971,7 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
         constexpr int D = decltype(d)::value, FMT = decltype(fmt)::value;
         launch_kernel(sets == 1 ? chunk_attn_kernel<D, FMT, 1> : chunk_attn_kernel<D, FMT, 2>, dim3((unsigned)std::max<uint64_t>(units, a.parts)),
                       dim3(THREADS), (hipStream_t)stream, a);
-        if (a.parts) launch_kernel(join_kernel<D>, dim3((unsigned)a.parts, (unsigned)rows / 32), dim3(256), (hipStream_t)stream, a);
+        if (a.parts) launch_kernel(sets == 1 ? join_kernel<D, 1> : join_kernel<D, 2>, dim3((unsigned)a.parts, (unsigned)rows / 32, D / 64), dim3(256), (hipStream_t)stream, a);
     };
     auto of = [&](auto d) {
         if (kv->fmt == QH_KV_I8) go(d, std::integral_constant<int, QH_KV_I8>{});

@@ -78,6 +78,26 @@ __device__ __forceinline__ double exp2_64(double t) {
     return __builtin_ldexp(p, (int)fmax(n, -2000.0));
 }
 
+// The same where there are many: 2^(n / 64) by a table of 64 in LDS, the rest |x| <= ln 2 / 128 by four terms (what is left is below 4e-14).
+// 13 operations instead of 21: the logits' own reading is then as long.
+struct Table {
+    double pow2[64];
+};
+__device__ __forceinline__ void fill(Table& table) {
+    if (threadIdx.x < 64) table.pow2[threadIdx.x] = exp2_64((double)threadIdx.x / 64.0 - 1.0) * 2.0;
+}
+__device__ __forceinline__ double exp2_64(const Table& table, double t64) {  // of t64 / 64
+    constexpr double C = 0.69314718055994530942 / 64;
+    const double n = __builtin_rint(t64), f = t64 - n;
+    const int i = max((int)n, -200000);
+    double p = C * C * C * C / 24;
+    p = fma(p, f, C * C * C / 6);
+    p = fma(p, f, C * C / 2);
+    p = fma(p, f, C);
+    p = fma(p, f, 1.0);
+    return __builtin_ldexp(p * table.pow2[i & 63], i >> 6);
+}
+
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
@@ -136,10 +156,16 @@ __global__ __launch_bounds__(THREADS) void verify_stats_kernel(const Args a) {
     __shared__ float tops[THREADS / 64];
     __shared__ int32_t places[THREADS / 64];
     __shared__ double sums[THREADS / 64];
+    __shared__ Table table;
     const int row = blockIdx.x / a.blocks, part = blockIdx.x - row * a.blocks, at = part * BLOCK, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float x[PER];
     load(a.logits + row * a.ld, at, a.vocab, -INFINITY, x);
+    fill(table);
     const double sharp = sharpness(a, seq_of(a, row));
+    if (part == 0 && threadIdx.x == 0) {  // (what no sequence has work for says nothing)
+        a.emit[row] = -1;
+        if (a.src) a.src[row] = a.dst[row] = -1;
+    }
     float top = -INFINITY;
     bool nan = false;
 #pragma unroll
@@ -167,7 +193,7 @@ __global__ __launch_bounds__(THREADS) void verify_stats_kernel(const Args a) {
     double sum = 0.0;
     if (sharp > 0.0 && top > -INFINITY && top < INFINITY) {
 #pragma unroll
-        for (int k = 0; k < PER; k++) sum += x[k] == -INFINITY ? 0.0 : exp2_64(((double)x[k] - (double)top) * sharp);
+        for (int k = 0; k < PER; k++) sum += x[k] == -INFINITY ? 0.0 : exp2_64(table, ((double)x[k] - (double)top) * (64.0 * sharp));
     }
     sum = wave_sum(sum);
     if (lane == 0) sums[wave] = sum;
@@ -179,35 +205,44 @@ __global__ __launch_bounds__(THREADS) void verify_stats_kernel(const Args a) {
     }
 }
 
+// A row's parts, the first 64 (of a vocabulary of 262,144 all) in the lanes' registers.
+struct Parts {
+    const Stat* stats;
+    Stat mine;
+    int blocks;
+    __device__ __forceinline__ Parts(const Args& a, int row) : stats(a.stats + (size_t)row * a.blocks), blocks(a.blocks) {
+        mine = stats[min((int)(threadIdx.x & 63), blocks - 1)];
+    }
+    __device__ __forceinline__ Stat at(int k) const { return k < 64 ? mine : stats[k]; }  // (of lane k % 64)
+};
+
 // A row from its parts, by one wave: its largest logit, where, and Z. False where it has no choice (NaN, infinity, nothing).
 struct Row {
     float max;
     int32_t at;
     double z;
 };
-__device__ __forceinline__ bool row_of(const Args& a, int row, double sharp, Row* out) {
+__device__ __forceinline__ bool row_of(const Parts& parts, double sharp, Row* out) {
     const int lane = threadIdx.x & 63;
-    const Stat* const stats = a.stats + (size_t)row * a.blocks;
     float top = -INFINITY;
     int where = 0x7fffffff;
     bool nan = false;
-    for (int k = lane; k < a.blocks; k += 64) {
-        const Stat s = stats[k];
+    for (int k = lane; k < parts.blocks; k += 64) {
+        const Stat s = parts.at(k);
         nan |= s.max != s.max;
         where = s.max > top ? s.at : s.max == top ? min(where, s.at) : where;
         top = fmaxf(top, s.max);
     }
+    const float mine = top;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float other = __shfl_xor(top, d);
-        const int its = __shfl_xor(where, d);
-        where = other > top ? its : other == top ? min(where, its) : where;
-        top = fmaxf(top, other);
-    }
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    where = mine == top ? where : 0x7fffffff;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) where = min(where, __shfl_xor(where, d));
     double z = 0.0;
     if (sharp > 0.0)
-        for (int k = lane; k < a.blocks; k += 64) {
-            const Stat s = stats[k];
+        for (int k = lane; k < parts.blocks; k += 64) {
+            const Stat s = parts.at(k);
             if (s.max > -INFINITY) z += s.sum * exp2_64(((double)s.max - (double)top) * sharp);
         }
     out->max = top, out->at = where, out->z = wave_sum(z);
@@ -215,7 +250,7 @@ __device__ __forceinline__ bool row_of(const Args& a, int row, double sharp, Row
 }
 
 // The first part in which the sum passes `goal`, by the workgroup's every wave alike, and the sum before it; the last part that
-// adds anything where none does (its rounding).
+// adds anything where none does (its rounding). `part(k)`: of lane k % 64.
 template <class F>
 __device__ __forceinline__ int find_block(const Args& a, double goal, F&& part, double* before) {
     const int lane = threadIdx.x & 63;
@@ -239,6 +274,24 @@ __device__ __forceinline__ int find_block(const Args& a, double goal, F&& part, 
     }
     *before = last_before;
     return last;
+}
+
+// A thread's 16 logits (or probabilities) one after the other, as a search among them needs them.
+__device__ __forceinline__ void load_run(const float* row, int at, int vocab, float fill, float (&x)[PER]) {
+#pragma unroll
+    for (int r = 0; r < PER; r += 4) {
+        const int i = at + (int)threadIdx.x * PER + r;
+        f4u v = {fill, fill, fill, fill};
+        if (i + 4 <= vocab) {
+            v = *(const f4u*)(row + i);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k < vocab) v[k] = row[i + k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[r + k] = v[k];
+    }
 }
 
 // The first token of a part in which the sum passes `goal`: weights w[k] of the tokens at + 16 tid + k. One workgroup.
@@ -271,33 +324,34 @@ __device__ __forceinline__ int find_token(int at, const double (&w)[PER], double
 }
 
 // A row's choice by u, of w. One workgroup; every thread gets it.
-__device__ __forceinline__ int choose(const Args& a, int row, double sharp, const Row& r, float u) {
+__device__ __forceinline__ int choose(const Args& a, const Table& table, const Parts& parts, int row, double sharp, const Row& r, float u) {
     if (sharp == 0.0) return r.at;
-    const Stat* const stats = a.stats + (size_t)row * a.blocks;
     const double goal = (double)u * r.z;
     double before;
     const int block = find_block(a, goal, [&](int k) {
-        const Stat s = stats[k];
+        const Stat s = parts.at(k);
         return s.max > -INFINITY ? s.sum * exp2_64(((double)s.max - (double)r.max) * sharp) : 0.0;
     }, &before);
-    const float* const x = a.logits + row * a.ld;
+    float x[PER];
+    load_run(a.logits + row * a.ld, block * BLOCK, a.vocab, -INFINITY, x);
     double w[PER];
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-        const int i = block * BLOCK + (int)threadIdx.x * PER + k;
-        const float l = i < a.vocab ? x[i] : -INFINITY;
-        w[k] = l == -INFINITY ? 0.0 : exp2_64(((double)l - (double)r.max) * sharp);
-    }
+    for (int k = 0; k < PER; k++) w[k] = x[k] == -INFINITY ? 0.0 : exp2_64(table, ((double)x[k] - (double)r.max) * (64.0 * sharp));
     return find_token(block * BLOCK, w, before, goal);
 }
 
 // Each row's choice, a workgroup a row.
 __global__ __launch_bounds__(THREADS) void verify_pick_kernel(const Args a) {
+    __shared__ Table table;
     const int row = blockIdx.x;
+    const float u = a.u[2 * row + 1];
+    const Parts parts(a, row);
+    fill(table);
+    __syncthreads();
     const double sharp = sharpness(a, seq_of(a, row));
     Row r;
-    const bool any = row_of(a, row, sharp, &r);
-    const int token = any ? choose(a, row, sharp, r, a.u[2 * row + 1]) : -1;
+    const bool any = row_of(parts, sharp, &r);
+    const int token = any ? choose(a, table, parts, row, sharp, r, u) : -1;
     if (threadIdx.x == 0) a.pick[row] = token;
 }
 
@@ -360,14 +414,6 @@ __device__ __forceinline__ Seq seq_part(const Args& a, int b) {
     return s;
 }
 
-// Tokens that no sequence has work for say nothing.
-__global__ __launch_bounds__(64) void verify_clear_kernel(const Args a) {
-    const int i = blockIdx.x * 64 + threadIdx.x;
-    if (i >= a.t.n) return;
-    a.emit[i] = -1;
-    if (a.src) a.src[i] = a.dst[i] = -1;
-}
-
 // Drafts without probabilities: from the rows' choices to the paths, a wave a sequence.
 __global__ __launch_bounds__(64) void verify_walk_kernel(const Args a) {
     const int b = blockIdx.x, lane = threadIdx.x;
@@ -383,9 +429,9 @@ __global__ __launch_bounds__(64) void verify_walk_kernel(const Args a) {
     const int choice = __shfl(pick, max(parent, 0));
     bool right = there && (lane == 0 || (parent >= 0 && choice == token && token >= 0));
     // of children that say the same, the first
-    for (int k = 0; k < s.news; k++) {
-        const int its_parent = __shfl(parent, k), its_token = __shfl(token, k);
-        if (k < lane && lane > 0 && its_parent == parent && its_token == token) right = false;
+    for (uint64_t left = __ballot(right) & ~1ull; left; left &= left - 1) {
+        const int k = __ffsll((unsigned long long)left) - 1, its_parent = __builtin_amdgcn_readlane(parent, k);
+        if (k < lane && its_parent == parent) right = false;
     }
     const uint64_t rights = __ballot(right);
     const uint64_t path = __ballot(there && (seen & ~rights) == 0 && (seen & 1));
@@ -398,6 +444,7 @@ __global__ __launch_bounds__(THREADS) void verify_accept_kernel(const Args a) {
     __shared__ double z[64];
     __shared__ float top[64];
     __shared__ int32_t at[64], fine[64];
+    __shared__ Table table;
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq s = seq_part(a, b);
     if (s.news == 0) {
@@ -405,38 +452,42 @@ __global__ __launch_bounds__(THREADS) void verify_accept_kernel(const Args a) {
         return;
     }
     const double sharp = sharpness(a, b);
+    // (what says whether a draft is kept is asked for before the rows are added up)
+    const size_t mine = (size_t)s.first + min(lane, s.news - 1);
+    const int t = lane + 1 < s.news ? a.tokens[mine + 1] : -1;
+    const bool drafted = t >= 0 && t < a.vocab;
+    const float logit = drafted ? a.logits[mine * a.ld + t] : 0.0f, likely = drafted ? a.draft[mine * a.draft_ld + t] : 0.0f;
+    const float u = a.u[2 * mine];
+    fill(table);
     for (int k = wave; k < s.news; k += THREADS / 64) {
         Row r;
-        const bool any = row_of(a, s.first + k, sharp, &r);
+        const bool any = row_of(Parts(a, s.first + k), sharp, &r);
         if (lane == 0) z[k] = r.z, top[k] = r.max, at[k] = r.at, fine[k] = any;
     }
     __syncthreads();
     bool kept = false;
-    if (lane + 1 < s.news && fine[lane]) {
-        const size_t row = (size_t)s.first + lane;
-        const int t = a.tokens[row + 1];
-        if (t >= 0 && t < a.vocab) {
-            const double w = exp2_64(((double)a.logits[row * a.ld + t] - (double)top[lane]) * sharp);
-            kept = sharp == 0.0 ? t == at[lane] : (double)a.u[2 * row] * (double)a.draft[row * a.draft_ld + t] * z[lane] < w;
-        }
+    if (drafted && fine[lane]) {
+        const double w = exp2_64(table, ((double)logit - (double)top[lane]) * (64.0 * sharp));
+        kept = sharp == 0.0 ? t == at[lane] : (double)u * (double)likely * z[lane] < w;
     }
     const uint64_t no = ~__ballot(kept);
     const int k = __ffsll((unsigned long long)no) - 1;  // (the last token has no successor that could be kept)
     const int row = s.first + k;
     const bool open = fine[k] && sharp > 0.0 && k + 1 < s.news;
     int next = -1;
-    if (fine[k] && !open) next = choose(a, row, sharp, Row{top[k], at[k], z[k]}, a.u[2 * row + 1]);
+    if (fine[k] && !open) next = choose(a, table, Parts(a, row), row, sharp, Row{top[k], at[k], z[k]}, a.u[2 * row + 1]);
     if (threadIdx.x == 0) a.ends[b] = End{z[k], top[k], row, next, open, k};
     if (wave == 0 && !open)
         put_path(a, b, s, ~0ull >> (63 - k), lane < s.news ? a.tokens[s.first + lane] : -1, next);
 }
 
 // max(0, w - Z q) of the tokens at + 16 tid + k of a sequence's last kept row
-__device__ __forceinline__ double left_over(float l, float q, double sharp, const End& e) {
-    return l == -INFINITY ? 0.0 : fmax(exp2_64(((double)l - e.max) * sharp) - e.z * (double)q, 0.0);
+__device__ __forceinline__ double left_over(const Table& table, float l, float q, double sharp, const End& e) {
+    return l == -INFINITY ? 0.0 : fmax(exp2_64(table, ((double)l - e.max) * (64.0 * sharp)) - e.z * (double)q, 0.0);
 }
 __global__ __launch_bounds__(THREADS) void verify_rest_kernel(const Args a) {
     __shared__ double sums[THREADS / 64];
+    __shared__ Table table;
     const int b = blockIdx.y, at = blockIdx.x * BLOCK;
     const End e = a.ends[b];
     if (!e.open) return;
@@ -444,9 +495,11 @@ __global__ __launch_bounds__(THREADS) void verify_rest_kernel(const Args a) {
     float x[PER], q[PER];
     load(a.logits + e.row * a.ld, at, a.vocab, -INFINITY, x);
     load(a.draft + e.row * a.draft_ld, at, a.vocab, 0.0f, q);
+    fill(table);
+    __syncthreads();
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < PER; k++) sum += left_over(x[k], q[k], sharp, e);
+    for (int k = 0; k < PER; k++) sum += left_over(table, x[k], q[k], sharp, e);
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
@@ -458,9 +511,14 @@ __global__ __launch_bounds__(THREADS) void verify_rest_kernel(const Args a) {
 
 // The token after a rejection, a workgroup a sequence.
 __global__ __launch_bounds__(THREADS) void verify_finish_kernel(const Args a) {
+    __shared__ Table table;
     const int b = blockIdx.x;
     const End e = a.ends[b];
     if (!e.open) return;
+    const Seq s = sequence_of(a, b);
+    const int lane = threadIdx.x & 63, said = lane < s.news ? a.tokens[s.first + lane] : -1;
+    fill(table);
+    __syncthreads();
     const double sharp = sharpness(a, b);
     const double* const rest = a.rest + (size_t)b * a.blocks;
     double all = 0.0;
@@ -472,19 +530,17 @@ __global__ __launch_bounds__(THREADS) void verify_finish_kernel(const Args a) {
         const double goal = (double)u * all;
         double before;
         const int block = find_block(a, goal, [&](int k) { return rest[k]; }, &before);
+        float x[PER], q[PER];
+        load_run(a.logits + e.row * a.ld, block * BLOCK, a.vocab, -INFINITY, x);
+        load_run(a.draft + e.row * a.draft_ld, block * BLOCK, a.vocab, 0.0f, q);
         double w[PER];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const int i = block * BLOCK + (int)threadIdx.x * PER + k;
-            w[k] = i < a.vocab ? left_over(a.logits[e.row * a.ld + i], a.draft[e.row * a.draft_ld + i], sharp, e) : 0.0;
-        }
+        for (int k = 0; k < PER; k++) w[k] = left_over(table, x[k], q[k], sharp, e);
         next = find_token(block * BLOCK, w, before, goal);
     } else {  // the drafts' probabilities are the target's own
-        next = choose(a, e.row, sharp, Row{(float)e.max, 0, e.z}, u);
+        next = choose(a, table, Parts(a, e.row), e.row, sharp, Row{(float)e.max, 0, e.z}, u);
     }
-    const Seq s = sequence_of(a, b);
-    const int lane = threadIdx.x & 63;
-    if (threadIdx.x < 64) put_path(a, b, s, ~0ull >> (63 - e.kept), lane < s.news ? a.tokens[s.first + lane] : -1, next);
+    if (threadIdx.x < 64) put_path(a, b, s, ~0ull >> (63 - e.kept), said, next);
 }
 
 }  // namespace
@@ -529,7 +585,6 @@ extern "C" int qh_verify(qh_ctx* ctx, void* stream, const float* logits, size_t 
     a.rest = (double*)(scratch + stats + ends);
     a.pick = (int32_t*)(scratch + stats + ends + rest);
     const hipStream_t s = (hipStream_t)stream;
-    launch_kernel(verify_clear_kernel, dim3((unsigned)((n + 63) / 64)), dim3(64), s, a);
     launch_kernel(verify_stats_kernel, dim3((unsigned)(a.blocks * n)), dim3(THREADS), s, a);
     if (draft) {
         launch_kernel(verify_accept_kernel, dim3((unsigned)seqs), dim3(THREADS), s, a);

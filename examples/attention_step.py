@@ -55,7 +55,8 @@ class Layer:
                   q, gate, kv=self.kv, slots=dev(self.slots(old + np.arange(n))))
         mid = torch.empty((n, HEADS * DIM), dtype=BF16, device="cuda")
         tree = TreeStep(n, dev([0, n]), dev([old]), self.table, n, None if masks is None else dev(masks, torch.int64))
-        self.gemm.tree_attn(stream, q, HEADS, self.kv, tree, mid, gate)
+        attend = self.gemm.chunk_attn if masks is None else self.gemm.tree_attn
+        attend(stream, q, HEADS, self.kv, tree, mid, gate)
         y = torch.empty((self.out.split(n), n, HIDDEN), dtype=torch.float32, device="cuda")
         splits = self.gemm.run(stream, n, self.out, mid, y)
         nxt = torch.empty((n, HIDDEN), dtype=BF16, device="cuda")
@@ -74,7 +75,7 @@ def main():
     layer = Layer(gemm, rng)
     tokens = lambda n: (dev(rng.standard_normal((n, HIDDEN)), BF16), torch.zeros((n, HIDDEN), device="cuda"))  # noqa: E731
     old = 0
-    for part in (64, 64, 5):  # a prompt of 133 tokens, up to 64 to a step
+    for part in (128, 5):  # a prompt of 133 tokens, in two chunks
         layer.step(*tokens(part), old, range(part))
         old += part
     # trees of the last accepted token and four drafted ones, 0 -> 1 -> 2 and 0 -> 3 -> 4: a token sees itself and its ancestors

@@ -15,6 +15,8 @@
  *   Gemm::block_stage (:675-680); the kernels the engine launches on the products' partials: add_rmsnorm and
  *   sum_parts (kernels/qwen.cu:57-80, :141-143), the LoRA epilogue (kernels/lora.cuh:52-113); and the trainer's
  *   dequant (kernels/qwen_train.cu:84-103).
+ * Beside the products: the paged, quantised cache and the attention of steps and prompts over it (qh_kv_*, qh_attn_prep, qh_tree_attn,
+ * qh_chunk_attn), the cache's pages among a server's sequences (qh_kv_plan, qh_kv_release) and the verification of drafts (qh_verify).
  */
 #ifndef QWENNY_HIP_H
 #define QWENNY_HIP_H
@@ -384,8 +386,10 @@ int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh
 
 /* A prompt's attention: qh_tree_attn for sequences of any number of new tokens (step->max_new: the most of one sequence;
  * n <= 2^20). mask must be NULL: a token sees the cached positions, itself and the step's tokens of its sequence before it.
- * Everything else as qh_tree_attn: the step's tokens are in the cache already, padding gets zeros, what does not fit NaN, rounding,
- * alignment, scratch. Sequences of one token may stand beside chunks of thousands. Launch only. */
+ * Everything else as qh_tree_attn: the step's tokens are in the cache already, padding gets zeros, what does not fit NaN, alignment,
+ * scratch, the same bits each time. Probabilities, values' scales and values times their scales are rounded to f16 each: a value's part
+ * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 of the largest such scale that the row sees. Sequences of one token may stand beside
+ * chunks of thousands. Launch only. */
 int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
                   float scale, const void* gate, void* out);
 
@@ -437,7 +441,8 @@ int qh_kv_plan(void* stream, const qh_kv_pool* pool, const int32_t* len, const i
  * tokens' slots (of the step's table, of pages of `page` tokens) together, -1 where nothing moves; new_len int32 [n_seq] (or NULL):
  * the positions then cached, len + 1 + count. A row with a NaN, an infinite largest logit or none that is finite, or whose temp is
  * negative or not finite, ends its sequence with next = -1. A sequence without tokens, or whose numbers do not fit (qh_tree), has
- * next = -1, count = 0, new_len = len; tokens of none get -1 everywhere. Sums are 64-bit. n_seq and max_new as qh_tree's;
+ * next = -1, count = 0, new_len = len; tokens of none get -1 everywhere. (It knows nothing of qh_kv_plan's `granted`:
+ * what it says of a sequence whose tokens got no slots is to be left aside, its len stays.) Sums are 64-bit. n_seq and max_new as qh_tree's;
  * it uses the context's scratch (calls on one context must not run concurrently on two streams). Launch only. */
 int qh_verify(qh_ctx* ctx, void* stream, const float* logits, size_t ld, size_t vocab, const qh_tree* step, int page,
               const int32_t* tokens, const float* draft, size_t draft_ld, const float* temp, const float* u,

@@ -6,8 +6,9 @@ mirror of the reference's `Mat` / `Gemm` runtime and checkpoint formats.
 """
 
 from .core import (SKINNY_MAX_M, AttnRows, Epi, Gemm, Graph, KvCache, KvFmt, KvPool, Mat, Quant, TreeStep, Wt, add_rmsnorm,
-                   attn_prep, dequant, kv_move, kv_plan, kv_read, kv_release, kv_write, lora_add, lora_silu, pack_dense_bf16, pack_dense_int8, pack_quant,
-                   packed_sizes, row_order, sum_parts, unpack_rows, unpack_rows_bf16)
+                   attn_prep, dequant, kv_move, kv_plan, kv_read, kv_release, kv_write, lora_add, lora_silu,
+                   pack_dense_bf16, pack_dense_int8, pack_quant, packed_sizes, row_order, sum_parts, unpack_rows,
+                   unpack_rows_bf16)
 
 __all__ = ["SKINNY_MAX_M", "AttnRows", "Epi", "Gemm", "Graph", "KvCache", "KvFmt", "KvPool", "Mat", "Quant", "TreeStep", "Wt",
            "add_rmsnorm", "attn_prep", "dequant", "kv_move", "kv_plan", "kv_read", "kv_release", "kv_write", "lora_add", "lora_silu",

@@ -2,8 +2,22 @@
 //
 // For each row (a token and one of its query heads) over the positions t up to its token's own:
 //   s_t = c q.k_t,  o = sum_t exp(s_t) v_t / sum_t exp(s_t),  then o * sigmoid(gate) where a gate is given,
-// with k_t = sk_t * (codes), v_t = sv_t * (codes). One pass over the cache for each 256 rows of a kv head: the running maximum
-// and sum of the softmax beside the unnormalised o, rescaled when the maximum grows.
+// with k_t = sk_t * (codes), v_t = sv_t * (codes). One pass over the cache for each 256 rows of a kv head (128 where there are few):
+// the running maximum and sum of the softmax beside the unnormalised o, rescaled when the maximum has grown by 2^15.
+//
+// Bound by the matrix instructions, 4 d operations for each row and position; the cache is read once for 256 rows of them (2 bytes of codes
+// for 1,024 operations: far below what memory gives, and neighbours read the same tiles from L2). So everything else goes beside the
+// products:
+//  - A wave has 64 rows: 64 x d outputs in accumulation registers, its queries and two blocks' scores in vector registers, 512 in all for
+//    d = 256, one wave for each SIMD. Scores are made as s^T = k q^T, so that a lane holds its row's: the softmax needs one
+//    exchange between two lanes, and its results are the next product's operands as they stand.
+//  - Four waves share a tile of 64 tokens in LDS, as f16 operands, two tiles in turn: codes come from memory a tile ahead, are
+//    made operands beside the score products, and one barrier a tile separates the two.
+//  - The rows are two sets of 32. While one's softmax runs, the other's products do: the second set's value products stand behind the next
+//    block's scores. With d = 256 a block of 32 tokens is 64 products of 32 cycles; 1,274 us of 1,647 at 2,048 tokens behind
+//    30,000 cached ones are the products alone (timed without the rest; the clock falls under them), 1,345 with their operands from LDS.
+// Measured at 24 heads over 4 of 256, int8: those 2,048 tokens 1.65 ms, 948 TFLOP/s (a large f16 product reaches about 1,200);
+// none cached 125 us; 131 tokens behind 120,000 676 us. The simplest form that was right: 4.0 ms, 266 us, 15.0 ms.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -142,7 +156,7 @@ __device__ __forceinline__ float sigmoid(float x) {
 constexpr int NO_EXP = -100;
 __device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? max(min(__builtin_amdgcn_frexp_expf(s), 126), NO_EXP) : NO_EXP; }
 
-// The sequences' places: first unit (of 256 rows of a kv head), first token and tokens.
+// The sequences' places: first unit (of ROWS rows of a kv head), first token and tokens.
 struct Plan {
     int32_t base[TREE_MAX_SEQS], first[TREE_MAX_SEQS], news[TREE_MAX_SEQS];
     int32_t sums[2][WAVES];
@@ -151,7 +165,7 @@ constexpr int REST_DISORDER = 1, REST_SOME = 2;  // starts are not in order; som
 
 constexpr int MAX_UNITS = 2048;  // units of a call that may be shared in equal parts
 
-// A unit: 256 rows of a sequence's kv head, and the tiles that they see.
+// A unit: up to ROWS rows of a sequence's kv head, and the tiles that they see.
 struct Unit {
     int b, first, old, head, row0, last, tiles;
 };
@@ -301,14 +315,17 @@ struct Shared {
 };
 
 // The rounds that unshared units take against equal parts, in tiles: equal parts cost the partial results' way through memory and a
-// second launch, about as much as JOIN_TILES.
+// second launch, about as much as JOIN_TILES. (12 mixed chunks of 32 x 128 and 2,048 tokens of 24 x 256, none cached, take 111 + 11 and 145 us with
+// 25; with 10 the second is shared too and takes 167, with 40 the first is not and takes 164. Cold.) No part is below PART_TILES.
+constexpr int JOIN_TILES = 25, PART_TILES = 4;
+// Tables up to so many tiles have units of 128 rows where 256 would be less than two for each workgroup: half the work at the end of the
+// last round, for tiles that are read for half the rows. (2,048 tokens, none cached: 125 us, 278 with 256 rows; behind 30,000 positions
+// a tile's work for 128 rows takes 0.7 of that for 256, and equal parts leave no last round to shorten.)
 constexpr int SHORT_TILES = 80;
-constexpr int JOIN_TILES = 25, PART_TILES = 4;  // (and no part is below PART_TILES)
 __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
     const int even = (all + parts - 1) / parts;
     return (units <= parts ? most : max(most, even + most / 2)) > even + JOIN_TILES;
 }
-
 
 // A lane's row's softmax: the reference m that scores are taken against (in powers of two), and the sums of 2^(score - m). A score
 // may come to m + 15, since f16 holds that; m is set 7 below a largest score, so that probabilities keep f16's full bits down to 2^-21
@@ -614,7 +631,7 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
         constexpr int r = decltype(set)::value;
         const float most = both_max(mx[r]);
         const bool none = m[r] == -INFINITY;
-        const float up = most * late > ROOM || (none && most > -INFINITY) 
+        const float up = most * late > ROOM || (none && most > -INFINITY)
                              ? (fabsf(most * late) < 0x1p30f ? floorf(most * late - BELOW) / late : most) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 16; k++) x[r][k] -= up;
@@ -857,7 +874,8 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
 }
 
 // The partial results of a unit that several parts have: a workgroup for 32 rows of it and 64 dimensions. The maxima's powers of two and
-// the units of the parts are joined; four parts' results are under way at once. Bound by their bytes.
+// the units of the parts are joined; four parts' results are under way at once. Bound by their bytes: 256 parts of 256 x 256 in 27 us
+// (a workgroup for all dimensions, two under way: 78).
 template <int D, int SETS>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     constexpr int ROWS = rows_of(SETS), AHEAD = 4, PIECES = 2;  // pieces of 8 dimensions that a wave has

@@ -5,8 +5,11 @@
 // the child that is its row's choice, while there is one. Drafts with probabilities q (chains): token t after row i is kept
 // where u0 q(t) Z < w(t); where it is not, the choice is among max(0, w - Z q) instead of w.
 // Everything behind the logits is 64-bit: in a flat distribution over 248,320 tokens a token's part of the sum is 4e-6 of it,
-// and an error of 1e-7 in a sum, as 32 bits leave it, would pick the neighbour once in a few dozen choices. (The vector units
-// take 64-bit products at the rate of 32-bit ones that are not packed; e^x is a polynomial of degree 11.)
+// and an error of 1e-7 in a sum, as 32 bits leave it, would pick the neighbour once in a few dozen choices.
+// One read of the logits leaves each 4,096 of them with a maximum and a sum (bound by the read, and at few rows by one workgroup's way
+// from its loads to its sum); what follows knows a row from those, reads a choice's 4,096 logits again and is bound by the chain of its trips
+// to memory. Kernel times over 248,320 tokens: 5 rows 6.9 us for the stats, 10.9 the choices, 3.4 the path; 64 rows 23.2 (63 MB, 2.7 TB/s),
+// 10.8, 4.1; 12 drafted chains of 5 17.6, 14.0 for the kept ones, 5.7 and 8.2 for the token after a rejection.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -79,7 +82,7 @@ __device__ __forceinline__ double exp2_64(double t) {
 }
 
 // The same where there are many: 2^(n / 64) by a table of 64 in LDS, the rest |x| <= ln 2 / 128 by four terms (what is left is below 4e-14).
-// 13 operations instead of 21: the logits' own reading is then as long.
+// 13 operations instead of 21: the stats of 64 rows take 23 us, with the other 28.
 struct Table {
     double pow2[64];
 };

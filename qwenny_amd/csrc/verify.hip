@@ -117,15 +117,16 @@ __device__ __forceinline__ double wave_scan(double v) {
     return v;
 }
 
-// The sequence of a token: the last that begins at or before it (starts in order), or -1.
+// The sequence of a token: the first within whose start and end it lies, or -1. (Where starts are not in order another may have it too, but
+// none that has work: that one begins below an earlier end.)
 __device__ __forceinline__ int seq_of(const Args& a, int token) {
     const int lane = threadIdx.x & 63;
-    int n = 0;
     for (int c = 0; c < a.t.n_seq; c += 64) {
-        const int b = c + lane;
-        n += __popcll(__ballot(b < a.t.n_seq && a.t.start[min(b, a.t.n_seq - 1)] <= token));
+        const int b = min(c + lane, a.t.n_seq - 1), end = a.t.start[b + 1];
+        const uint64_t in = __ballot(a.t.start[b] <= token && token < end && end <= a.t.n);
+        if (in) return min(c + __ffsll((unsigned long long)in) - 1, a.t.n_seq - 1);
     }
-    return n - 1;
+    return -1;
 }
 
 // The row's temperature as log2e / T, 0 where the likeliest token is wanted; negative: the row's sequence has none.

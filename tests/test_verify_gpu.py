@@ -288,6 +288,22 @@ def test_numbers_that_do_not_fit(gemm, start, lens, kinds):
                 assert got["next"][b] == want["next"][b] and np.array_equal(got["emit"][rows], want["emit"][rows])
 
 
+@pytest.mark.parametrize("draft", [False, True])
+def test_starts_that_go_back_into_a_sequence(gemm, draft):
+    """The sequences whose numbers fit keep their own temperatures, whoever else claims their tokens."""
+    c = Case([10, 0, 10, 10], 400, draft=draft, temps=(1.3, 0.2, 0.4, 0.8), sharp=1.0)
+    if not draft:
+        for i in range(1, 10):  # the first sequence's path goes through all of its rows
+            c.tokens[i] = _choose(_chances(c.logits[i - 1], c.temp[0]), c.u[i - 1, 1])
+    want = c.want()
+    c.start = np.array([0, 10, 5, 20, 30], np.int32)
+    got = {k: v.cpu().numpy() for k, v in c.run(gemm).items()}
+    for b, rows in ((0, slice(0, 10)), (3, slice(20, 30))):
+        assert got["next"][b] == want["next"][b] and got["count"][b] == want["count"][b]
+        assert np.array_equal(got["emit"][rows], want["emit"][rows])
+    assert (got["next"][1:3] == -1).all() and (got["emit"][10:20] == -1).all()
+
+
 def test_moves_without_tables(gemm):
     """Who wants no moves gives none; pages outside of any cache move nothing."""
     c = Case([4, 5], 300, tree=True)

@@ -550,18 +550,19 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
     auto put_scales = [&](Tile<D>& to, int t) INLINE {
         if (none) ks = vs = NAN;
         const bool whole = (t + 1) * KV_TILE <= all_see;
-        apart_next = apart_next || !whole || late > 1.0f || __any(!(vs < INFINITY));  // (and so for good: units then only grow)
-        if (UNLIKELY(!apart_next && __any(vs > __builtin_ldexpf(1.0f, ref_next)))) {
-            float most = vs;
+        apart_next = apart_next || !whole || late > 1.0f || __any(!(fabsf(vs) < INFINITY));  // (and so for good: units then only grow)
+        if (UNLIKELY(!apart_next && __any(fabsf(vs) > __builtin_ldexpf(1.0f, ref_next)))) {
+            float most = fabsf(vs);
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
             ref_next = __builtin_amdgcn_readfirstlane(max(ref_next, scale_exp(most)));
         }
-        // (Each wave writes them all: one that did it alone would be late for the others.) A value that is not finite goes by its token's
-        // score: what sees it is NaN, and nothing else.
-        to.key_scale[lane] = vs < INFINITY ? ks * key_factor : NAN;
-        to.value_scale[lane] = vs < INFINITY ? vs : 0.0f;
-        to.factor[lane] = apart_next ? (_Float16)1.0f : (_Float16)__builtin_ldexpf(vs, VALUE_EXP - ref_next);
+        to.key_scale[lane] = fabsf(vs) < INFINITY ? ks * key_factor : NAN;
+        to.value_scale[lane] = fabsf(vs) < INFINITY ? fabsf(vs) : 0.0f;
+        // (A tile's unwritten tokens may have any scale. Where the scales go to the probabilities, a negative one's sign stays with the value.
+        // 2^VALUE_EXP bounds nothing else; by selects instead the widest heads' kernel spills.)
+        const float most = apart_next ? 1.0f : 0x1p7f;
+        to.factor[lane] = (_Float16)__builtin_amdgcn_fmed3f(__builtin_ldexpf(vs, apart_next ? 250 : VALUE_EXP - ref_next), -most, most);
     };
     auto written = [&](int t) INLINE { return none ? 0 : min(old + news - t * KV_TILE, KV_TILE); };  // tokens of the tile
 

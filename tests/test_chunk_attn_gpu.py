@@ -44,7 +44,7 @@ class Chunk(Step):
                 # a probability is rounded to f16, and so are a value's scale and the value: 2^-11 of it each (where a row does not see all of
                 # a tile, only the probability times the scale is); or half of f16's smallest step relative to the largest scale that
                 # the row sees (the reference is at most twice that)
-                small = seen * 2.0**-25 * 2 * np.where(late, 0, vs).max(-1, keepdims=True) * TOP[self.kv.fmt] / l
+                small = seen * 2.0**-25 * 2 * np.where(late, 0, np.abs(vs)).max(-1, keepdims=True) * TOP[self.kv.fmt] / l
                 tol[mine, head] = (3 * 2.0**-11 + 4 * ds + (seen + 64) * 2.0**-23) * (p @ np.abs(v) / l) + small
         if self.gate is not None:
             sig = 1 / (1 + np.exp(-_f64(self.gate)))
@@ -107,6 +107,25 @@ def test_many_sequences(gemm, form):
     """As many sequences as a step takes: the plan's last places."""
     print("1024 sequences", flush=True)
     form([(b % 70, b % 3 if b % 100 else 80) for b in range(1024)], KvFmt.I8, 2, 1, 64, 64).check(gemm)
+
+
+@FORMS
+@pytest.mark.parametrize("fmt", list(KvFmt))
+@pytest.mark.parametrize("written", [False, True])
+@pytest.mark.parametrize("seqs", [[(16, 5)], [(300, 70), (0, 3), (1000, 130)]], ids=str)
+def test_negative_scales(gemm, form, fmt, written, seqs):
+    """Where nothing was written the cache may hold any; where a program wrote its own codes, scales of either sign."""
+    s = form(seqs, fmt, 8, 2, 128, 64, gate=True)
+    held = s.kv.scales.clone()
+    sign = torch.where(torch.rand(held.shape, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0).cuda()
+    if written:
+        s.kv.scales.copy_(held * sign)
+    else:
+        scales = Host(s.kv).scales
+        s.kv.scales.copy_(torch.where(torch.isfinite(held) & (held < 1e38), held, sign * 0.37))
+        every = np.concatenate(s.slots)
+        assert np.array_equal(Host(s.kv).scales[every], scales[every])
+    s.check(gemm)
 
 
 @pytest.mark.parametrize("fmt,seqs,h,j,d", [(KvFmt.I8, [(20001, 66)], 6, 1, 256), (KvFmt.E4M3, [(9000, 90)], 12, 2, 128),

@@ -17,7 +17,7 @@
 //    block's scores. With d = 256 a block of 32 tokens is 64 products of 32 cycles; 1,274 us of 1,647 at 2,048 tokens behind
 //    30,000 cached ones are the products alone (timed without the rest; the clock falls under them), 1,345 with their operands from LDS.
 // Measured at 24 heads over 4 of 256, int8: those 2,048 tokens 1.65 ms, 948 TFLOP/s (a large f16 product reaches about 1,200);
-// none cached 125 us; 131 tokens behind 120,000 676 us. The simplest form that was right: 4.0 ms, 266 us, 15.0 ms.
+// none cached 131 us; 131 tokens behind 120,000 606 us. The simplest form that was right: 4.0 ms, 266 us, 15.0 ms.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -319,7 +319,7 @@ struct Shared {
 // 25; with 10 the second is shared too and takes 167, with 40 the first is not and takes 164. Cold.) No part is below PART_TILES.
 constexpr int JOIN_TILES = 25, PART_TILES = 4;
 // Tables up to so many tiles have units of 128 rows where 256 would be less than two for each workgroup: half the work at the end of the
-// last round, for tiles that are read for half the rows. (2,048 tokens, none cached: 125 us, 278 with 256 rows; behind 30,000 positions
+// last round, for tiles that are read for half the rows. (2,048 tokens, none cached: 128 us, 278 with 256 rows; behind 30,000 positions
 // a tile's work for 128 rows takes 0.7 of that for 256, and equal parts leave no last round to shorten.)
 constexpr int SHORT_TILES = 80;
 __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
@@ -977,10 +977,15 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
     const int sets = most <= SHORT_TILES && units_of(2) < 2 * wgs ? 1 : 2;
     const uint64_t units = units_of(sets);
     // Work is shared in equal parts where units alone might leave compute units without: not where a table names few tiles, nor with many
-    // units. (Which it is to be the device decides, from the lengths.)
+    // units. (Which it is to be the device decides, from the lengths. What the step's own tokens see makes equal parts so long at least; where
+    // they then gain nothing for sure, a second launch and the count of the tiles are spared: 2,048 tokens of 24 x 256 with none cached take
+    // 131 us, 134 with them.)
     const uint64_t longest = most + UNIT_TILES;
+    const double tokens = (double)step->n, per_head = (double)q_heads / rows_of(sets);
+    const double least = per_head * tokens * (tokens / step->n_seq / (2 * KV_TILE) + UNIT_TILES) / std::min<uint64_t>(wgs, TREE_MAX_WGS);
+    const bool gains = longest > 2 * JOIN_TILES || (double)longest > least + JOIN_TILES;
     const size_t rows = rows_of(sets), slot = rows * kv->head_dim * 4 + rows * sizeof(f4);
-    if (most > JOIN_TILES && units <= MAX_UNITS && units * longest <= 0x7fffffff) {
+    if (gains && units <= MAX_UNITS && units * longest <= 0x7fffffff) {
         a.parts = (int32_t)std::min<uint64_t>({wgs, TREE_MAX_WGS, (PF_SK_PART_BYTES - TREE_MAX_WGS * sizeof(Cut)) / (2 * slot)});
         a.part = (float*)ctx_partials(ctx);
         a.part_rows = (f4*)((uint8_t*)a.part + 2 * a.parts * rows * kv->head_dim * 4);

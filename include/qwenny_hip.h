@@ -388,7 +388,7 @@ int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh
  * n <= 2^20). mask must be NULL: a token sees the cached positions, itself and the step's tokens of its sequence before it.
  * Everything else as qh_tree_attn: the step's tokens are in the cache already, padding gets zeros, what does not fit NaN, alignment,
  * scratch, the same bits each time. Probabilities, values' scales and values times their scales are rounded to f16 each: a value's part
- * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 of the largest such scale that the row sees. Sequences of one token may stand beside
+ * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 of the largest such scale that the row sees (at least 2^-100). Sequences of one token may stand beside
  * chunks of thousands. Launch only. */
 int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
                   float scale, const void* gate, void* out);
@@ -441,7 +441,7 @@ int qh_kv_plan(void* stream, const qh_kv_pool* pool, const int32_t* len, const i
  * tokens' slots (of the step's table, of pages of `page` tokens) together, -1 where nothing moves; new_len int32 [n_seq] (or NULL):
  * the positions then cached, len + 1 + count. A row with a NaN, an infinite largest logit or none that is finite, or whose temp is
  * negative or not finite, ends its sequence with next = -1. A sequence without tokens, or whose numbers do not fit (qh_tree), has
- * next = -1, count = 0, new_len = len; tokens of none get -1 everywhere. (It knows nothing of qh_kv_plan's `granted`:
+ * next = -1, count = 0, new_len = len; tokens of none get -1 everywhere; with n = 0 nothing is written. (It knows nothing of qh_kv_plan's `granted`:
  * what it says of a sequence whose tokens got no slots is to be left aside, its len stays.) Sums are 64-bit. n_seq and max_new as qh_tree's;
  * it uses the context's scratch (calls on one context must not run concurrently on two streams). Launch only. */
 int qh_verify(qh_ctx* ctx, void* stream, const float* logits, size_t ld, size_t vocab, const qh_tree* step, int page,

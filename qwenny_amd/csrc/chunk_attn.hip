@@ -421,7 +421,7 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
     auto load_places = [&](int t) INLINE {
         const int mine = min(t + lane, t_end - 1);
         const int page = a.table[(size_t)b * a.t.table_ld + (mine >> (a.kv.page_shift - 6))];
-        places = (uint32_t)((page * a.kv.heads + head) * 2 * page_tiles + (mine & (page_tiles - 1)));
+        places = (((uint32_t)page * a.kv.heads + head) * 2) * page_tiles + (mine & (page_tiles - 1));
         if (page < 0 || ((int64_t)page << a.kv.page_shift) >= a.kv.slots) places = NONE;
     };
     load_places(t_begin);

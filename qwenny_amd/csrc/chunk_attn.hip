@@ -97,6 +97,13 @@ __device__ __forceinline__ h4 operands(uint32_t a) {
 // before it in the same registers needs no wait.
 #define OPERANDS_READY() asm volatile("s_nop 1")
 #define PRODUCTS_READY() asm volatile("s_nop 15\n\ts_nop 3")
+// Of products that the compiler's own instructions read, the wait has the registers as its operands: no reader is moved before it. (Outputs are
+// read by assembly, `kept`, that stays behind it as it is.)
+template <int SETS>
+__device__ __forceinline__ void products_ready(f16 (&x)[SETS]) {
+    if constexpr (SETS == 1) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0]));
+    else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));
+}
 // (WAIT: where the compiler may fetch an operand from elsewhere right before. It does with D = 64, whose kernel has half the registers; a
 // test looks at what was built.)
 template <bool WAIT>
@@ -746,7 +753,7 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
         }
     };
     auto first_set = [&](const Tile<D>& tile, int t, int tb) INLINE {
-        PRODUCTS_READY();
+        products_ready(x);
         widen();
         each<16>([&](auto k) INLINE { relative(tile, tb, Set<0>{}, k); });
         mask(tile, t, tb, Set<0>{});

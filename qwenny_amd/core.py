@@ -227,6 +227,7 @@ class Gemm:
         """Attention of a prompt's tokens: tree_attn for sequences of any number of new tokens (`step`: a TreeStep without
         mask), single tokens beside chunks of thousands."""
         s = kv.head_dim ** -0.5 if scale is None else scale
+        _rows_bf16(step.c.n * q_heads * kv.head_dim, q=q, gate=gate, out=out)
         q, gate, out = _ptrs(q, gate, out)
         check(lib().qh_chunk_attn(self._ctx, _stream(stream), q, q_heads, kv.c, step.c, s, gate, out))
 
@@ -499,6 +500,21 @@ def _int32(**arrays):
     for name, t in arrays.items():
         if hasattr(t, "data_ptr") and t.dtype is not _INT32:
             raise ValueError(f"{name}: int32 needed, not {t.dtype}")
+
+
+_BF16 = None  # torch.bfloat16, likewise
+
+
+def _rows_bf16(n, **arrays):
+    """Refuses rows of queries, gates or outputs that are not bf16, not in one piece or less than n numbers."""
+    global _BF16
+    if _BF16 is None:
+        import torch
+
+        _BF16 = torch.bfloat16
+    for name, t in arrays.items():
+        if hasattr(t, "data_ptr") and (t.dtype is not _BF16 or t.numel() < n or not t.is_contiguous()):
+            raise ValueError(f"{name}: a contiguous bfloat16 tensor of {n} needed, not {t.dtype} of {t.numel()}")
 
 
 class KvFmt(IntEnum):

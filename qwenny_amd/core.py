@@ -641,9 +641,9 @@ _FLOAT32 = None  # torch.float32, likewise
 
 def _sized(name, t, n, dtype):
     """Refuses an array of a call that is missing, of another type, not in one piece or too short."""
-    if t is None or t.dtype is not dtype or t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} needed"
-                         + ("" if t is None else f", not {t.dtype} of {t.numel()}"))
+    if getattr(t, "dtype", None) is not dtype or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} needed, not "
+                         + (f"{t.dtype} of {t.numel()}" if hasattr(t, "numel") else type(t).__name__))
 
 
 def _verify_arrays(n, n_seq, vocab, logits, draft, tokens, u, temp, next, count, emit, src, dst, new_len):
@@ -655,8 +655,9 @@ def _verify_arrays(n, n_seq, vocab, logits, draft, tokens, u, temp, next, count,
     for name, t in (("logits", logits), ("draft", draft)):
         if t is None and name == "draft":
             continue
-        if t.dtype is not _FLOAT32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < n or t.shape[1] < vocab:
-            raise ValueError(f"{name}: float32 [{n}][{vocab}] with contiguous rows needed, not {t.dtype} {list(t.shape)}")
+        if getattr(t, "dtype", None) is not _FLOAT32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < n or t.shape[1] < vocab:
+            raise ValueError(f"{name}: float32 [{n}][{vocab}] with contiguous rows needed, not "
+                             + (f"{t.dtype} {list(t.shape)}" if hasattr(t, "shape") else type(t).__name__))
     for name, t in (("tokens", tokens), ("emit", emit), ("src", src), ("dst", dst)):
         if t is not None or name in ("tokens", "emit"):
             _sized(name, t, n, _INT32)
@@ -704,15 +705,19 @@ def kv_plan(stream, pool, len, add, n, start, slots, pos, granted, mask=None):
     pages that it lacks, and writes start int32 [n_seq + 1], slots and pos int32 [n] (with mask, a tree's positions), and
     granted int32 [n_seq] (0: no pages, its tokens' slots are -1)."""
     n_seq = pool.c.n_seq
-    for name, t, k in (("len", len, n_seq), ("add", add, n_seq), ("start", start, n_seq + 1), ("slots", slots, n), ("pos", pos, n),
-                       ("granted", granted, n_seq)):
-        if t.dtype is not _INT32 or t.numel() < k or not t.is_contiguous():
-            _sized(name, t, k, _INT32)
+    try:
+        for name, t, k in (("len", len, n_seq), ("add", add, n_seq), ("start", start, n_seq + 1), ("slots", slots, n), ("pos", pos, n),
+                           ("granted", granted, n_seq)):
+            if t.dtype is not _INT32 or t.numel() < k or not t.is_contiguous():
+                _sized(name, t, k, _INT32)
+    except AttributeError:  # (no tensor)
+        _sized(name, t, k, _INT32)
     if mask is not None:
         import torch
 
-        if mask.dtype not in (torch.int64, torch.uint64) or mask.numel() < n or not mask.is_contiguous():
-            raise ValueError(f"mask: a contiguous int64 or uint64 tensor of {n} needed, not {mask.dtype} of {mask.numel()}")
+        if getattr(mask, "dtype", None) not in (torch.int64, torch.uint64) or mask.numel() < n or not mask.is_contiguous():
+            raise ValueError(f"mask: a contiguous int64 or uint64 tensor of {n} needed, not "
+                             + (f"{mask.dtype} of {mask.numel()}" if hasattr(mask, "numel") else type(mask).__name__))
     len, add, mask, start, slots, pos, granted = _ptrs(len, add, mask, start, slots, pos, granted)
     check(lib().qh_kv_plan(_stream(stream), pool.c, len, add, mask, n, start, slots, pos, granted))
 

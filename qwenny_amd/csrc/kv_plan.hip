@@ -115,7 +115,7 @@ __device__ __forceinline__ void put_token(const Args& a, int i, int node, int64_
     const int64_t slot = (page << a.page_shift) + (at & ((1 << a.page_shift) - 1));
     a.slots[i] = granted && page >= 0 && page < a.pages ? (int32_t)slot : -1;
     int depth = node;
-    if (a.mask && node < 64) depth = max((int)__popcll(a.mask[i] & ~0ull >> (63 - node)) - 1, 0);
+    if (a.mask && node < 64) depth = (int)__popcll(a.mask[i] & ((1ull << node) - 1));  // (whether it sees itself or not)
     a.pos[i] = (int32_t)min(len + depth, (int64_t)0x7fffffff);
 }
 

@@ -426,20 +426,18 @@ __global__ __launch_bounds__(64) void verify_walk_kernel(const Args a) {
     const bool there = lane < s.news;
     const size_t i = (size_t)s.first + min(lane, s.news - 1);
     const int token = a.tokens[i], pick = a.pick[i];
-    // itself and its ancestors
-    const uint64_t seen = there ? (a.mask ? a.mask[i] | 1ull << lane : ~0ull) & ~0ull >> (63 - lane) : 0;
-    const uint64_t above = seen & ~(1ull << lane);
+    // its parent: the last that it sees before itself
+    const uint64_t above = (a.mask ? a.mask[i] : ~0ull) & ((1ull << lane) - 1);
     const int parent = above ? 63 - __clzll((long long)above) : -1;
     const int choice = __shfl(pick, max(parent, 0));
-    bool right = there && (lane == 0 || (parent >= 0 && choice == token && token >= 0));
-    // of children that say the same, the first
-    for (uint64_t left = __ballot(right) & ~1ull; left; left &= left - 1) {
-        const int k = __ffsll((unsigned long long)left) - 1, its_parent = __builtin_amdgcn_readlane(parent, k);
-        if (k < lane && its_parent == parent) right = false;
+    const bool right = there && parent >= 0 && choice == token && token >= 0;
+    // from the first token on to the child that says the choice, of equal ones the first
+    uint64_t path = 1;
+    int last = 0;
+    while (const uint64_t children = __ballot(right && parent == last)) {
+        last = __ffsll((unsigned long long)children) - 1;  // (behind its parent)
+        path |= 1ull << last;
     }
-    const uint64_t rights = __ballot(right);
-    const uint64_t path = __ballot(there && (seen & ~rights) == 0 && (seen & 1));
-    const int last = 63 - __clzll((long long)path);
     put_path(a, b, s, path, token, __shfl(pick, last));
 }
 

@@ -61,7 +61,8 @@ struct Args {
     Kv kv;
     TreeArrays t;
     const int32_t* table;  // [n_seq][table_ld]
-    float scale;           // softmax scale * log2(e)
+    float scale;           // softmax scale * log2(e), without its power of two:
+    int32_t scale_exp;
     int32_t parts;         // workgroups that the work may be shared among in equal parts; 0: each has a unit
     float* part;           // [2 parts][256 rows x D], as the lanes hold them, and of each row (maximum, sum, unit):
     f4* part_rows;         // [2 parts][256]
@@ -491,7 +492,8 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
     // Where queries reach 2^55, the rest of the power is left to the differences of scores (`late`): the scores themselves might be
     // infinite. All tiles are then taken apart.
     h8 q[SETS][D / 16];
-    float key_factor, late;
+    float late;
+    int key_exp;
     bool wide = false;
     {
         constexpr int LOW = -1000;
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
             });
         });
         auto alike = [&](float v) INLINE { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); };
-        key_factor = alike(fmaxf(__builtin_ldexpf(a.scale, min(most, 40)), 1e-37f));
+        key_exp = __builtin_amdgcn_readfirstlane(a.scale_exp + min(most, 40));
         late = alike(__builtin_ldexpf(1.0f, max(most - 40, 0)));
     }
 
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(THREADS, waves_of(D)) void chunk_attn_kernel(const 
             for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
             ref_next = __builtin_amdgcn_readfirstlane(max(ref_next, scale_exp(most)));
         }
-        to.key_scale[lane] = fabsf(vs) < INFINITY ? ks * key_factor : NAN;
+        to.key_scale[lane] = fabsf(vs) < INFINITY ? __builtin_ldexpf(ks * a.scale, key_exp) : NAN;
         to.value_scale[lane] = fabsf(vs) < INFINITY ? fabsf(vs) : 0.0f;
         // (A tile's unwritten tokens may have any scale. Where the scales go to the probabilities, a negative one's sign stays with the value.
         // 2^VALUE_EXP bounds nothing else; by selects instead the widest heads' kernel spills.)
@@ -978,7 +980,7 @@ extern "C" int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_hea
     a.t = TreeArrays{step->start, step->len, (int64_t)step->table_ld, a.kv.page_shift, (int)step->n, step->n_seq, step->max_new,
                      group};
     a.table = step->table;
-    a.scale = scale * 1.4426950408889634f;
+    a.scale = std::frexp(scale, &a.scale_exp) * 1.4426950408889634f;
     const uint64_t most = (step->table_ld * kv->page + KV_TILE - 1) / KV_TILE, wgs = (uint64_t)ctx_cus(ctx) * waves_of(kv->head_dim);
     // Units of 128 rows where there are less than two of 256 for each workgroup that runs at once, and none is long
     const int sets = most <= SHORT_TILES && units_of(2) < 2 * wgs ? 1 : 2;

@@ -388,8 +388,9 @@ int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh
  * n <= 2^20). mask must be NULL: a token sees the cached positions, itself and the step's tokens of its sequence before it.
  * Everything else as qh_tree_attn: the step's tokens are in the cache already, padding gets zeros, what does not fit NaN, alignment,
  * scratch, the same bits each time. Probabilities, values' scales and values times their scales are rounded to f16 each: a value's part
- * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 of the largest such scale that the row sees (at least 2^-100). Sequences of one token may stand beside
- * chunks of thousands. Launch only. */
+ * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 (QH_KV_E4M3, whose codes are larger: 2^-22) of the largest scale that the row
+ * sees (at least 2^-100) times the row's largest probability, where that is more. Sequences of one token may stand beside chunks of
+ * thousands. Launch only. */
 int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
                   float scale, const void* gate, void* out);
 

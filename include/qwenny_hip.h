@@ -390,7 +390,8 @@ int qh_tree_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh
  * scratch, the same bits each time. Probabilities, values' scales and values times their scales are rounded to f16 each: a value's part
  * of the sum is off by 3 * 2^-11 of itself, or by 2^-24 (QH_KV_E4M3, whose codes are larger: 2^-22) of the largest scale that the row
  * sees (at least 2^-100) times the row's largest probability, where that is more. Sequences of one token may stand beside chunks of
- * thousands. Launch only. */
+ * thousands. Which form of the kernel runs hangs on table_ld, since the lengths are on the device: the first chunks of prompts do well to have a
+ * narrow table (2,048 tokens of 24 x 256, none cached: 130 us with tables of up to 5,120 positions, 202 with wider ones). Launch only. */
 int qh_chunk_attn(qh_ctx* ctx, void* stream, const void* q, int q_heads, const qh_kv* kv, const qh_tree* step,
                   float scale, const void* gate, void* out);
 
@@ -420,8 +421,8 @@ int qh_kv_release(void* stream, const qh_kv_pool* pool, const int32_t* len);
  * add[b] new tokens (int32 [n_seq]; 0: none in this step). It takes the pages it lacks for len[b] + add[b] positions, the
  * sequences in turn; from the first for which there are not enough free pages on, those that need any get none. granted[b] (int32): 1,
  * or 0 where it got none or its numbers do not fit (negative, past its table): its tokens' slots are -1 then, its table and held as they
- * were. start int32 [n_seq + 1]: sums of add (a negative one counts as 0; no more than n). slots, pos int32 [n]: each token's slot and
- * position, len[b] and the number of tokens before it in its sequence, or with mask (u64 [n] as qh_tree's, sequences up to 64 tokens)
+ * were. start int32 [n_seq + 1]: sums of add (a negative one counts as 0), no more than n: what passes n is in no sequence of this
+ * step, though it has its pages, so n is to be no less than all of add. slots, pos int32 [n]: each token's slot and position, len[b] and the number of tokens before it in its sequence, or with mask (u64 [n] as qh_tree's, sequences up to 64 tokens)
  * of those that it sees before itself (no more than 2^31 - 1). Tokens from start[n_seq] on: slot -1, position 0. No page is given back: qh_kv_release
  * does that. Launch only. */
 int qh_kv_plan(void* stream, const qh_kv_pool* pool, const int32_t* len, const int32_t* add, const uint64_t* mask,

@@ -9,15 +9,18 @@
 // for 1,024 operations: far below what memory gives, and neighbours read the same tiles from L2). So everything else goes beside the
 // products:
 //  - A wave has 64 rows: 64 x d outputs in accumulation registers, its queries and two blocks' scores in vector registers, 512 in all for
-//    d = 256, one wave for each SIMD. Scores are made as s^T = k q^T, so that a lane holds its row's: the softmax needs one
-//    exchange between two lanes, and its results are the next product's operands as they stand.
+//    d = 256, one wave for each SIMD (and 11 to 13 more, a unit's numbers, that are put by in scratch memory while its loop runs). Scores are
+//    made as s^T = k q^T, so that a lane holds its row's: the softmax needs one exchange between two lanes, and its results are the next
+//    product's operands as they stand.
 //  - Four waves share a tile of 64 tokens in LDS, as f16 operands, two tiles in turn: codes come from memory a tile ahead, are
 //    made operands beside the score products, and one barrier a tile separates the two.
 //  - The rows are two sets of 32. While one's softmax runs, the other's products do: the second set's value products stand behind the next
 //    block's scores. With d = 256 a block of 32 tokens is 64 products of 32 cycles; 1,274 us of 1,647 at 2,048 tokens behind
 //    30,000 cached ones are the products alone (timed without the rest; the clock falls under them), 1,345 with their operands from LDS.
 // Measured at 24 heads over 4 of 256, int8: those 2,048 tokens 1.65 ms, 948 TFLOP/s (a large f16 product reaches about 1,200);
-// none cached 131 us; 131 tokens behind 120,000 606 us. The simplest form that was right: 4.0 ms, 266 us, 15.0 ms.
+// none cached 130 us (202 with a table of more than 5,120 positions, see SHORT_TILES); 131 tokens behind 120,000 607 us. The simplest form
+// that was right: 4.0 ms, 266 us, 15.0 ms. 2,048 tokens behind 29,952 of 32 heads over 8, int8: of 128 dimensions 1.32 ms, 788 TFLOP/s, of 64 0.79 ms,
+// 656 (a score's exponential takes as long whatever d is: at d = 64 a block's 32 take as many cycles as its 16 products).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -253,7 +256,8 @@ __device__ __forceinline__ Unit unit_at(const Args& a, const Plan& plan, int u, 
 }
 
 // What a unit takes beside its tiles, in tiles: queries in, outputs out, the first tile's way (24 x 256 in units of 128 rows: 14 us and
-// 3.1 a tile).
+// 3.1 a tile, which is 4.5 of them; shares by 4, 6 and 9: 12 mixed chunks of 32 x 128 118, 120 and 125 us, 131 tokens of 24 x 256 behind 120,000 604, 600
+// and 595, 2,048 behind 30,000 1,639, 1,643 and 1,638).
 constexpr int UNIT_TILES = 6;
 __device__ __forceinline__ int length(const Unit& v) { return v.tiles + UNIT_TILES; }
 
@@ -323,12 +327,19 @@ struct Shared {
 };
 
 // The rounds that unshared units take against equal parts, in tiles: equal parts cost the partial results' way through memory and a
-// second launch, about as much as JOIN_TILES. (12 mixed chunks of 32 x 128 and 2,048 tokens of 24 x 256, none cached, take 111 + 11 and 145 us with
-// 25; with 10 the second is shared too and takes 167, with 40 the first is not and takes 164. Cold.) No part is below PART_TILES.
+// second launch, about as much as JOIN_TILES. With equal parts always, 2,048 tokens of
+// 24 x 256, none cached, take 150 us instead of 127, of 32 x 128 132 instead of 111, of 32 x 64 75 instead of 68; without them, 12 mixed chunks of 32 x 128 take
+// 153 instead of 115, 300 tokens of 24 x 256 behind 2,000 143 instead of 76, of 32 x 64 74 instead of 53. Between them, where few units leave
+// most of the GPU idle, a difference of 25 tiles is too much to ask: behind 1,000 positions (16 to 21 tiles) 70 tokens of 24 x 256 take 82 us, and with
+// equal parts 48, 300 of 32 x 128 69 and 52, of 32 x 64 51 and 43. No part is below PART_TILES. (All warm.)
 constexpr int JOIN_TILES = 25, PART_TILES = 4;
 // Tables up to so many tiles have units of 128 rows where 256 would be less than two for each workgroup: half the work at the end of the
-// last round, for tiles that are read for half the rows. (2,048 tokens, none cached: 128 us, 278 with 256 rows; behind 30,000 positions
-// a tile's work for 128 rows takes 0.7 of that for 256, and equal parts leave no last round to shorten.)
+// last round, for tiles that are read for half the rows. It goes by what a table can hold, since the lengths are on the device: with a wider one short prompts
+// have units of 256 rows, too. In us, 128 rows against 256: 2,048 tokens of 24 x 256, 32 tiles in all 126 and 202, 48 237 and 278, 64 299 and 266, 80
+// 370 and 322, 112 508 and 433, 500 2,020 and 1,680; 512 tokens, 8 tiles 50 and 83, 48 113 and 103, 112 187 and 164. 32 x 128, 2,048 tokens, 32 tiles
+// 112 and 129, 48 204 and 179, 80 341 and 260; 512 tokens, 48 tiles 90 and 93, 112 156 and 145. 32 x 64, 2,048 tokens, 32 tiles 67 and 78, 80 156 and 157, 160
+// 300 and 282; 512 tokens, 80 tiles 79 and 91, 288 180 and 183. So the two cross between 32 and 64 tiles at d = 256 and 128, and between 80 and
+// 300 at d = 64. (Warm.)
 constexpr int SHORT_TILES = 80;
 __device__ __forceinline__ bool share(int units, int all, int most, int parts) {
     const int even = (all + parts - 1) / parts;

@@ -6,8 +6,8 @@
 // not pass the free pages. The list of free pages is a stack: a plan takes from its end, a release puts the same pages back
 // in the places that a plan took them from. Prefix sums over the sequences say where each one's part begins; which sequence
 // a page or a token belongs to is found in them by halving. Bound by the launch and a few trips to memory one after the other:
-// a step's arrays are small, and one workgroup has the sums in its LDS. (Kernel times: one sequence 2.8 us and its release 2.0; 1,000
-// sequences of 5 tokens with 4 of them released 10.2 and 4.0; 16 prompts 7.0 and 2.5.)
+// a step's arrays are small, and one workgroup has the sums in its LDS. (Kernel times, medians of a trace: one sequence 2.7 us and
+// its release 1.9; 1,000 sequences of up to 8 tokens 9.6 and 3.7; 16 prompts 7.0 and 2.4.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void kv_fill_kernel(const Args a) {
 }
 
 // A workgroup's threads: one for each sequence, and for each of `work` pages or tokens up to THREADS. A single sequence's plan and
-// release take 2.8 + 2.0 us so, 4.9 + 2.9 with 1,024 always.
+// release take 2.7 + 1.9 us so, 4.9 + 2.9 with 1,024 always.
 dim3 threads_for(const Args& a, size_t work) { return dim3((unsigned)std::min<size_t>(THREADS, (std::max<size_t>(a.n_seq, work) + 63) / 64 * 64)); }
 
 int pool_check(const char* who, const qh_kv_pool* p, Args* a) {

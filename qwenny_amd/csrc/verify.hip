@@ -8,8 +8,8 @@
 // and an error of 1e-7 in a sum, as 32 bits leave it, would pick the neighbour once in a few dozen choices.
 // One read of the logits leaves each 4,096 of them with a maximum and a sum (bound by the read, and at few rows by one workgroup's way
 // from its loads to its sum); what follows knows a row from those, reads a choice's 4,096 logits again and is bound by the chain of its trips
-// to memory. Kernel times over 248,320 tokens: 5 rows 6.9 us for the stats, 10.9 the choices, 3.4 the path; 64 rows 23.2 (63 MB, 2.7 TB/s),
-// 10.8, 4.1; 12 drafted chains of 5 17.6, 14.0 for the kept ones, 5.7 and 8.2 for the token after a rejection.
+// to memory. Kernel times over 248,320 tokens (medians of a trace): 5 rows 6.1 us for the stats, 11.2 the choices, 3.9 the path; 64 rows 23.0
+// (63 MB, 2.8 TB/s), 10.0, 3.9; 12 drafted chains of 5 16.4, 14.2 for the kept ones, 5.7 and 8.4 for the token after a rejection.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -62,8 +62,8 @@ struct Args {
     int32_t *next, *count, *emit, *src, *dst, *new_len;
 };
 
-// 2^t for t <= 0 to 2^-50 of it (the polynomial is e^x's series to its 11th power, |x| <= ln 2 / 2: the rest is below 7e-15;
-// measured 1e-15).
+// 2^t for t <= 0 to 1e-14 of it: the polynomial is e^x's series to its 11th power, |x| <= ln 2 / 2, of which the rest is 8.7e-15 of e^x at
+// most (at x = -ln 2 / 2), beside a few roundings of 2^-53.
 __device__ __forceinline__ double exp2_64(double t) {
     const double n = __builtin_rint(t), x = (t - n) * 0.69314718055994530942;
     double p = 1.0 / 39916800;
